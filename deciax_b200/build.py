@@ -14,6 +14,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -58,33 +60,28 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     LIB_DIR.mkdir(exist_ok=True)
     inc, lib = nccl_paths()
-    cmd = [
-        nvcc(),
-        *ARCH,
-        "-O3",
-        "-lineinfo",
-        "-std=c++17",
-        "-Xcompiler",
-        "-fPIC",
-        "-shared",
-        f"-I{INCLUDE}",
-        f"-I{inc}",
-        str(CSRC / "clef.cu"),
-        "-o",
-        str(LIB) + ".tmp",
-        f"-L{lib}",
-        "-l:libnccl.so.2",
-        f"-Xlinker=-rpath,{lib}",
-    ]
+    flags = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
+        flags.insert(1, "-Xptxas=-v")
+    units = sorted(CSRC.glob("*.cu"))
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [str(Path(tmp) / (u.stem + ".o")) for u in units]
+        with ThreadPoolExecutor(len(units)) as pool:  # one nvcc per translation unit
+            logs = list(pool.map(lambda uo: run([*flags, f"-I{INCLUDE}", f"-I{inc}", "-c", str(uo[0]), "-o", uo[1]]),
+                                 zip(units, objects)))
+        logs.append(run([*flags, "-shared", *objects, "-o", str(LIB) + ".tmp", f"-L{lib}", "-l:libnccl.so.2",
+                         f"-Xlinker=-rpath,{lib}"]))
+    if verbose:
+        sys.stderr.write("".join(logs))
+    os.replace(str(LIB) + ".tmp", LIB)
+    return LIB
+
+
+def run(cmd: list[str]) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr[-8000:]}")
-    if verbose:
-        sys.stderr.write(res.stderr)
-    os.replace(str(LIB) + ".tmp", LIB)
-    return LIB
+    return res.stderr
 
 
 if __name__ == "__main__":
