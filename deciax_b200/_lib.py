@@ -43,6 +43,8 @@ EXPORTS = (
     "clef_op_qk_norm_rope_noalloc",
     "clef_op_attention",
     "clef_op_gdn_core",
+    "clef_op_qk_norm_rope_axes",
+    "clef_op_attention_packed",
 )
 
 
@@ -128,7 +130,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise ImportError(f"{LIB_PATH} is not built; run `python -m deciax_b200.build`")
         lib = ctypes.CDLL(str(LIB_PATH))
-        vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+        vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
         sigs = {
             "clef_nccl_unique_id": [ctypes.c_char_p],
             "clef_create": [ctypes.POINTER(ClefConfigC), i32, i32, i32, ctypes.c_char_p, i32, ctypes.POINTER(vp)],
@@ -153,6 +155,10 @@ def load() -> ctypes.CDLL:
             "clef_op_qk_norm_rope_noalloc": [i32, vp, i32, i32, i32, i32, i32, f32, f32, vp, vp, f32, vp],
             "clef_op_attention": [i32, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp],
             "clef_op_gdn_core": [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp],
+            "clef_op_qk_norm_rope_axes": [i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i32,
+                                          ctypes.POINTER(ctypes.c_int32), i32, i32, i32, i32, i32, i32, f32, vp, vp, f32, vp],
+            "clef_op_attention_packed": [i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, i32,
+                                         i32, i32, f32, i32, vp],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)

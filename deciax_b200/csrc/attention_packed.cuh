@@ -1,0 +1,279 @@
+// Causal grouped-head attention over packed sequences: rows cu[s] .. cu[s+1]-1
+// of the operands are sequence s, and row i attends to the keys
+// max(start of its sequence, i - window + 1) .. i:
+//
+//   x_ij = cap(q_i . k_j / sqrt d),  cap(x) = softcap tanh(x / softcap) or x
+//   o_i  = sum_j exp(x_ij - m_i) v_j / sum_j exp(x_ij - m_i),  times sigmoid(gate_i)
+//
+// A query tile is 64 (128 on the tensor cores) consecutive rows of the packed
+// stream, whatever sequences they belong to: the rows' key ranges differ only
+// by their lower ends, which never decrease, so the tile walks one contiguous
+// key range and a row masks what is not its own.  Hundreds of short sequences
+// then cost no more tiles than one long one.
+//
+// Masked entries are excluded by selection, so scores of foreign keys may hold
+// anything.  Their values enter P.V times zero, which is not zero where a value
+// is infinite or NaN; a row whose result holds a NaN is therefore computed once
+// more from its own keys alone (attn_packed_redo), so that what a sequence
+// holds never reaches another.
+//
+// attn_packed_simt_kernel (here): FP32 products on the CUDA cores, any head
+// size to 256, any strides and alignment.  64 x 64 score tiles, 4 x 4 a
+// thread; queries, keys, values and P in shared memory as FP32.  It issues
+// 12 shared-memory wavefronts for 16 cycles of FMA in Q.K and 36 for 64 in
+// P.V, so the FMA pipe is the bound.
+#pragma once
+
+#include "common.cuh"
+
+namespace clef {
+
+template <typename T>
+struct AttnPackedArgs {
+  const T* q;
+  const T* k;
+  const T* v;
+  const T* gate;  // nullptr = no gate
+  T* out;
+  long long ldq, hsq, ldk, hsk, ldv, hsv, ldg, hsg, ldo, hso;  // token and head strides (elements)
+  const int32_t* cu;  // [n_seqs + 1]
+  int n_seqs, tokens, H, Hk, d;
+  float softcap;
+  int window;
+  int* status;
+};
+
+// The packed rows that belong to a sequence: [first, total).  Whatever cu
+// holds, the bounds lie inside the buffers.
+template <typename A>
+__device__ __forceinline__ void packed_extent(const A& a, int& first, int& total) {
+  total = min(a.cu[a.n_seqs], a.tokens);
+  first = max(a.cu[0], 0);
+}
+
+// First key of `row`: the start of its sequence (the last s with cu[s] <= row)
+// or the window's edge.  Inside [0, row] whatever cu holds.
+template <typename A>
+__device__ __forceinline__ int packed_first_key(const A& a, int row, int lo_seq, int hi_seq) {
+  while (lo_seq < hi_seq) {  // cu[lo_seq] <= row < cu[hi_seq + 1]
+    const int mid = (lo_seq + hi_seq + 1) >> 1;
+    if (a.cu[mid] <= row)
+      lo_seq = mid;
+    else
+      hi_seq = mid - 1;
+  }
+  const int start = min(max(a.cu[lo_seq], 0), row);
+  return a.window > 0 ? max(start, row - a.window + 1) : start;
+}
+
+__device__ __forceinline__ float packed_score(float x, float scale, float softcap) {
+  x *= scale;
+  return softcap > 0.f ? softcap * tanhf(x / softcap) : x;
+}
+
+// One row again from its own keys [lo, row] alone, by the whole block (NT
+// threads, d <= NT): chunks of NT keys, a key a thread for the scores, an
+// element a thread for P.V.  smem: 256 + 2 * NT floats.  For rows that came
+// out NaN; every thread of the block must call it.
+template <typename T, int NT>
+__device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int row, int lo, float* smem) {
+  float* sq = smem;            // [d]
+  float* sp = smem + 256;      // [NT]
+  float* red = smem + 256 + NT;  // [NT]
+  const int tid = threadIdx.x, hk = h / (a.H / a.Hk);
+  const T* q = a.q + row * a.ldq + h * a.hsq;
+  const T* k = a.k + hk * a.hsk;
+  const T* v = a.v + hk * a.hsv;
+  const float scale = rsqrtf(static_cast<float>(a.d));
+  for (int c = tid; c < a.d; c += NT) sq[c] = to_f32(q[c]);
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int k0 = lo; k0 <= row; k0 += NT) {
+    const int n = min(NT, row + 1 - k0);
+    __syncthreads();  // sq is staged; the last chunk's sp has been read
+    float x = -INFINITY;
+    if (tid < n) {
+      const T* kr = k + (k0 + tid) * a.ldk;
+      float s = 0.f;
+      for (int c = 0; c < a.d; ++c) s = fmaf(sq[c], to_f32(kr[c]), s);
+      x = packed_score(s, scale, a.softcap);
+    }
+    red[tid] = x;
+    __syncthreads();
+    for (int w = NT; w > 1;) {  // NT need not be a power of two
+      const int half = (w + 1) / 2;
+      if (tid + half < w) red[tid] = fmaxf(red[tid], red[tid + half]);
+      w = half;
+      __syncthreads();
+    }
+    const float mn = fmaxf(m, red[0]);
+    const float corr = m == mn ? 1.f : expf(m - mn);
+    m = mn;
+    sp[tid] = tid < n ? expf(x - mn) : 0.f;
+    __syncthreads();
+    l *= corr;
+    o *= corr;
+    for (int j = 0; j < n; ++j) {
+      l += sp[j];
+      if (tid < a.d) o = fmaf(sp[j], to_f32(v[(k0 + j) * a.ldv + tid]), o);
+    }
+  }
+  if (tid < a.d) {
+    float y = o / l;
+    if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + tid]));
+    a.out[row * a.ldo + h * a.hso + tid] = from_f32<T>(y);
+  }
+  __syncthreads();
+}
+
+template <int DP>
+struct AttnPackedSimtShape {
+  static constexpr int BQ = 64, BK = 64, LD = DP + 4, LDP = BK + 4;
+  static constexpr size_t SMEM = (2 * 64 * LD + 64 * DP + BQ * LDP) * sizeof(float);
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel(const __grid_constant__ AttnPackedArgs<T> a) {
+  using Sh = AttnPackedSimtShape<DP>;
+  constexpr int BQ = Sh::BQ, BK = Sh::BK, LD = Sh::LD, LDP = Sh::LDP, NC = DP / 64;
+  constexpr float LOG2E = 1.4426950408889634f;
+  extern __shared__ __align__(16) float simt_smem[];
+  float* sQ = simt_smem;
+  float* sK = sQ + BQ * LD;
+  float* sV = sK + BK * LD;
+  float* sP = sV + BK * DP;
+  __shared__ int s_lo[BQ];
+  __shared__ unsigned long long s_nan;
+
+  int first, total;
+  packed_extent(a, first, total);
+  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
+  const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
+  if (q_first >= q_end) return;  // no row of this tile belongs to a sequence
+  const int hk = h / (a.H / a.Hk);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  if (tid < BQ) {  // rows outside the sequences see no key
+    const int row = q0 + tid;
+    s_lo[tid] = row >= q_first && row < q_end ? packed_first_key(a, row, 0, a.n_seqs - 1) : row + 1;
+  }
+  if (tid == 0) s_nan = 0;
+  for (int i = tid; i < BQ * DP; i += 256) {
+    const int r = i / DP, c = i % DP;
+    sQ[r * LD + c] = q0 + r < q_end && c < a.d ? to_f32(a.q[(q0 + r) * a.ldq + h * a.hsq + c]) : 0.f;
+  }
+  __syncthreads();
+  int lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lo[i] = s_lo[ty * 4 + i];
+  const int k_begin = s_lo[q_first - q0];
+  const float scale = rsqrtf(static_cast<float>(a.d));
+  float m[4], l[4], o[4][4 * NC];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
+  }
+  for (int k0 = k_begin; k0 < q_end; k0 += BK) {
+    __syncthreads();  // the last tile has been read
+    for (int i = tid; i < BK * DP; i += 256) {
+      const int r = i / DP, c = i % DP;
+      const bool in = k0 + r < q_end && c < a.d;
+      sK[r * LD + c] = in ? to_f32(a.k[(k0 + r) * a.ldk + hk * a.hsk + c]) : 0.f;
+      sV[r * DP + c] = in ? to_f32(a.v[(k0 + r) * a.ldv + hk * a.hsv + c]) : 0.f;
+    }
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 4
+    for (int c = 0; c < DP; c += 4) {
+      float4 qf[4], kf[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * LD + c]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sK[(tx + 16 * j) * LD + c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = fmaf(qf[i].x, kf[j].x, s[i][j]);
+          s[i][j] = fmaf(qf[i].y, kf[j].y, s[i][j]);
+          s[i][j] = fmaf(qf[i].z, kf[j].z, s[i][j]);
+          s[i][j] = fmaf(qf[i].w, kf[j].w, s[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = q0 + ty * 4 + i;
+      float mt = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx + 16 * j;
+        s[i][j] = key >= lo[i] && key <= row ? packed_score(s[i][j], scale, a.softcap) * LOG2E : -INFINITY;
+        mt = fmaxf(mt, s[i][j]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, w));
+      const float mn = fmaxf(m[i], mt);
+      const float base = mn == -INFINITY ? 0.f : mn;  // no key of this row yet: every p is exp2(-inf) = 0
+      const float corr = exp2f(m[i] - base);
+      m[i] = mn;
+      float ps = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        sP[(ty * 4 + i) * LDP + tx + 16 * j] = p;
+        ps += p;
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
+      l[i] = l[i] * corr + ps;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) o[i][c] = corr == 0.f ? 0.f : o[i][c] * corr;
+    }
+    __syncwarp();  // a row's P is written and read by one half-warp
+#pragma unroll 2
+    for (int j = 0; j < BK; j += 4) {
+      float4 pf[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * LDP + j]);
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float4 vf = *reinterpret_cast<const float4*>(&sV[(j + jj) * DP + 64 * c + tx * 4]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
+            o[i][4 * c] = fmaf(p, vf.x, o[i][4 * c]);
+            o[i][4 * c + 1] = fmaf(p, vf.y, o[i][4 * c + 1]);
+            o[i][4 * c + 2] = fmaf(p, vf.z, o[i][4 * c + 2]);
+            o[i][4 * c + 3] = fmaf(p, vf.w, o[i][4 * c + 3]);
+          }
+        }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = q0 + ty * 4 + i;
+    if (row < q_first || row >= q_end) continue;
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < 4 * NC; ++c) {
+      const int col = 64 * (c / 4) + tx * 4 + (c & 3);
+      if (col >= a.d) continue;
+      float y = o[i][c] / l[i];
+      bad |= y != y;
+      if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + col]));
+      a.out[row * a.ldo + h * a.hso + col] = from_f32<T>(y);
+    }
+    if (bad) atomicOr(&s_nan, 1ULL << (ty * 4 + i));
+  }
+  __syncthreads();
+  for (unsigned long long rows = s_nan; rows; rows &= rows - 1) {
+    const int r = __ffsll(static_cast<long long>(rows)) - 1;
+    attn_packed_redo<T, 256>(a, h, q0 + r, s_lo[r], simt_smem);
+  }
+}
+
+}  // namespace clef

@@ -1,0 +1,554 @@
+// Packed causal attention (attention_packed.cuh) on the 5th-generation tensor
+// cores: bf16 operands with 16-byte aligned rows, head size a multiple of 8 up
+// to 256 (computed as 64, 128 or 256: TMA reads zeros past the head's end).
+//
+// One CTA = 128 consecutive packed rows of one query head:
+//   warp 0      TMA producer: the Q tile, then K and V tiles through one ring
+//               each, then the gate tile into the K stages.
+//   warp 1      issues tcgen05.mma: S_t = Q K_t^T into one of two TMEM
+//               buffers, then O += P_{t-1} V_{t-1}.
+//   the others  softmax: thread r owns query row r (two warps a row at D =
+//               256, half of each key tile apiece): mask, running maximum and
+//               sum, P back over its S buffer in tensor memory (D >= 128) or
+//               into shared memory, at the end O / l * sigmoid(gate).
+// Key tiles are aligned to the query tile's end, so the diagonal is the last
+// tile (the last two at 64 keys) and only tiles that reach below some row's
+// first key need a mask besides.  The maximum moves, and O is rescaled, only
+// when it grows by more than 2^8; a row that saw no key yet has O = 0 written
+// rather than scaled, so what foreign tiles left there is gone.
+//
+// Differs from attention_sm100.cuh in what bounds a row's keys, and in the
+// rounding: the sigmoid gate multiplies in FP32 and the result is rounded once.
+#pragma once
+
+#include "attention_packed.cuh"
+#include "attention_sm100.cuh"
+#include "common.cuh"
+
+namespace clef {
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+// Every store of this thread's bulk groups is complete, not only read.
+__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Tensor maps [d][head][row] with boxes of 64 x 1 x 64.
+struct AttnPackedMaps {
+  CUtensorMap q, k, v, gate, out;
+};
+
+// The last s in [0, n) with cu[s] <= row (cu[0] <= row), by a whole warp: 32 probes a round.
+__device__ __forceinline__ int packed_seq_warp(const int32_t* cu, int n, int row, int lane) {
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const int at = lane * step;
+    const unsigned hit = __ballot_sync(0xffffffffu, at < n && cu[lo + at] <= row);
+    const int j = hit ? 31 - __clz(hit) : 0;
+    lo += j * step;
+    n = min(step, n - j * step);
+  }
+  return lo;
+}
+
+template <int D>
+struct AttnPackedTcShape : AttnTcShape<D> {
+  using S = AttnTcShape<D>;
+  static constexpr int CTAS = D <= 128 ? 2 : 1;  // per SM: shared memory and 256 TMEM columns each
+  static_assert(CTAS * (S::SMEM + 1024) <= 228 * 1024, "shared memory");
+};
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcShape<D>::CTAS)
+    attn_packed_tc_kernel(const __grid_constant__ AttnPackedMaps maps,
+                          const __grid_constant__ AttnPackedArgs<__nv_bfloat16> a) {
+  using Sh = AttnPackedTcShape<D>;
+  constexpr int BQ = Sh::BQ, BK = Sh::BK, ATOMS = Sh::ATOMS, KST = Sh::KST;
+  constexpr uint32_t IDESC_QK = idesc_bf16_f32(BQ, BK);
+  constexpr uint32_t IDESC_PV = idesc_bf16_f32(BQ, D) | (1u << 16);  // B (V) is MN-major
+  constexpr float LOG2E = 1.4426950408889634f;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + Sh::Q_BYTES;          // KST stages
+  uint8_t* sV = sK + KST * Sh::KV_BYTES;   // KST stages
+  uint8_t* sP = sV + KST * Sh::KV_BYTES;   // 2 buffers (none when P lives in tensor memory)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + (Sh::P_TMEM ? 0 : 2 * Sh::P_BYTES));
+  uint64_t* qfull = bars;
+  uint64_t* kfull = bars + 1;
+  uint64_t* kempty = bars + 3;
+  uint64_t* vfull = bars + 5;
+  uint64_t* vempty = bars + 7;
+  uint64_t* sfull = bars + 9;
+  uint64_t* sfree = bars + 11;
+  uint64_t* pfull = bars + 13;
+  uint64_t* pempty = bars + 15;
+  uint64_t* ofull = bars + 17;
+  uint64_t* ofinal = bars + 18;
+  uint64_t* drain = bars + 19;
+  uint64_t* gfull = bars + 20;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* s_begin = abort_flag + 1;  // first key of the tile's first row
+  uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out NaN
+  float* xbuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);  // softmax parts' exchange
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int first, total;
+  packed_extent(a, first, total);
+  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
+  const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
+  if (q_first >= q_end) return;  // no row of this tile belongs to a sequence
+  const int hk = h / (a.H / a.Hk);
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&maps.q);
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+    for (int i = 0; i < 21; ++i) {
+      const bool softmax_arrives = (i >= 11 && i < 15);  // sfree[2], pfull[2]: one arrive per softmax thread
+      mbar_init(&bars[i], softmax_arrives ? 128 * Sh::NP : 1);
+    }
+    *abort_flag = 0;
+    s_nan[0] = s_nan[1] = s_nan[2] = s_nan[3] = 0u;
+    fence_barrier_init();
+    fence_async_smem();
+    // the query rows do not wait for the key range
+    mbar_arrive_expect_tx(qfull, Sh::Q_BYTES);
+    for (int at = 0; at < ATOMS; ++at)
+      for (int half = 0; half < 2; ++half)
+        tma_load_3d(sQ + at * (BQ * 128) + half * (64 * 128), &maps.q, qfull, at * 64, h, q0 + half * 64);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Sh::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 2) {
+    const int s = packed_seq_warp(a.cu, a.n_seqs, q_first, lane);
+    if (lane == 0) *s_begin = packed_first_key(a, q_first, s, s);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // key tiles end with the query tile (with its last row in use): tile t holds
+  // keys k_org + t BK .., the first of them possibly below the buffer (read as zero)
+  const int k_hi = q0 + (q_end - q0 + BK - 1) / BK * BK;
+  const int n = (k_hi - *s_begin + BK - 1) / BK;
+  const int k_org = k_hi - n * BK;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer ----------------
+      // K runs one tile ahead of V: a K stage frees when its QK^T is done,
+      // a V stage only after the (later) P.V that reads it.
+      int nk = 0, nv = 0;  // tiles whose K / V load has been issued
+      for (int i = 0; i <= n && !*abort_flag; ++i) {
+        if (i < n) {
+          const int s = i % KST;
+          if (!mbar_wait(&kempty[s], ((i / KST) & 1) ^ 1, a.status, kTimeoutAttention)) {
+            *abort_flag = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&kfull[s], Sh::KV_BYTES);
+          for (int at = 0; at < ATOMS; ++at)
+            for (int bx = 0; bx < BK / 64; ++bx)
+              tma_load_3d(sK + s * Sh::KV_BYTES + at * (BK * 128) + bx * (64 * 128), &maps.k, &kfull[s], at * 64, hk,
+                          k_org + i * BK + bx * 64);
+          nk = i + 1;
+        }
+        if (i >= 1) {
+          const int u = i - 1, s = u % KST;
+          if (!mbar_wait(&vempty[s], ((u / KST) & 1) ^ 1, a.status, kTimeoutAttention)) {
+            *abort_flag = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&vfull[s], Sh::KV_BYTES);
+          for (int at = 0; at < ATOMS; ++at)
+            for (int bx = 0; bx < BK / 64; ++bx)
+              tma_load_3d(sV + s * Sh::KV_BYTES + at * (BK * 128) + bx * (64 * 128), &maps.v, &vfull[s], at * 64, hk,
+                          k_org + u * BK + bx * 64);
+          nv = u + 1;
+        }
+      }
+      // Gate prefetch: once the last QK^T has consumed every K stage, load
+      // this tile's gate rows (128 x D) into them for the epilogue.
+      bool gate_issued = false;
+      if (a.gate && !*abort_flag && nk == n) {
+        bool free_ = true;
+        for (int t = max(0, n - KST); t < n; ++t)
+          free_ = free_ && mbar_wait(&kempty[t % KST], (t / KST) & 1, a.status, kTimeoutAttention);
+        if (free_) {
+          mbar_arrive_expect_tx(gfull, Sh::Q_BYTES);
+          for (int at = 0; at < ATOMS; ++at)
+            for (int half = 0; half < 2; ++half)
+              tma_load_3d(sK + at * (BQ * 128) + half * (64 * 128), &maps.gate, gfull, at * 64, h, q0 + half * 64);
+          gate_issued = true;
+        } else {
+          *abort_flag = 1;
+        }
+      }
+      // Every issued load must land before the CTA may exit.
+      mbar_wait(qfull, 0, a.status, kTimeoutDrain);
+      if (gate_issued) mbar_wait(gfull, 0, a.status, kTimeoutDrain);
+      for (int t = max(0, nk - KST); t < nk; ++t) mbar_wait(&kfull[t % KST], (t / KST) & 1, a.status, kTimeoutDrain);
+      for (int t = max(0, nv - KST); t < nv; ++t) mbar_wait(&vfull[t % KST], (t / KST) & 1, a.status, kTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (lane 0; the warp waits together) ----------------
+    const uint32_t q_addr = smem_u32(sQ);
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.status, kTimeoutAttention));
+    };
+    auto issue_pv = [&](int u) -> bool {
+      const int s = u & 1, vs = u % KST;  // S/P buffer, V stage
+      if (!wait(&vfull[vs], (u / KST) & 1)) return false;
+      const int live = total - (k_org + u * BK);  // value rows of this tile that belong to a sequence
+      if (live < BK) {
+        // rows behind the last sequence hold anything: zero times it is not zero
+        for (int i = max(live, 0) * 8 + lane; i < BK * 8; i += 32)
+          for (int at = 0; at < ATOMS; ++at)
+            *reinterpret_cast<uint4*>(sV + vs * Sh::KV_BYTES + at * (BK * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
+      }
+      if (!wait(&pfull[s], (u >> 1) & 1)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t v_addr = smem_u32(sV + vs * Sh::KV_BYTES);
+        if constexpr (Sh::P_TMEM) {
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)  // 16 keys of P = 8 TMEM columns
+            umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8,
+                         smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
+        } else {
+          const uint32_t p_addr = smem_u32(sP + s * Sh::P_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            umma_bf16(tmem + Sh::O_COL, smem_desc_k128(p_addr + kk * 32),
+                      smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
+        }
+        umma_commit(&vempty[vs]);
+        umma_commit(&pempty[s]);
+        umma_commit(ofull);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = wait(qfull, 0);
+    auto stopped = [&] { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };  // the same answer in every lane
+    for (int t = 0; ok && t < n; ++t) {
+      const int s = t & 1, ks = t % KST;  // S buffer, K stage
+      if (stopped() || !wait(&kfull[ks], (t / KST) & 1) || !wait(&sfree[s], ((t >> 1) & 1) ^ 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t k_addr = smem_u32(sK + ks * Sh::KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int at = kk >> 2, w = kk & 3;
+          umma_bf16(tmem + Sh::S_COL + s * BK, smem_desc_k128(q_addr + at * (BQ * 128) + w * 32),
+                    smem_desc_k128(k_addr + at * (BK * 128) + w * 32), IDESC_QK, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&kempty[ks]);
+        umma_commit(&sfull[s]);
+      }
+      __syncwarp();
+      if (t >= 1 && !issue_pv(t - 1)) {
+        ok = false;
+        break;
+      }
+    }
+    ok = ok && !stopped() && issue_pv(n - 1);
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      umma_commit(ofinal);
+      umma_commit(drain);
+      mbar_wait(drain, 0, a.status, kTimeoutDrain);
+    }
+  } else {
+    // ---------------- softmax / epilogue warps ----------------
+    // NP warps per TMEM lane quarter: part p of row r takes keys
+    // [p BKP, (p + 1) BKP) of every tile and O columns [p D/NP, (p + 1) D/NP).
+    // The parts exchange their tile maxima through shared memory (one
+    // barrier per tile); their row sums are added once, at the end.
+    constexpr int NP = Sh::NP, BKP = BK / NP, NWP = BKP / 32, NT = 128 * NP, DP = D / NP;
+    const int q4 = warp & 3;  // TMEM lane quarter
+    const int part = (warp - 2) >> 2;
+    const int c0 = part * BKP;  // this part's first key column within a tile
+    const int r = q4 * 32 + lane;
+    const int row = q0 + r;
+    const bool live = row >= q_first && row < q_end;
+    // first key of this row (none for a row outside the sequences), and over the warp's rows
+    int lo = row + 1;
+    {
+      const int w0 = max(q0 + q4 * 32, q_first), w1 = min(q0 + q4 * 32 + 31, q_end - 1);
+      if (w0 <= w1) {
+        const int s0 = packed_seq_warp(a.cu, a.n_seqs, w0, lane), s1 = packed_seq_warp(a.cu, a.n_seqs, w1, lane);
+        if (live) lo = packed_first_key(a, row, s0, s1);
+      }
+    }
+    const int lo_max = __reduce_max_sync(0xffffffffu, lo);
+    const uint32_t t_lane = static_cast<uint32_t>(q4 * 32) << 16;
+    const float scale = rsqrtf(static_cast<float>(a.d));
+    const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
+    float m = -INFINITY, l = 0.f;  // running max (log2 units, possibly stale by < 8) and this part's sum
+    bool ok = true;
+    // A failed wait sets `fail`.  With one part a warp leaves the loop at
+    // once; with several, never alone: the next tile's exchange barrier ORs
+    // the flags and every part leaves together.
+    bool fail = false;
+    for (int t = 0; t < n; ++t) {
+      const int s = t & 1;
+      const uint32_t ph = (t >> 1) & 1;
+      const int k0 = k_org + t * BK + c0;  // first key of this part
+      if (!fail) {
+        const bool ready = mbar_wait(&sfull[s], ph, a.status, kTimeoutAttention);
+        __syncwarp();
+        fail = !__all_sync(0xffffffffu, ready);
+      }
+      if constexpr (NP == 1) {
+        if (fail) {
+          ok = false;
+          break;
+        }
+      }
+      tc_fence_after();
+      uint32_t sr[BKP];
+      if (!fail) {
+#pragma unroll
+        for (int w = 0; w < NWP; ++w)
+          tmem_ld32(tmem + t_lane + Sh::S_COL + s * BK + c0 + 32 * w, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * w]));
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&sfree[s]);
+      }
+      if constexpr (CAP) {
+#pragma unroll
+        for (int c = 0; c < BKP; ++c)
+          sr[c] = __float_as_uint(packed_score(__uint_as_float(sr[c]), scale, a.softcap));
+      }
+      if (k0 + BKP - 1 > q0 + q4 * 32 || k0 < lo_max) {  // some key of this part is masked for some row of the warp
+        const int top = row - k0, low = lo - k0;
+#pragma unroll
+        for (int c = 0; c < BKP; ++c) sr[c] = c >= low && c <= top ? sr[c] : 0xff800000u;  // -inf
+      }
+      // Row max with 8 independent partial maxima (short dependency chains).
+      float pm[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sr[e]);
+#pragma unroll
+      for (int c = 8; c < BKP; ++c) pm[c & 7] = fmaxf(pm[c & 7], __uint_as_float(sr[c]));
+      float mt = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
+      if constexpr (NP > 1) {
+        // both parts of a row end with the same maximum, bit for bit
+        xbuf[(s * NP + part) * 128 + r] = mt;
+        if (bar_red_or(1, NT, fail)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) mt = fmaxf(mt, xbuf[(s * NP + p) * 128 + r]);
+      }
+      const float mn = fmaxf(m, mt * scale_log2);
+      if (t == 0) {
+        m = mn;
+      } else {
+        // the parts of a row see the same m and mn, so they decide alike
+        const bool need = mn > m + 8.f;
+        if (__any_sync(0xffffffffu, need)) {
+          // O must hold P_{t-1} V_{t-1} before it is rescaled.
+          const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, done)) {
+            fail = true;
+            if constexpr (NP == 1) {
+              ok = false;
+              break;
+            } else {
+              continue;
+            }
+          }
+          tc_fence_after();
+          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);  // 0 for a row's first keys
+          m = mn;
+          l *= corr;
+#pragma unroll 1
+          for (int c = part * DP; c < (part + 1) * DP; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = corr == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st32(tmem + t_lane + Sh::O_COL + c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
+      const bool pe = mbar_wait(&pempty[s], ph ^ 1, a.status, kTimeoutAttention);
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, pe)) {
+        fail = true;
+        if constexpr (NP == 1) {
+          ok = false;
+          break;
+        } else {
+          continue;
+        }
+      }
+      const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
+      float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if constexpr (Sh::P_TMEM) {
+        // packed as bf16 pairs over the first BK/2 columns of its S buffer
+        // (key j in column j/2): this part's keys in columns [c0/2, (c0 + BKP)/2)
+#pragma unroll
+        for (int w = 0; w < NWP / 2; ++w) {
+          uint32_t pw[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int c = 64 * w + 2 * e;
+            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), scale_log2, neg_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), scale_log2, neg_m));
+            ps[c & 7] += p0;
+            ps[(c + 1) & 7] += p1;
+            pw[e] = pack_bf16x2(p0, p1);
+          }
+          tmem_st32(tmem + t_lane + Sh::S_COL + s * BK + c0 / 2 + 32 * w, pw);
+        }
+        tmem_wait_st();
+      } else {
+        // row r of the swizzled [128 x 64] P tile in shared memory (one part)
+        uint8_t* prow = sP + s * Sh::P_BYTES + r * 128;
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[ch * 8 + 2 * e]), scale_log2, neg_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[ch * 8 + 2 * e + 1]), scale_log2, neg_m));
+            ps[2 * e] += p0;
+            ps[2 * e + 1] += p1;
+            w[e] = pack_bf16x2(p0, p1);
+          }
+          *reinterpret_cast<uint4*>(prow + ((ch ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_async_smem();
+      }
+      l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+      tc_fence_before();
+      mbar_arrive(&pfull[s]);
+    }
+    ok = ok && !fail;
+    if (!ok) *abort_flag = 1;
+    if constexpr (NP > 1) {
+      // the row sum: the parts' sums, added in part order
+      float* lbuf = xbuf + 2 * NP * 128;
+      lbuf[part * 128 + r] = l;
+      asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");
+      l = 0.f;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) l += lbuf[p * 128 + r];
+    }
+    // ---------------- epilogue ----------------
+    // Phase 1: thread r forms its row (its part's columns) and writes it into
+    // the Q buffer (free: every MMA has completed once ofinal fires) in the
+    // TMA layout [atom][128 rows][128 B] with the 128-byte swizzle; the gate
+    // rows come from the same layout in the K stages.
+    const bool fin = ok && mbar_wait(ofinal, 0, a.status, kTimeoutAttention);
+    const bool have_gate = fin && a.gate && mbar_wait(gfull, 0, a.status, kTimeoutAttention);
+    __syncwarp();
+    if (__all_sync(0xffffffffu, fin && (have_gate || !a.gate))) {
+      tc_fence_after();
+      const float inv = 1.f / l;
+      bool bad = false;
+#pragma unroll 1
+      for (int c = part * DP; c < (part + 1) * DP; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int v4 = 0; v4 < 4; ++v4) {
+          const int chunk = (c >> 3) + v4;
+          const uint32_t off = (chunk >> 3) * (BQ * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
+            bad |= y[e] != y[e];
+          }
+          if (a.gate) {
+            const uint4 gq = *reinterpret_cast<const uint4*>(sK + off);
+            const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] *= sigmoid_fast(__uint_as_float(gw[e] << 16));
+              y[2 * e + 1] *= sigmoid_fast(__uint_as_float(gw[e] & 0xffff0000u));
+            }
+          }
+          *reinterpret_cast<uint4*>(sQ + off) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                           pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+        }
+      }
+      const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
+      if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
+    }
+    fence_async_smem();  // generic-proxy writes -> visible to the TMA engine
+    asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");  // every softmax warp
+    // Phase 2: a tile of sequence rows only leaves through TMA bulk stores;
+    // otherwise its rows leave through coalesced 16-byte stores, and rows
+    // outside the sequences stay as they were.
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    if (!*abort_flag) {
+      if (q_first == q0 && q_end == q0 + BQ) {
+        if (tid == 0) {
+          for (int at = 0; at < ATOMS && at * 64 < a.d; ++at)
+            for (int half = 0; half < 2; ++half)
+              tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
+          tma_store_commit();
+          // the staging buffer must outlive the copy; a row that is computed again must find it done
+          if (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3])
+            tma_store_wait_all();
+          else
+            tma_store_wait_read();
+        }
+      } else {
+        const int chunks = a.d / 8;
+        for (int idx = tid; idx < BQ * chunks; idx += NT) {
+          const int rr = idx / chunks, ch = idx % chunks;
+          if (q0 + rr < q_first || q0 + rr >= q_end) continue;
+          *reinterpret_cast<uint4*>(a.out + (q0 + rr) * a.ldo + h * a.hso + ch * 8) =
+              *reinterpret_cast<const uint4*>(sQ + (ch >> 3) * (BQ * 128) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, Sh::TMEM_COLS);
+  if (*abort_flag) return;
+  for (int w = 0; w < 4; ++w)
+    for (uint32_t rows = s_nan[w]; rows; rows &= rows - 1) {
+      const int row = q0 + w * 32 + __ffs(static_cast<int>(rows)) - 1;
+      attn_packed_redo<__nv_bfloat16, Sh::THREADS>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1),
+                                                   reinterpret_cast<float*>(sQ));
+    }
+}
+
+}  // namespace clef

@@ -1,0 +1,270 @@
+// Entry points of the packed-prompt operators: rotary positions with several
+// axes, causal attention over packed sequences, token log probabilities.
+// Declared in include/clef_b200.h beside the other single-kernel entry points.
+
+#include <algorithm>
+#include <cmath>
+#include <set>
+
+#include "attention_packed.cuh"
+#include "attention_packed_sm100.cuh"
+#include "common.cuh"
+#include "host.cuh"
+#include "rope_axes.cuh"
+
+using bf16 = __nv_bfloat16;
+
+namespace clef {
+
+// Runs an entry point's body; no exception leaves the C ABI.
+template <typename F>
+static int op_guarded(F&& f) {
+  try {
+    f();
+    return CLEF_OK;
+  } catch (const Error& e) {
+    set_global_error(e.what());
+    return e.code;
+  } catch (const std::exception& e) {
+    set_global_error(e.what());
+    return CLEF_EINVAL;
+  } catch (...) {
+    set_global_error("unknown failure");
+    return CLEF_EINVAL;
+  }
+}
+
+// A kernel that follows a host pointer, or one into another GPU's memory,
+// faults: refuse such a pointer before the launch.
+static void require_on_device(std::initializer_list<const void*> pointers) {
+  const int dev = current_device();
+  for (const void* p : pointers) {
+    if (!p) continue;
+    cudaPointerAttributes at{};
+    CUDA_CHECK(cudaPointerGetAttributes(&at, p));
+    REQUIRE((at.type == cudaMemoryTypeDevice && at.device == dev) || at.type == cudaMemoryTypeManaged,
+            "an operand is not in the current device's memory");
+  }
+}
+
+static int size_of(int dtype) {
+  REQUIRE(dtype == CLEF_DTYPE_BF16 || dtype == CLEF_DTYPE_F32, "dtype must be CLEF_DTYPE_BF16 or CLEF_DTYPE_F32");
+  return dtype == CLEF_DTYPE_BF16 ? 2 : 4;
+}
+
+static void rope_frequencies(RopeAxesArgs& a, int rot, double theta, int axes, const int32_t* sections,
+                             int interleaved) {
+  const int half = rot / 2;
+  a.half = half;
+  for (int i = 0; i < half; ++i) {
+    const long double turn = std::pow(static_cast<long double>(theta), static_cast<long double>(-2 * i) / rot) /
+                             6.283185307179586476925286766559L;
+    a.turn[i] = static_cast<unsigned long long>(std::ldexp(turn, 64));
+    a.axis[i] = 0;
+  }
+  if (axes == 1) return;
+  if (interleaved) {  // pair i turns with axis i % axes while that axis has pairs left, else with axis 0
+    for (int i = 0; i < half; ++i)
+      if (i / axes < sections[i % axes]) a.axis[i] = static_cast<unsigned char>(i % axes);
+  } else {
+    int i = 0;
+    for (int ax = 0; ax < axes; ++ax)
+      for (int n = 0; n < sections[ax]; ++n) a.axis[i++] = static_cast<unsigned char>(ax);
+  }
+}
+
+template <typename T>
+static void rope_axes(const RopeAxesArgs& a, cudaStream_t st) {
+  const long long items = static_cast<long long>(a.tokens) * (a.heads[0] + a.heads[1]);
+  rope_axes_any_kernel<T><<<static_cast<int>((items + 7) / 8), 256, 8 * a.d * sizeof(float), st>>>(a);
+  CUDA_CHECK(cudaGetLastError());
+}
+
+// bf16 [tokens][heads][d] with token stride ld and head stride hs: boxes of 64
+// elements of one head x 64 tokens, 128-byte swizzle, zeros outside.
+static CUtensorMap tmap_bf16_heads(const void* ptr, int tokens, int heads, int d, long long ld, long long hs) {
+  CUtensorMap m;
+  if (heads == 1) hs = (d + 7) / 8 * 8;  // never stepped
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[3] = {64, 1, 64};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, es,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(CLEF_EINVAL, "cuTensorMapEncodeTiled rejected an attention operand");
+  return m;
+}
+
+// Dynamic shared memory beyond the default is a per-device attribute of a kernel.
+template <typename K>
+static void allow_smem(K kern, size_t bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  const std::pair<int, const void*> key{current_device(), reinterpret_cast<const void*>(kern)};
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count(key)) return;
+  CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  done.insert(key);
+}
+
+template <typename T, int DP>
+static void launch_packed_simt(const AttnPackedArgs<T>& a, cudaStream_t st) {
+  constexpr size_t smem = AttnPackedSimtShape<DP>::SMEM;
+  allow_smem(attn_packed_simt_kernel<T, DP>, smem);
+  attn_packed_simt_kernel<T, DP><<<dim3((a.tokens + 63) / 64, a.H), 256, smem, st>>>(a);
+  CUDA_CHECK(cudaGetLastError());
+}
+
+template <int D, bool CAP>
+static void launch_packed_tc(const AttnPackedMaps& maps, const AttnPackedArgs<bf16>& a, cudaStream_t st) {
+  using Sh = AttnPackedTcShape<D>;
+  allow_smem(attn_packed_tc_kernel<D, CAP>, Sh::SMEM);
+  attn_packed_tc_kernel<D, CAP><<<dim3((a.tokens + 127) / 128, a.H), Sh::THREADS, Sh::SMEM, st>>>(maps, a);
+  CUDA_CHECK(cudaGetLastError());
+}
+
+template <typename T>
+static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    // TMA needs 16-byte aligned rows; everything else runs on the CUDA cores
+    const auto rows = [](const void* p, long long ld, long long hs, int heads) {
+      return !p || (aligned16(p) && ld > 0 && ld % 8 == 0 && (heads == 1 || (hs > 0 && hs % 8 == 0)));
+    };
+    if (a.d % 8 == 0 && rows(a.q, a.ldq, a.hsq, a.H) && rows(a.k, a.ldk, a.hsk, a.Hk) && rows(a.v, a.ldv, a.hsv, a.Hk) &&
+        rows(a.gate, a.ldg, a.hsg, a.H) && rows(a.out, a.ldo, a.hso, a.H)) {
+      AttnPackedMaps maps;
+      maps.q = tmap_bf16_heads(a.q, a.tokens, a.H, a.d, a.ldq, a.hsq);
+      maps.k = tmap_bf16_heads(a.k, a.tokens, a.Hk, a.d, a.ldk, a.hsk);
+      maps.v = tmap_bf16_heads(a.v, a.tokens, a.Hk, a.d, a.ldv, a.hsv);
+      maps.gate = a.gate ? tmap_bf16_heads(a.gate, a.tokens, a.H, a.d, a.ldg, a.hsg) : maps.q;
+      maps.out = tmap_bf16_heads(a.out, a.tokens, a.H, a.d, a.ldo, a.hso);
+      const bool cap = a.softcap > 0.f;
+      if (a.d <= 64)
+        cap ? launch_packed_tc<64, true>(maps, a, st) : launch_packed_tc<64, false>(maps, a, st);
+      else if (a.d <= 128)
+        cap ? launch_packed_tc<128, true>(maps, a, st) : launch_packed_tc<128, false>(maps, a, st);
+      else
+        cap ? launch_packed_tc<256, true>(maps, a, st) : launch_packed_tc<256, false>(maps, a, st);
+      return;
+    }
+  }
+  if (a.d <= 64)
+    launch_packed_simt<T, 64>(a, st);
+  else if (a.d <= 128)
+    launch_packed_simt<T, 128>(a, st);
+  else
+    launch_packed_simt<T, 256>(a, st);
+}
+
+}  // namespace clef
+
+extern "C" {
+
+int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
+                             const void* v, int64_t ldv, int64_t hsv, const void* gate, int64_t ldg, int64_t hsg, void* out,
+                             int64_t ldo, int64_t hso, const int32_t* cu_seqlens, int n_seqs, int tokens, int hq, int hkv,
+                             int d, float softcap, int window, void* stream) {
+  using namespace clef;
+  return op_guarded([&] {
+    size_of(dtype);
+    REQUIRE(n_seqs >= 0 && tokens >= 0, "sequences and tokens must not be negative");
+    REQUIRE(tokens <= 1 << 30, "at most 2^30 tokens");
+    REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be a multiple of key/value heads");
+    REQUIRE(hq <= 65535, "at most 65535 query heads");
+    REQUIRE(d > 0 && d <= 256, "attention head size must be in [1, 256]");
+    REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must not be negative (0 = off)");
+    REQUIRE(window >= 0, "window must not be negative (0 = off)");
+    if (n_seqs == 0 || tokens == 0) return;
+    REQUIRE(q && k && v && out && cu_seqlens, "null operand");
+    const auto rows = [&](int heads, int64_t ld, int64_t hs) {
+      return (heads == 1 || hs >= d) && (tokens == 1 || ld >= d) && ld >= 0 && hs >= 0;
+    };
+    REQUIRE(rows(hq, ldq, hsq) && rows(hkv, ldk, hsk) && rows(hkv, ldv, hsv) && (!gate || rows(hq, ldg, hsg)) &&
+                rows(hq, ldo, hso),
+            "token and head strides must be at least head_dim");
+    require_on_device({q, k, v, gate, out, cu_seqlens});
+    auto call = [&](auto* type) {
+      using T = std::remove_pointer_t<decltype(type)>;
+      AttnPackedArgs<T> a{};
+      a.q = static_cast<const T*>(q);
+      a.k = static_cast<const T*>(k);
+      a.v = static_cast<const T*>(v);
+      a.gate = static_cast<const T*>(gate);
+      a.out = static_cast<T*>(out);
+      a.ldq = ldq, a.hsq = hsq, a.ldk = ldk, a.hsk = hsk, a.ldv = ldv, a.hsv = hsv;
+      a.ldg = ldg, a.hsg = hsg, a.ldo = ldo, a.hso = hso;
+      a.cu = cu_seqlens;
+      a.n_seqs = n_seqs;
+      a.tokens = tokens;
+      a.H = hq;
+      a.Hk = hkv;
+      a.d = d;
+      a.softcap = softcap;
+      a.window = window;
+      attention_packed<T>(a, static_cast<cudaStream_t>(stream));
+    };
+    if (dtype == CLEF_DTYPE_BF16)
+      call(static_cast<bf16*>(nullptr));
+    else
+      call(static_cast<float*>(nullptr));
+  });
+}
+
+int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
+                              void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, int64_t ldko, int64_t hsko,
+                              const int32_t* positions, int64_t ldp, int axes, const int32_t* sections, int interleaved,
+                              int tokens, int hq, int hkv, int d, int rot, float rope_theta, const void* q_norm,
+                              const void* k_norm, float eps, void* stream) {
+  using namespace clef;
+  return op_guarded([&] {
+    size_of(dtype);
+    REQUIRE(tokens >= 0 && hq >= 0 && hkv >= 0 && hq + hkv > 0, "tokens and heads must not be negative");
+    REQUIRE(hq <= 65536 && hkv <= 65536, "at most 65536 heads");
+    REQUIRE(d > 0 && d <= 2 * kRopeMaxHalf, "head_dim must be in [1, 256]");
+    REQUIRE(rot > 0 && rot % 2 == 0 && rot <= d, "invalid partial rotary dimension");
+    REQUIRE(std::isfinite(rope_theta) && rope_theta >= 1.f, "rope_theta must be at least 1");
+    REQUIRE(axes >= 1 && axes <= 8, "axes must be in [1, 8]");
+    if (axes > 1) {
+      REQUIRE(sections, "several axes need their sections");
+      long long sum = 0;
+      for (int i = 0; i < axes; ++i) {
+        REQUIRE(sections[i] >= 0 && sections[i] <= rot / 2, "a section must be in [0, rot / 2]");
+        REQUIRE(!interleaved || i == 0 || i + static_cast<long long>(axes) * (sections[i] - 1) < rot / 2,
+                "interleaved sections: an axis has more pairs than every axes-th one");
+        sum += sections[i];
+      }
+      REQUIRE(sum == rot / 2, "sections must add up to rot / 2 frequency pairs");
+    }
+    if (tokens == 0) return;
+    REQUIRE((hq == 0 || (q && q_out)) && (hkv == 0 || (k && k_out)) && positions, "null operand");
+    const auto rows = [&](int heads, int64_t ld, int64_t hs) {
+      return heads == 0 || ((heads == 1 || hs >= d) && (tokens == 1 || ld >= d) && ld >= 0 && hs >= 0);
+    };
+    REQUIRE(rows(hq, ldq, hsq) && rows(hq, ldqo, hsqo) && rows(hkv, ldk, hsk) && rows(hkv, ldko, hsko),
+            "token and head strides must be at least head_dim");
+    REQUIRE(axes == 1 || ldp >= tokens, "the positions' axis stride is below the token count");
+    REQUIRE(static_cast<long long>(tokens) * (hq + hkv) < (1LL << 33), "tokens * heads must be below 2^33");
+    require_on_device({hq ? q : nullptr, hq ? q_out : nullptr, hkv ? k : nullptr, hkv ? k_out : nullptr, positions,
+                       hq ? q_norm : nullptr, hkv ? k_norm : nullptr});
+    RopeAxesArgs a{};
+    a.x[0] = q, a.x[1] = k;
+    a.out[0] = q_out, a.out[1] = k_out;
+    a.w[0] = q_norm, a.w[1] = k_norm;
+    a.ldx[0] = ldq, a.ldx[1] = ldk, a.hsx[0] = hsq, a.hsx[1] = hsk;
+    a.ldo[0] = ldqo, a.ldo[1] = ldko, a.hso[0] = hsqo, a.hso[1] = hsko;
+    a.heads[0] = hq, a.heads[1] = hkv;
+    a.pos = positions;
+    a.ldp = ldp;
+    a.tokens = tokens;
+    a.d = d;
+    a.eps = eps;
+    rope_frequencies(a, rot, rope_theta, axes, sections, interleaved);
+    if (dtype == CLEF_DTYPE_BF16)
+      rope_axes<bf16>(a, static_cast<cudaStream_t>(stream));
+    else
+      rope_axes<float>(a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

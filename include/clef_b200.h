@@ -277,6 +277,58 @@ int clef_op_gdn_core(int dtype, const void* proj, int ldp, const void* conv, int
                      const void* dt_bias, const void* norm_w, void* out, int b, int s, int nh, int nv, int dh, float eps,
                      void* stream);
 
+/* ---- packed prompts (no counterpart in the reference) ----
+ * Sequences laid end to end instead of padded to a rectangle: positions that
+ * are given, attention that stays inside each sequence, and the language
+ * head's own answer.  Operands are device memory of the current device
+ * (anything else is CLEF_EINVAL); strides count elements; arithmetic is FP32
+ * with one rounding to the operand type at each store.  No call synchronises
+ * the host. */
+
+/* Per-head RMSNorm scaling by (1 + w), then rotate-half RoPE over the first
+ * `rot` of d elements at given positions, for hq query and hkv key heads of
+ * `tokens` rows in one launch:
+ *   out[i]         = y[i] cos A_i - y[i + rot/2] sin A_i       i < rot/2
+ *   out[i + rot/2] = y[i + rot/2] cos A_i + y[i] sin A_i
+ *   A_i = positions[axis(i)][token] * rope_theta^(-2i/rot)
+ * Head h of token t starts at q + t * ldq + h * hsq (k alike); the outputs have
+ * their own strides and either are the inputs (same pointer and strides) or do
+ * not overlap them.  positions: int32 [axes, tokens], row stride ldp, any
+ * value (angles are exact to far positions).  axes = 1..8: one row of
+ * positions for text, (time, height, width) for images and video.  sections:
+ * host array [axes], the frequency pairs of each axis, adding up to rot/2
+ * (read only when axes > 1).  interleaved = 0: the first sections[0] pairs
+ * turn with axis 0, the next sections[1] with axis 1, ...; 1: pair i turns with
+ * axis i % axes while that axis has pairs left, else with axis 0.  q_norm /
+ * k_norm [d], NULL = rotate without a norm.  d <= 256; hq or hkv may be 0, and
+ * tokens = 0 does nothing.  Differs from clef_op_qk_norm_rope at positions
+ * 0..s-1 by that call's intermediate bf16 roundings. */
+int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
+                              void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, int64_t ldko, int64_t hsko,
+                              const int32_t* positions, int64_t ldp, int axes, const int32_t* sections, int interleaved,
+                              int tokens, int hq, int hkv, int d, int rot, float rope_theta, const void* q_norm,
+                              const void* k_norm, float eps, void* stream);
+
+/* Causal grouped-head attention over packed sequences: rows cu_seqlens[i] ..
+ * cu_seqlens[i+1]-1 of every operand are sequence i (device int32 [n_seqs+1],
+ * not decreasing, cu_seqlens[n_seqs] <= tokens; a sequence may be empty), and a
+ * row attends to its own sequence's rows up to itself:
+ *   out = sigmoid(gate) * softmax(cap(q k^T / sqrt d)) v
+ * q, gate and out have hq heads, k and v hkv (hq % hkv == 0; query head h reads
+ * key head h / (hq / hkv)); head h of row t starts at p + t * ld + h * hs.  gate
+ * NULL = no gate; softcap > 0 caps scaled scores at softcap * tanh(x / softcap);
+ * window > 0 keeps the last `window` keys.  tokens = rows of the buffers: rows
+ * outside [cu_seqlens[0], cu_seqlens[n_seqs]) belong to no sequence, are not
+ * read as keys, may hold anything, and their out is left as it was.  Infinities
+ * and NaN of one sequence never reach another.  out must not overlap the
+ * inputs.  d <= 256; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
+ * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; anything
+ * else on the CUDA cores in FP32. */
+int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
+                             const void* v, int64_t ldv, int64_t hsv, const void* gate, int64_t ldg, int64_t hsg, void* out,
+                             int64_t ldo, int64_t hso, const int32_t* cu_seqlens, int n_seqs, int tokens, int hq, int hkv,
+                             int d, float softcap, int window, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

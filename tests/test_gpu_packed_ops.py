@@ -1,0 +1,437 @@
+"""Packed-prompt operators against plain 64-bit implementations.
+
+Tolerances are derived, not fitted.  u is half a step of the output type
+(bf16 2^-8 of the value's power of two, so at most 2^-8 relative; fp32 2^-24).
+
+* Rotary: y = x r (1 + w) carries a handful of FP32 roundings (sum of d squares
+  in 32 lanes: (d/32 + 5) 2^-24 relative on the mean, halved by the root; rsqrt
+  and three products: 4 * 2^-24), the angle at most 2^-24 of half a turn (so
+  pi 2^-24 on cos and sin) plus sincospi's 2 ulp, and the rotation two products
+  and a sum of |y_lo| + |y_hi|.  All together below 32 * 2^-24 (|y_lo| + |y_hi|);
+  a bf16 result adds u |out|.
+* Attention, with A = sum_j p_j |v_j| / l over a row's own keys: a score of d
+  products in FP32 is off by at most e = (d + 8) 2^-24 sum_c |q_c k_c| / sqrt d (and
+  as much again for sums that truncate, and for tanh under a cap), which moves
+  each p, and l, by that factor: 4 e A.  P rounded to bf16 (tensor cores) adds
+  2^-8 A; FP32 sums of n terms add n 2^-24 A; exponentials and the sigmoid are
+  good to 2^-21.  The store adds u |out|.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from deciax_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0**-24
+U = {"bf16": 2.0**-8, "fp32": U32}
+
+
+def lib():
+    return _lib.load()
+
+
+def code(dtype: str) -> int:
+    return _lib.DTYPE_BF16 if dtype == "bf16" else _lib.DTYPE_F32
+
+
+def torch_type(dtype: str):
+    import torch
+
+    return torch.bfloat16 if dtype == "bf16" else torch.float32
+
+
+def normal(g, *shape, dtype="bf16", std=1.0):
+    import torch
+
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(torch_type(dtype))
+
+
+def generator(seed):
+    import torch
+
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def stream():
+    import torch
+
+    return torch.cuda.current_stream().cuda_stream
+
+
+# --------------------------------------------------------------------------- rotary positions
+
+
+def run_rope(q, k, q_out, k_out, positions, sections, interleaved, rot, theta, q_norm, k_norm, eps=1e-6):
+    """q, k and outputs [tokens, heads, d] with any strides whose last is 1; positions [axes, tokens]."""
+    t, _, d = (q if q is not None else k).shape
+    args = []
+    for x in (q, k, q_out, k_out):
+        args += [None, 0, 0] if x is None else [x.data_ptr(), x.stride(0), x.stride(1)]
+    sec = (ctypes.c_int32 * len(sections))(*sections) if sections else None
+    status = lib().clef_op_qk_norm_rope_axes(
+        code("bf16" if (q if q is not None else k).element_size() == 2 else "fp32"), *args, positions.data_ptr(), positions.stride(0),
+        positions.shape[0], sec, int(interleaved), t, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0, d, rot, theta,
+        q_norm.data_ptr() if q_norm is not None else None, k_norm.data_ptr() if k_norm is not None else None, eps, stream())
+    _lib.check(status)
+
+
+def axis_of_pairs(sections, interleaved, half):
+    if not sections:
+        return [0] * half
+    if not interleaved:
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    n = len(sections)
+    return [i % n if i // n < sections[i % n] else 0 for i in range(half)]
+
+
+def rope_64(x, w, positions, sections, interleaved, rot, theta, eps=1e-6):
+    """(expected, scale of its rounding error), in 64 bits on the host."""
+    x = x.double().cpu().numpy()
+    half = rot // 2
+    y = x
+    if w is not None:
+        y = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * (1 + w.double().cpu().numpy())
+    axis = axis_of_pairs(sections, interleaved, half)
+    pos = positions.cpu().numpy().astype(np.longdouble)
+    theta = np.longdouble(np.float32(theta))
+    angle = pos[axis].T * theta ** (np.longdouble(-2) * np.arange(half) / rot)
+    cos, sin = np.cos(angle).astype(np.float64)[:, None], np.sin(angle).astype(np.float64)[:, None]
+    lo, hi = y[..., :half], y[..., half:rot]
+    out = np.concatenate((lo * cos - hi * sin, hi * cos + lo * sin, y[..., rot:]), -1)
+    size = np.abs(lo) + np.abs(hi)
+    return out, np.concatenate((size, size, np.abs(y[..., rot:])), -1)
+
+
+def assert_rope(got, expected, scale, dtype):
+    got = got.double().cpu().numpy()
+    tol = 32 * U32 * scale + (U["bf16"] * np.abs(expected) if dtype == "bf16" else 0) + 1e-30
+    worst = np.abs(got - expected) / tol
+    assert worst.max() <= 1, (worst.max(), np.unravel_index(worst.argmax(), worst.shape))
+
+
+ROPE_CASES = [
+    # tokens, hq, hkv, d, rot, sections, interleaved, first position
+    (1, 16, 8, 256, 64, None, False, 0),
+    (129, 16, 8, 256, 64, None, False, 0),
+    (37, 4, 2, 128, 128, (24, 20, 20), False, 70000),
+    (37, 4, 2, 128, 128, (24, 20, 20), True, 70000),
+    (50, 3, 1, 64, 32, (6, 5, 5), True, -1000),
+    (50, 3, 1, 96, 96, (16, 0, 16, 16), False, 5),
+    (9, 2, 2, 80, 20, (4, 6), False, 1 << 30),
+    (9, 2, 2, 30, 14, (5, 2), True, 123),
+    (3, 1, 1, 2, 2, None, False, 9),
+    (65, 32, 16, 128, 64, (16, 16), True, (1 << 31) - 70),
+    (300, 14, 2, 256, 256, None, False, 2000000),
+    (5, 0, 3, 64, 64, None, False, 11),
+    (5, 3, 0, 48, 16, None, False, 11),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("case", ROPE_CASES, ids=str)
+def test_rope_axes(case, dtype):
+    import torch
+
+    t, hq, hkv, d, rot, sections, interleaved, first = case
+    g = generator(t + d + rot)
+    q, k = normal(g, t, hq, d, dtype=dtype, std=3.0), normal(g, t, hkv, d, dtype=dtype)
+    qw, kw = normal(g, d, dtype=dtype, std=0.2), normal(g, d, dtype=dtype, std=0.2)
+    axes = len(sections) if sections else 1
+    pos = torch.stack([(torch.arange(t, device="cuda", dtype=torch.int64) // (1 + 3 * a) + first).clamp_(max=2**31 - 1)
+                       for a in range(axes)]).int()
+    qo, ko = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+    run_rope(q if hq else None, k if hkv else None, qo if hq else None, ko if hkv else None, pos, sections, interleaved, rot, 1e4, qw, kw)
+    for x, w, o in ((q, qw, qo), (k, kw, ko)):
+        if x.shape[1]:
+            assert_rope(o, *rope_64(x, w, pos, sections, interleaved, rot, 1e4), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,rot,shift", [(256, 64, 0), (128, 128, 0), (64, 32, 1), (40, 24, 4)])
+def test_rope_axes_in_place_on_a_packed_projection(d, rot, shift, dtype):
+    """The packed projection [q | gate per head, k, v] rotated in place, at a row
+    stride with slack and (shift) away from 16-byte boundaries: gate, v and the
+    slack keep their bits."""
+    import torch
+
+    hq, hkv, t = 4, 2, 33
+    width = 2 * hq * d + 2 * hkv * d
+    g = generator(d + shift)
+    buf = normal(g, t, width + 24, dtype=dtype)
+    before = buf.clone()
+    view = buf[:, shift : shift + width]
+    q, k = view[:, : 2 * hq * d].view(t, hq, 2 * d)[..., :d], view[:, 2 * hq * d : 2 * hq * d + hkv * d].view(t, hkv, d)
+    pos = torch.arange(t, device="cuda", dtype=torch.int32)[None] + 100
+    qw, kw = normal(g, d, dtype=dtype, std=0.2), normal(g, d, dtype=dtype, std=0.2)
+    qe, ke = rope_64(q, qw, pos, None, False, rot, 5e5), rope_64(k, kw, pos, None, False, rot, 5e5)
+    run_rope(q, k, q, k, pos, None, False, rot, 5e5, qw, kw)
+    assert_rope(q, *qe, dtype)
+    assert_rope(k, *ke, dtype)
+    touched = torch.zeros_like(buf, dtype=torch.bool)
+    tv = touched[:, shift : shift + width]
+    tv[:, : 2 * hq * d].view(t, hq, 2 * d)[..., :d] = True
+    tv[:, 2 * hq * d : 2 * hq * d + hkv * d] = True
+    assert torch.equal(buf[~touched], before[~touched])
+
+
+@pytest.mark.parametrize("d,rot", [(128, 64), (36, 12)])
+def test_rope_axes_without_norm_keeps_the_tail(d, rot):
+    import torch
+
+    g = generator(1)
+    q = normal(g, 17, 3, d)
+    pos = torch.randint(-(2**31), 2**31 - 1, (1, 17), generator=g, device="cuda").int()
+    out = torch.empty_like(q)
+    run_rope(q, None, out, None, pos, None, False, rot, 1e6, None, None)
+    assert_rope(out, *rope_64(q, None, pos, None, False, rot, 1e6), "bf16")
+    assert torch.equal(out[..., rot:], q[..., rot:])
+
+
+def test_rope_axes_zero_rows_and_infinities_stay_in_their_head():
+    """A zero head stays zero (eps), an infinite one spoils only itself."""
+    import torch
+
+    q = normal(generator(2), 4, 3, 128)
+    q[1, 1] = 0
+    q[2, 0, 5] = float("inf")
+    out, w = torch.empty_like(q), torch.zeros(128, dtype=torch.bfloat16, device="cuda")
+    pos = torch.arange(4, device="cuda", dtype=torch.int32)[None]
+    run_rope(q, None, out, None, pos, None, False, 64, 1e4, w, None)
+    assert (out[1, 1] == 0).all()
+    ok = torch.ones(4, 3, dtype=torch.bool, device="cuda")
+    ok[2, 0] = False
+    assert torch.isfinite(out[ok]).all() and out[2, 0].isnan().any()
+
+
+def test_rope_axes_refuses_host_memory():
+    import torch
+
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    pos = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="current device"):
+        run_rope(x, None, x, None, pos, None, False, 64, 1e4, None, None)
+
+
+def test_rope_axes_captured_and_replayed_on_another_stream():
+    import torch
+
+    g = generator(3)
+    q = normal(g, 40, 4, 128)
+    out, pos = torch.empty_like(q), torch.arange(40, device="cuda", dtype=torch.int32)[None].contiguous()
+    w = normal(g, 128, std=0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_rope(q, None, out, None, pos, None, False, 64, 1e4, w, None)
+    for shift in (0, 1000):
+        pos.copy_(torch.arange(40, device="cuda")[None] + shift)
+        graph.replay()
+        assert_rope(out, *rope_64(q, w, pos, None, False, 64, 1e4), "bf16")
+
+
+# --------------------------------------------------------------------------- packed attention
+
+
+def run_attention(q, k, v, gate, out, cu, softcap=0.0, window=0):
+    args = []
+    for x in (q, k, v, gate, out):
+        args += [None, 0, 0] if x is None else [x.data_ptr(), x.stride(0), x.stride(1)]
+    t, hq, d = q.shape
+    _lib.check(lib().clef_op_attention_packed(code("bf16" if q.element_size() == 2 else "fp32"), *args, cu.data_ptr(), cu.numel() - 1, t, hq,
+                                              k.shape[1], d, softcap, window, stream()))
+
+
+def attention_64(q, k, v, gate, bounds, softcap, window, rounded_p):
+    """{(first, end): (expected [rows, heads, d], tolerance before the store)} of each sequence, in 64 bits."""
+    import torch
+
+    hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
+    found = {}
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        if a == b:
+            continue
+        qs = q[a:b].double().transpose(0, 1)
+        ks, vs = (x[a:b].double().transpose(0, 1).repeat_interleave(hq // hkv, 0) for x in (k, v))
+        s = qs @ ks.transpose(1, 2) / d**0.5
+        e = (d + 8) * U32 * (qs.abs() @ ks.abs().transpose(1, 2)) / d**0.5
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        i = torch.arange(b - a, device="cuda")
+        ago = i[:, None] - i
+        seen = (ago >= 0) & ((ago < window) if window else True)
+        s = s.masked_fill(~seen, float("-inf"))
+        p = torch.softmax(s, -1)
+        e = torch.where(seen, e, 0).amax(-1, keepdim=True)
+        y, size = p @ vs, p @ vs.abs()
+        g = torch.sigmoid(gate[a:b].double().transpose(0, 1)) if gate is not None else 1.0
+        tol = (4 * e + (2.0**-8 if rounded_p else 0) + (b - a + 16) * U32 + 2.0**-21) * size * g
+        found[a, b] = (y * g).transpose(0, 1), tol.transpose(0, 1)
+    return found
+
+
+def check_attention(lens, hq, hkv, d, dtype="bf16", *, gate=True, softcap=0.0, window=0, layout="packed", lead=0, pad=0, qscale=1.0, seed=0,
+                    tensor_cores=True, spoil=None):
+    import torch
+
+    g = generator(seed + d + len(lens))
+    n = lead + sum(lens)
+    t = n + pad
+    bounds = [lead]
+    for x in lens:
+        bounds.append(bounds[-1] + x)
+    if layout in ("packed", "odd"):  # one projection [q | gate per head, k, v]; odd: off 16-byte boundaries
+        width, off = 2 * hq * d + 2 * hkv * d, 1 if layout == "odd" else 0
+        proj = normal(g, t, width + 8 + off, dtype=dtype)[:, off : off + width]
+        heads = proj[:, : 2 * hq * d].unflatten(1, (hq, 2 * d))
+        q, gt = heads[..., :d], heads[..., d:]
+        k = proj[:, 2 * hq * d : 2 * hq * d + hkv * d].unflatten(1, (hkv, d))
+        v = proj[:, 2 * hq * d + hkv * d :].unflatten(1, (hkv, d))
+        out = normal(g, t, hq, d, dtype=dtype)
+    elif layout == "heads":  # [heads, rows, d]
+        q, gt, k, v, out = (normal(g, h, t, d, dtype=dtype).transpose(0, 1) for h in (hq, hq, hkv, hkv, hq))
+    else:
+        q, gt, k, v, out = (normal(g, t, h, d, dtype=dtype) for h in (hq, hq, hkv, hkv, hq))
+    q.mul_(qscale)
+    for x in (q, gt, k, v):  # rows of no sequence hold anything
+        x[:lead] = float("nan")
+        x[n:] = float("inf")
+        x[n + 1 :] = float("nan")
+    spoiled = spoil(bounds, q, k, v) if spoil else ()
+    before = out.clone()
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    run_attention(q, k, v, gt if gate else None, out, cu, softcap, window)
+    assert torch.equal(out[:lead], before[:lead]) and torch.equal(out[n:], before[n:])
+    u = U[dtype]
+    for (a, b), (y, tol) in attention_64(q, k, v, gt if gate else None, bounds, softcap, window, tensor_cores and dtype == "bf16").items():
+        if (a, b) in spoiled:
+            continue
+        off = (out[a:b].double() - y).abs() / (tol + u * y.abs() + 1e-30)
+        assert off.max() <= 1, ((a, b), off.max().item(), (off.isnan().sum()).item(), np.unravel_index(off.argmax().item(), off.shape))
+    return out, bounds
+
+
+LENGTHS = {
+    "one": [1], "tile": [128], "small": [1, 31, 64], "empty": [0, 0, 5, 0, 130, 0], "ragged": [257, 1, 1, 300], "long": [700],
+    "many": [(7 * i * i + 3 * i) % 21 for i in range(120)],
+}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens", LENGTHS)
+def test_attention_packed_lengths(lens, d, dtype):
+    check_attention(LENGTHS[lens], 4, 2, d, dtype, pad=37 if lens != "tile" else 0)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 1), (6, 3), (14, 2)])
+@pytest.mark.parametrize("layout", ["packed", "heads", "split"])
+@pytest.mark.parametrize("gate", [True, False])
+def test_attention_packed_heads_and_strides(hq, hkv, layout, gate):
+    check_attention([100, 60, 33], hq, hkv, 128, gate=gate, layout=layout, pad=3, lead=5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [8, 40, 72, 96, 200])
+def test_attention_packed_other_head_sizes(d, dtype):
+    check_attention([140, 3, 77], 4, 2, d, dtype, layout="split", pad=60)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,layout", [(30, "packed"), (64, "odd"), (1, "split"), (255, "heads")])
+def test_attention_packed_unaligned_rows(d, layout, dtype):
+    check_attention([90, 0, 41], 4, 2, d, dtype, layout=layout, pad=2, tensor_cores=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window,softcap", [(1, 0.0), (50, 0.0), (200, 5.0), (0, 30.0), (1 << 30, 0.0)])
+def test_attention_packed_window_and_softcap(window, softcap, d, dtype):
+    check_attention([300, 17, 260], 2, 1, d, dtype, window=window, softcap=softcap, qscale=3.0, pad=1)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_packed_long_rows_with_large_scores(d):
+    """The running maximum moves often: O is rescaled in tensor memory."""
+    check_attention([1500, 20, 600], 2, 1, d, qscale=6.0)
+
+
+@pytest.mark.parametrize("dtype,tokens", [("bf16", 4500), ("fp32", 1100)])
+def test_attention_packed_benchmark_heads(dtype, tokens):
+    check_attention([tokens], 16, 8, 256, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
+def test_attention_packed_infinities_stay_in_their_sequence(dtype, d):
+    """Values and keys of the middle sequence are infinite or NaN: its rows from
+    there on are, and its earlier rows and every other sequence keep their values."""
+
+    def spoil(bounds, q, k, v):
+        a = bounds[1]
+        v[a + 20, 0, 3] = float("inf")
+        v[a + 25, :, :] = float("nan")
+        k[a + 30, 0, 0] = float("nan")
+        return [(bounds[1], bounds[2])]
+
+    out, bounds = check_attention([40, 35, 30, 100], 4, 2, d, dtype, spoil=spoil, pad=30)
+    a = bounds[1]
+    assert out[a : a + 20].isfinite().all()
+    assert (~out[a + 20 : bounds[2], :2, 3].isfinite()).all()
+    assert out[a + 20 : a + 25, 2:].isfinite().all() and out[a + 25 : bounds[2]].isnan().any(-1).all()
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("bf16", 30), ("fp32", 64)])
+def test_attention_packed_offsets_past_32_bits(dtype, d):
+    """The last rows of buffers of more than 2^31 elements."""
+    import torch
+
+    hq, ld = 2, 1 << 16
+    t = (1 << 31) // ld + 200
+    buf = torch.empty(t, ld, dtype=torch_type(dtype), device="cuda")
+    n, at = 150, t - 170
+    buf[at:] = normal(generator(4), t - at, ld, dtype=dtype)
+    q, k, v, out = (buf[:, i * hq * d : (i + 1) * hq * d].unflatten(1, (hq, d)) for i in range(4))
+    cu = torch.tensor([at, at + 100, at + n], dtype=torch.int32, device="cuda")
+    run_attention(q, k, v, None, out, cu)
+    for (a, b), (y, tol) in attention_64(q, k, v, None, [at, at + 100, at + n], 0.0, 0, d == 128).items():
+        assert ((out[a:b].double() - y).abs() <= tol + U[dtype] * y.abs()).all()
+
+
+def test_attention_packed_captured_and_replayed_with_other_lengths():
+    """The lengths are device data: a captured call follows them."""
+    import torch
+
+    g = generator(5)
+    q, k, v, out = (normal(g, 400, h, 128) for h in (4, 2, 2, 4))
+    cu = torch.tensor([0, 100, 400, 400], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_attention(q, k, v, None, out, cu)
+    for bounds in ([0, 100, 400, 400], [0, 1, 1, 333], [10, 200, 201, 390]):
+        cu.copy_(torch.tensor(bounds))
+        out.fill_(7)
+        graph.replay()
+        for (a, b), (y, tol) in attention_64(q, k, v, None, bounds, 0.0, 0, True).items():
+            assert ((out[a:b].double() - y).abs() <= tol + U["bf16"] * y.abs()).all()
+        assert (out[: bounds[0]] == 7).all() and (out[bounds[-1] :] == 7).all()
+
+
+def test_attention_packed_rows_do_not_depend_on_their_neighbours():
+    """Twice the same call gives the same bits, and so do two streams at once."""
+    import torch
+
+    g = generator(6)
+    q, k, v = (normal(g, 600, h, 256) for h in (4, 2, 2))
+    cu = torch.tensor([0, 250, 600], dtype=torch.int32, device="cuda")
+    outs = [torch.empty_like(q) for _ in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s, o in zip(streams, outs):
+        with torch.cuda.stream(s):
+            run_attention(q, k, v, None, o, cu)
+    torch.cuda.synchronize()
+    run_attention(q, k, v, None, outs[2], cu)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])

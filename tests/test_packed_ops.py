@@ -1,0 +1,77 @@
+"""Refusals of the packed-prompt operators: argument errors come back as
+CLEF_EINVAL before anything reaches a device, so they are checked without one."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from deciax_b200 import _lib
+from deciax_b200.build import build
+
+BF16, F32 = _lib.DTYPE_BF16, _lib.DTYPE_F32
+P = 4096  # a pointer that no refused call follows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build()
+    return _lib.load()
+
+
+def sections(*values):
+    return (ctypes.c_int32 * len(values))(*values)
+
+
+def rope(lib, **kw):
+    a = dict(dtype=BF16, q=P, ldq=512, hsq=128, k=P, ldk=256, hsk=128, qo=P, ldqo=512, hsqo=128, ko=P, ldko=256, hsko=128, pos=P, ldp=10,
+             axes=1, sections=None, interleaved=0, tokens=10, hq=4, hkv=2, d=128, rot=64, theta=1e4, qw=P, kw=P, eps=1e-6)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.clef_op_qk_norm_rope_axes(*a.values(), None)
+
+
+ROPE_REFUSED = [
+    dict(dtype=2), dict(tokens=-1), dict(hq=-1), dict(hq=0, hkv=0), dict(d=0), dict(d=257, rot=64), dict(rot=0), dict(rot=63), dict(rot=130),
+    dict(theta=0.5), dict(theta=float("nan")), dict(axes=0), dict(axes=9, sections=sections(*[4] * 9)), dict(axes=2),
+    dict(axes=2, sections=sections(16, 15)), dict(axes=2, sections=sections(33, -1)), dict(axes=3, sections=sections(8, 8, 16), interleaved=1),
+    dict(axes=2, sections=sections(16, 16), ldp=9), dict(q=None), dict(qo=None), dict(k=None), dict(ko=None), dict(pos=None),
+    dict(hsq=127), dict(hsko=64), dict(ldk=100), dict(ldqo=0),
+]
+
+
+@pytest.mark.parametrize("kw", ROPE_REFUSED, ids=lambda kw: "-".join(f"{k}" for k in kw))
+def test_rope_axes_refusals(lib, kw):
+    assert rope(lib, **kw) == _lib.CLEF_EINVAL
+    with pytest.raises(ValueError):
+        _lib.check(rope(lib, **kw))
+
+
+def test_rope_axes_without_tokens_is_a_no_op(lib):
+    assert rope(lib, tokens=0, q=None, k=None) == _lib.CLEF_OK
+
+
+def attention(lib, **kw):
+    a = dict(dtype=BF16, q=P, ldq=512, hsq=128, k=P, ldk=256, hsk=128, v=P, ldv=256, hsv=128, gate=P, ldg=512, hsg=128, out=P, ldo=512,
+             hso=128, cu=P, n_seqs=2, tokens=10, hq=4, hkv=2, d=128, softcap=0.0, window=0)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.clef_op_attention_packed(*a.values(), None)
+
+
+ATTENTION_REFUSED = [
+    dict(dtype=-1), dict(n_seqs=-1), dict(tokens=-1), dict(tokens=(1 << 30) + 1), dict(hq=0), dict(hkv=0), dict(hkv=3), dict(hq=65536, hkv=1),
+    dict(d=0), dict(d=264), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(window=-1), dict(q=None),
+    dict(k=None), dict(v=None), dict(out=None), dict(cu=None), dict(hsq=64), dict(ldk=127), dict(ldv=-256), dict(hsg=0), dict(hso=8),
+]
+
+
+@pytest.mark.parametrize("kw", ATTENTION_REFUSED, ids=lambda kw: "-".join(f"{k}" for k in kw))
+def test_attention_packed_refusals(lib, kw):
+    assert attention(lib, **kw) == _lib.CLEF_EINVAL
+
+
+@pytest.mark.parametrize("kw", [dict(n_seqs=0), dict(tokens=0)])
+def test_attention_packed_without_rows_is_a_no_op(lib, kw):
+    assert attention(lib, q=None, cu=None, **kw) == _lib.CLEF_OK
