@@ -45,6 +45,7 @@ EXPORTS = (
     "clef_op_gdn_core",
     "clef_op_qk_norm_rope_axes",
     "clef_op_attention_packed",
+    "clef_op_token_logprobs",
 )
 
 
@@ -159,6 +160,7 @@ def load() -> ctypes.CDLL:
                                           ctypes.POINTER(ctypes.c_int32), i32, i32, i32, i32, i32, i32, f32, vp, vp, f32, vp],
             "clef_op_attention_packed": [i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, i32,
                                          i32, i32, f32, i32, vp],
+            "clef_op_token_logprobs": [i32, vp, i64, vp, i64, i32, i32, i32, f32, vp, i32, vp, vp, i32, vp, vp, vp],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)

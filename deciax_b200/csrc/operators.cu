@@ -4,13 +4,18 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
+#include <initializer_list>
 #include <set>
+#include <type_traits>
 
 #include "attention_packed.cuh"
 #include "attention_packed_sm100.cuh"
 #include "common.cuh"
 #include "host.cuh"
 #include "rope_axes.cuh"
+#include "token_logprobs.cuh"
+#include "token_logprobs_sm100.cuh"
 
 using bf16 = __nv_bfloat16;
 
@@ -157,9 +162,168 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
     launch_packed_simt<T, 256>(a, st);
 }
 
+// Runs of vocabulary tiles a row tile is cut into: as many as leave the fewest
+// rounds of tiles on `workers`, where a run costs a quarter of a tile besides
+// (its first columns fill a new list, its state is stored and joined).
+static int logprob_splits(int num_m, int num_n, int workers) {
+  int best = 1;
+  long long least = INT64_MAX;
+  for (int s = 1; s <= std::min(num_n, 256); ++s) {
+    const long long rounds = (static_cast<long long>(num_m) * s + workers - 1) / workers;
+    const long long cost = rounds * (4LL * ((num_n + s - 1) / s) + 1);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Stream-ordered scratch of one call, freed on the stream when the call's kernels are enqueued.
+struct OpScratch {
+  cudaStream_t st;
+  void* p = nullptr;
+  OpScratch(size_t bytes, cudaStream_t s) : st(s) {
+    CUDA_CHECK(cudaMallocFromPoolAsync(&p, bytes, op_scratch_pool(current_device()), st));
+  }
+  ~OpScratch() {
+    if (p) cudaFreeAsync(p, st);
+  }
+};
+
+// Clusters of two CTAs of the pair kernel that fit the device at once.
+template <bool CAP>
+static int logprob_pairs(int dev, cudaLaunchConfig_t cfg) {
+  static std::mutex mu;
+  static std::map<int, int> fits;
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = fits.find(dev);
+  if (it != fits.end()) return it->second;
+  cfg.gridDim = dim3(sm_count(dev) / 2 * 2);
+  cfg.dynamicSmemBytes = LogprobShape<true>::smem(kTopMax);
+  int n = 0;
+  CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, token_logprobs_tc_kernel<true, CAP>, &cfg));
+  REQUIRE(n > 0, "no CTA-pair cluster fits on this device");
+  fits[dev] = n;
+  return n;
+}
+
+template <typename T, bool CAP>
+static void token_logprobs(FinishArgs f, cudaStream_t st) {
+  LogprobArgs& a = f.l;
+  const int dev = current_device();
+  constexpr int kVec = 16 / sizeof(T);
+  const bool vec = a.dim % kVec == 0 && a.ldh % kVec == 0 && a.ldw % kVec == 0 && aligned16(a.hidden) && aligned16(a.head);
+  const bool tc = sizeof(T) == 2 && vec;
+  const bool pair = tc && a.rows > 128;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  int workers = sm_count(dev);
+  if (pair) {
+    allow_smem(token_logprobs_tc_kernel<true, CAP>, LogprobShape<true>::smem(kTopMax));
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(192);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    workers = logprob_pairs<CAP>(dev, cfg);
+  }
+  const int bm = pair ? 256 : 128, bn = tc ? 256 : 128;
+  a.num_m = (a.rows + bm - 1) / bm;
+  a.num_n = (a.vocab + bn - 1) / bn;
+  a.splits = logprob_splits(a.num_m, a.num_n, workers);
+  const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(a.num_m) * a.splits, workers));
+  const size_t states = static_cast<size_t>(a.splits) * a.rows;
+  OpScratch scratch(states * (3 + 2 * static_cast<size_t>(a.top)) * 4, st);
+  a.part_m = static_cast<float*>(scratch.p);
+  a.part_s = a.part_m + states;
+  a.part_t = a.part_s + states;
+  a.list_x = a.part_t + states;
+  a.list_id = reinterpret_cast<int32_t*>(a.list_x + states * a.top);
+  if constexpr (sizeof(T) == 2) {
+    if (tc) {
+      const CUtensorMap ta = tmap_bf16(a.hidden, a.rows, a.dim, a.ldh, 128);
+      const CUtensorMap tb = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, pair ? 128 : 256);
+      if (pair) {
+        cfg.gridDim = dim3(2 * grid);
+        cfg.dynamicSmemBytes = LogprobShape<true>::smem(a.top);
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprobs_tc_kernel<true, CAP>, ta, tb, a));
+      } else {
+        allow_smem(token_logprobs_tc_kernel<false, CAP>, LogprobShape<false>::smem(kTopMax));
+        token_logprobs_tc_kernel<false, CAP><<<grid, 192, LogprobShape<false>::smem(a.top), st>>>(ta, tb, a);
+        CUDA_CHECK(cudaGetLastError());
+      }
+    }
+  }
+  auto simt = [&](auto kern) {
+    allow_smem(kern, logprob_simt_smem(kTopMax));
+    kern<<<grid, 256, logprob_simt_smem(a.top), st>>>(a);
+    CUDA_CHECK(cudaGetLastError());
+  };
+  if constexpr (sizeof(T) == 4) {
+    if (vec)
+      simt(token_logprobs_simt_kernel<T, true, CAP>);
+    else
+      simt(token_logprobs_simt_kernel<T, false, CAP>);
+  } else {
+    if (!tc) simt(token_logprobs_simt_kernel<T, false, CAP>);
+  }
+  if (vec)
+    token_logprobs_finish_kernel<T, true, CAP><<<a.rows, 128, 0, st>>>(f);
+  else
+    token_logprobs_finish_kernel<T, false, CAP><<<a.rows, 128, 0, st>>>(f);
+  CUDA_CHECK(cudaGetLastError());
+}
+
 }  // namespace clef
 
 extern "C" {
+
+int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const void* lm_head, int64_t ldw, int rows, int vocab,
+                           int dim, float softcap, const int32_t* targets, int n_targets, float* logprobs, float* entropy,
+                           int top, int32_t* top_ids, float* top_logprobs, void* stream) {
+  using namespace clef;
+  return op_guarded([&] {
+    size_of(dtype);
+    REQUIRE(rows >= 0 && vocab > 0 && dim > 0, "rows must not be negative, vocab and dim must be positive");
+    REQUIRE(vocab <= 1 << 30 && dim <= 1 << 20 && rows <= 1 << 24, "at most 2^24 rows, 2^30 tokens and 2^20 dimensions");
+    REQUIRE(ldh >= dim && ldw >= dim, "row strides must be at least dim");
+    REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must not be negative (0 = off)");
+    REQUIRE(n_targets >= 0 && n_targets <= 1 << 20, "n_targets must be in [0, 2^20]");
+    REQUIRE(top >= 0 && top <= kTopMax && top <= vocab, "top must be in [0, min(32, vocab)]");
+    if (rows == 0) return;
+    REQUIRE(hidden && lm_head, "null operand");
+    REQUIRE(n_targets == 0 || (targets && logprobs), "targets need logprobs");
+    REQUIRE(top == 0 || (top_ids && top_logprobs), "top alternatives need their outputs");
+    REQUIRE(n_targets > 0 || top > 0 || entropy, "no output was asked for");
+    require_on_device({hidden, lm_head, n_targets ? targets : nullptr, n_targets ? logprobs : nullptr, entropy,
+                       top ? top_ids : nullptr, top ? top_logprobs : nullptr});
+    FinishArgs f{};
+    f.l.hidden = hidden;
+    f.l.head = lm_head;
+    f.l.ldh = ldh;
+    f.l.ldw = ldw;
+    f.l.rows = rows;
+    f.l.vocab = vocab;
+    f.l.dim = dim;
+    f.l.softcap = softcap;
+    f.l.top = top;
+    f.targets = targets;
+    f.n_targets = n_targets;
+    f.logprobs = logprobs;
+    f.entropy = entropy;
+    f.top_ids = top_ids;
+    f.top_logprobs = top_logprobs;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == CLEF_DTYPE_BF16)
+      softcap > 0.f ? token_logprobs<bf16, true>(f, st) : token_logprobs<bf16, false>(f, st);
+    else
+      softcap > 0.f ? token_logprobs<float, true>(f, st) : token_logprobs<float, false>(f, st);
+  });
+}
 
 int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
                              const void* v, int64_t ldv, int64_t hsv, const void* gate, int64_t ldg, int64_t hsg, void* out,

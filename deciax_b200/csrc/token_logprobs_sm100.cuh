@@ -1,0 +1,254 @@
+// Token log probabilities (token_logprobs.cuh) on the 5th-generation tensor
+// cores: bf16 operands with 16-byte aligned rows.
+//
+// The GEMM's shape, with the running state of a row in place of its store:
+//   warp 0      TMA producer: 64-deep stages of hidden rows and head rows
+//   warp 1      one thread issues tcgen05.mma into one of two TMEM accumulators
+//   warps 2..5  thread = row: reads 32 columns at a time and scans them
+// PAIR (more than 128 rows): CTA pairs on 256 rows x 256 columns, each CTA
+// loading half of both operands; otherwise one CTA on 128 rows x 256 columns,
+// where the head's bytes are the bound and a pair would only wait for its peer.
+// A unit is one row tile and one run of vocabulary tiles; units of the same run
+// are neighbours, so the row tiles that read it share it in L2.
+#pragma once
+
+#include "common.cuh"
+#include "gemm2_sm100.cuh"
+#include "token_logprobs.cuh"
+
+namespace clef {
+
+template <bool PAIR>
+struct LogprobShape {
+  static constexpr int BM = PAIR ? 256 : 128, BN = 256, BK = 64;
+  static constexpr int STAGES = PAIR ? 6 : 4;
+  static constexpr uint32_t A_BYTES = 128 * BK * 2;                 // rows a CTA holds
+  static constexpr uint32_t B_BYTES = (PAIR ? 128 : 256) * BK * 2;  // head rows a CTA holds
+  static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr size_t smem(int top) { return 1024 + STAGES * (A_BYTES + B_BYTES) + 256 + 128 * 8 * static_cast<size_t>(top); }
+};
+
+template <bool PAIR, bool CAP>
+__global__ void __launch_bounds__(192, 1)
+    token_logprobs_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                             const __grid_constant__ LogprobArgs args) {
+  using S = LogprobShape<PAIR>;
+  constexpr int BM = S::BM, BN = S::BN, BK = S::BK, STAGES = S::STAGES;
+  constexpr uint32_t IDESC = idesc_bf16_f32(BM, BN);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * S::A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sB + STAGES * S::B_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* lx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);
+  int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * args.top);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int units = args.num_m * args.splits;
+  const int num_kb = (args.dim + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tma_a);
+    prefetch_tmap(&tma_b);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], PAIR ? 8 : 4);  // one arrive per epilogue warp
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, S::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, S::TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // the peer's barriers exist before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : 0;
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      for (int unit = worker; unit < units && !*abort_flag; unit += workers) {
+        const int m = unit % args.num_m, split = unit / args.num_m;
+        const int n_end = split_begin(split + 1, args.num_n, args.splits);
+        for (int n = split_begin(split, args.num_n, args.splits); n < n_end && !*abort_flag; ++n) {
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, args.status, kTimeoutProducer) || *abort_flag) {
+              *abort_flag = 1;
+              break;
+            }
+            if constexpr (PAIR) {
+              if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (S::A_BYTES + S::B_BYTES));
+              const uint32_t bar = full0 + stage * 8;
+              tma_load_2d_pair(sA + stage * S::A_BYTES, &tma_a, bar, kb * BK, m * BM + rank * 128);
+              tma_load_2d_pair(sB + stage * S::B_BYTES, &tma_b, bar, kb * BK, n * BN + rank * 128);
+            } else {
+              mbar_arrive_expect_tx(&full[stage], S::A_BYTES + S::B_BYTES);
+              tma_load_2d(sA + stage * S::A_BYTES, &tma_a, &full[stage], kb * BK, m * BM);
+              tma_load_2d(sB + stage * S::B_BYTES, &tma_b, &full[stage], kb * BK, n * BN);
+            }
+            ++issued;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+      }
+      if constexpr (!PAIR) {
+        // Every issued load must land before the CTA may exit.
+        for (int i = 0; i < STAGES && i < issued; ++i) {
+          if (stage == 0) {
+            stage = STAGES - 1;
+            phase ^= 1;
+          } else {
+            --stage;
+          }
+          mbar_wait(&full[stage], phase, args.status, kTimeoutDrain);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int unit = worker; ok && unit < units; unit += workers) {
+        const int split = unit / args.num_m;
+        const int n_end = split_begin(split + 1, args.num_n, args.splits);
+        for (int n = split_begin(split, args.num_n, args.splits); ok && n < n_end; ++n, ++local) {
+          const int acc = local & 1;
+          ok = mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, args.status, kTimeoutMma) && !*abort_flag;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + acc * BN;
+          for (int kb = 0; ok && kb < num_kb; ++kb) {
+            if (!mbar_wait(&full[stage], phase, args.status, kTimeoutMma) || *abort_flag) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(sA + stage * S::A_BYTES);
+            const uint32_t b_addr = smem_u32(sB + stage * S::B_BYTES);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) {
+              if constexpr (PAIR)
+                umma_bf16_pair(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), IDESC,
+                               (kb | k) != 0 ? 1u : 0u);
+              else
+                umma_bf16(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), IDESC,
+                          (kb | k) != 0 ? 1u : 0u);
+            }
+            if constexpr (PAIR)
+              umma_commit_pair(&empty[stage]);
+            else
+              umma_commit(&empty[stage]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (ok) {
+            if constexpr (PAIR)
+              umma_commit_pair(&tfull[acc]);
+            else
+              umma_commit(&tfull[acc]);
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // Wait for this thread's MMAs to finish before the CTA can tear down.
+      if constexpr (PAIR)
+        umma_commit_pair(drain);
+      else
+        umma_commit(drain);
+      mbar_wait(drain, 0, args.status, kTimeoutDrain);
+    }
+  } else {
+    const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter; row within the CTA's 128
+    const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
+    int local = 0;
+    bool ok = true;
+    for (int unit = worker; ok && unit < units; unit += workers) {
+      const int m = unit % args.num_m, split = unit / args.num_m;
+      const int n_end = split_begin(split + 1, args.num_n, args.splits);
+      const int row = m * BM + static_cast<int>(rank) * 128 + r;
+      const bool any = row - lane < args.rows;  // some row of this warp exists
+      RowState st;
+      list_clear(lx, lid, args.top, r);
+      for (int n = split_begin(split, args.num_n, args.splits); n < n_end; ++n, ++local) {
+        const int acc = local & 1;
+        ok = mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue);
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
+        if (any) {
+          const int cols = min(BN, args.vocab - n * BN);
+#pragma unroll 1
+          for (int c = 0; c < cols; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(taddr + c, v);
+            tmem_wait_ld();
+            float x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
+            if (row < args.rows) scan32<CAP>(st, x, n * BN + c, cols - c, args.softcap, lx, lid, args.top, r);
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_cluster(tempty0 + acc * 8);
+          else
+            mbar_arrive(&tempty[acc]);
+        }
+      }
+      if (ok && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // no CTA frees TMEM while its pair may still use it
+  tc_fence_after();
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, S::TMEM_COLS);
+    else
+      tmem_dealloc(tmem_base, S::TMEM_COLS);
+  }
+}
+
+}  // namespace clef

@@ -329,6 +329,26 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
                              int64_t ldo, int64_t hso, const int32_t* cu_seqlens, int n_seqs, int tokens, int hq, int hkv,
                              int d, float softcap, int window, void* stream);
 
+/* Log probabilities of given tokens under the language head, the entropy of
+ * each row's distribution and its top alternatives, without the [rows, vocab]
+ * logits in memory:
+ *   x = hidden lm_head^T,  z = x or softcap * tanh(x / softcap) where softcap > 0
+ *   logprobs[r][c] = z[r][targets[r][c]] - log sum_v exp z[r][v]
+ *   entropy[r]     = -sum_v p[r][v] log p[r][v]      (nats)
+ * hidden [rows, dim] (final-normed states, row stride ldh), lm_head [vocab, dim]
+ * (row stride ldw), targets int32 [rows, n_targets] (several candidates of one
+ * position share its row): a negative id is a padded slot and gives 0, an id of
+ * vocab or more gives NaN.  top_ids / top_logprobs [rows, top]: the `top` largest
+ * x, largest first, equal ones by the lowest id (top <= 32).  Products and sums
+ * are FP32 and x is not rounded.  n_targets = 0, entropy = NULL and top = 0 leave
+ * an output out; rows = 0 does nothing.  A row with a NaN logit has NaN logprobs
+ * and entropy.  bf16 with 16-byte aligned rows (pointers, ldh, ldw, dim % 8 == 0)
+ * runs on the tensor cores.  Scratch comes from the library's stream-ordered
+ * pool: make one call on each device before capturing one into a graph. */
+int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const void* lm_head, int64_t ldw, int rows, int vocab,
+                           int dim, float softcap, const int32_t* targets, int n_targets, float* logprobs, float* entropy,
+                           int top, int32_t* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,12 @@ Tolerances are derived, not fitted.  u is half a step of the output type
   each p, and l, by that factor: 4 e A.  P rounded to bf16 (tensor cores) adds
   2^-8 A; FP32 sums of n terms add n 2^-24 A; exponentials and the sigmoid are
   good to 2^-21.  The store adds u |out|.
+* Log probabilities, with e = 2 (dim + 8) 2^-24 max_v sum_c |h_c w_c| for a score's
+  products: z and lse are each off by e, by 2^-23 of their size and lse by the
+  relative error r = (vocab / 32 + 64) 2^-24 + 2^-20 of the sum of exponentials
+  (vocab / 32 additions to a running sum; exponents to 2^-20).  The entropy's
+  two sums carry e and r against sum p |z - max| + 1.  Ids have to be equal:
+  operands lie on a grid on which every score is exact in FP32.
 """
 
 from __future__ import annotations
@@ -435,3 +441,173 @@ def test_attention_packed_rows_do_not_depend_on_their_neighbours():
     torch.cuda.synchronize()
     run_attention(q, k, v, None, outs[2], cu)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# --------------------------------------------------------------------------- token log probabilities
+
+
+def run_logprobs(hidden, head, targets=None, top=0, softcap=0.0, entropy=True):
+    import torch
+
+    n, dim = hidden.shape
+    c = targets.shape[1] if targets is not None else 0
+    logp = torch.full((n, c), 5.0, device="cuda")
+    ent = torch.full((n,), 5.0, device="cuda")
+    ids = torch.full((n, top), -7, dtype=torch.int32, device="cuda")
+    best = torch.full((n, top), 5.0, device="cuda")
+    _lib.check(lib().clef_op_token_logprobs(
+        code("bf16" if hidden.element_size() == 2 else "fp32"), hidden.data_ptr(), hidden.stride(0), head.data_ptr(), head.stride(0), n,
+        head.shape[0], dim, softcap, targets.data_ptr() if c else None, c, logp.data_ptr() if c else None,
+        ent.data_ptr() if entropy else None, top, ids.data_ptr() if top else None, best.data_ptr() if top else None, stream()))
+    return logp, ent, ids, best
+
+
+def grid_operands(g, n, vocab, dim, dtype, std=0.02, slack=0, twins=False):
+    """hidden on 1/16, head on 2^-11: every product and sum is exact in FP32."""
+    import torch
+
+    ty = torch_type(dtype)
+    hidden = (torch.randn(n, dim + slack, generator=g, device="cuda") * 16).round().clamp(-127, 127).div(16).to(ty)[:, :dim]
+    head = (torch.randn(vocab, dim + slack, generator=g, device="cuda") * (std * 2048)).round().clamp(-255, 255).div(2048)
+    if twins:  # every token has an equal one elsewhere
+        head = head[torch.arange(vocab, device="cuda") * 7 % (vocab // 2 + 1)]
+    return hidden, head.to(ty)[:, :dim]
+
+
+def check_logprobs(n, vocab, dim, dtype, top=8, n_targets=2, softcap=0.0, seed=0, **kw):
+    import torch
+
+    g = generator(seed + n + vocab + dim)
+    hidden, head = grid_operands(g, n, vocab, dim, dtype, **kw)
+    targets = torch.randint(0, vocab, (n, n_targets), generator=g, device="cuda", dtype=torch.int32)
+    if n_targets > 1:
+        targets[:, 1] = targets[:, 0]  # the same token twice
+    logp, ent, ids, best = run_logprobs(hidden, head, targets, top, softcap)
+    raw = hidden.double() @ head.double().T
+    z = softcap * torch.tanh(raw / softcap) if softcap else raw
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    want = z - lse
+    e = 2 * (dim + 8) * U32 * (hidden.double().abs() @ head.double().abs().T).amax(1, keepdim=True)
+    r = (vocab / 32 + 64) * U32 + 2.0**-20
+    tol = 2 * e + r + 2 * U32 * (z.abs() + lse.abs())
+    if n_targets:
+        t = targets.long()
+        assert ((logp.double() - want.gather(1, t)).abs() <= tol.gather(1, t)).all()
+    p = want.exp()
+    away = (p * (z - z.amax(1, keepdim=True)).abs()).sum(1)
+    assert ((ent.double() + (p * want).sum(1)).abs() <= (4 * e[:, 0] + 2 * r) * (away + 1)).all()
+    if top:
+        order = torch.sort(raw, dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(ids.long(), order)
+        assert ((best.double() - want.gather(1, order)).abs() <= tol.gather(1, order)).all()
+
+
+LOGPROB_SHAPES = [(1, 50, 8), (1, 5003, 1024), (5, 255, 72), (100, 256, 64), (128, 257, 128), (129, 3001, 256), (300, 70000, 512),
+                  (513, 1000, 320), (2, 40000, 3584)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,vocab,dim", LOGPROB_SHAPES)
+def test_token_logprobs_shapes(n, vocab, dim, dtype):
+    check_logprobs(n, vocab, dim, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 200])
+@pytest.mark.parametrize("top,n_targets", [(0, 1), (1, 0), (32, 9), (20, 1)])
+def test_token_logprobs_outputs(top, n_targets, n, dtype):
+    check_logprobs(n, 4000, 64, dtype, top=top, n_targets=n_targets)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 200])
+@pytest.mark.parametrize("softcap", [0.0, 30.0, 1.0])
+def test_token_logprobs_ties_go_to_the_lowest_id(softcap, n, dtype):
+    """Every token has a twin; under a low cap most capped scores are equal as well, and the order is still that of x."""
+    check_logprobs(n, 3000, 128, dtype, top=32, softcap=softcap, std=0.1, twins=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,dim,slack", [(7, 30, 0), (200, 64, 3), (9, 64, 8), (150, 128, 64), (1, 1, 0)])
+def test_token_logprobs_row_strides(n, dim, slack, dtype):
+    check_logprobs(n, 700, dim, dtype, slack=slack)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_token_logprobs_of_a_sharp_distribution(dtype):
+    """Scores of +-100: one token holds nearly all the probability."""
+    check_logprobs(140, 3000, 1024, dtype, std=0.1)
+
+
+def test_token_logprobs_every_token_is_an_alternative():
+    check_logprobs(130, 32, 64, "bf16", top=32)
+    check_logprobs(3, 5, 64, "fp32", top=5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [4, 150])
+def test_token_logprobs_padded_and_unknown_targets(n, dtype):
+    import torch
+
+    hidden, head = grid_operands(generator(9), n, 300, 64, dtype)
+    targets = torch.full((n, 3), -1, dtype=torch.int32, device="cuda")
+    targets[:, 1], targets[:, 2] = 300, 2**31 - 1
+    logp, _, _, _ = run_logprobs(hidden, head, targets)
+    assert (logp[:, 0] == 0).all() and logp[:, 1:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [4, 150])
+def test_token_logprobs_nan_rows_stay_alone(n, dtype):
+    import torch
+
+    hidden, head = grid_operands(generator(10), n, 500, 64, dtype)
+    targets = torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    clean = run_logprobs(hidden, head, targets, 4)
+    hidden[2, 5] = float("nan")
+    logp, ent, ids, best = run_logprobs(hidden, head, targets, 4)
+    assert logp[2].isnan().all() and ent[2].isnan()
+    keep = torch.arange(n, device="cuda") != 2
+    for got, want in zip((logp, ent, ids, best), clean):
+        assert torch.equal(got[keep], want[keep])
+
+
+def test_token_logprobs_captured_and_replayed():
+    import torch
+
+    g = generator(11)
+    hidden, head = grid_operands(g, 20, 900, 64, "bf16")
+    other, _ = grid_operands(g, 20, 900, 64, "bf16")
+    targets = torch.randint(0, 900, (20, 2), generator=g, device="cuda", dtype=torch.int32)
+    want = [run_logprobs(h, head, targets, 5) for h in (hidden, other)]
+    torch.cuda.synchronize()
+    graphs, outs, inputs = [], [], []
+    for h in (hidden, other):  # two captured calls, each with scratch of its own
+        inputs.append(h.clone())
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run_logprobs(inputs[-1], head, targets, 5))
+    for _ in range(2):
+        for s, graph in zip([torch.cuda.Stream(), torch.cuda.Stream()], graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+def test_token_logprobs_of_two_streams_at_once():
+    import torch
+
+    hidden, head = grid_operands(generator(12), 200, 5000, 256, "bf16")
+    targets = torch.zeros(200, 1, dtype=torch.int32, device="cuda")
+    want = run_logprobs(hidden, head, targets, 3)
+    torch.cuda.synchronize()
+    got = []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(run_logprobs(hidden, head, targets, 3))
+    torch.cuda.synchronize()
+    for x in got:
+        assert all(torch.equal(a, b) for a, b in zip(x, want))

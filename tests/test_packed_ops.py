@@ -75,3 +75,28 @@ def test_attention_packed_refusals(lib, kw):
 @pytest.mark.parametrize("kw", [dict(n_seqs=0), dict(tokens=0)])
 def test_attention_packed_without_rows_is_a_no_op(lib, kw):
     assert attention(lib, q=None, cu=None, **kw) == _lib.CLEF_OK
+
+
+def logprobs(lib, **kw):
+    a = dict(dtype=BF16, hidden=P, ldh=64, head=P, ldw=64, rows=3, vocab=100, dim=64, softcap=0.0, targets=P, n_targets=1, logprobs=P,
+             entropy=P, top=4, ids=P, top_logprobs=P)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.clef_op_token_logprobs(*a.values(), None)
+
+
+LOGPROBS_REFUSED = [
+    dict(dtype=7), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(dim=0), dict(dim=(1 << 20) + 1, ldh=1 << 21, ldw=1 << 21),
+    dict(ldh=63), dict(ldw=63), dict(softcap=-2.0), dict(softcap=float("inf")), dict(n_targets=-1), dict(top=-1), dict(top=33),
+    dict(top=9, vocab=8), dict(hidden=None), dict(head=None), dict(targets=None), dict(logprobs=None), dict(ids=None),
+    dict(top_logprobs=None), dict(n_targets=0, top=0, entropy=None),
+]
+
+
+@pytest.mark.parametrize("kw", LOGPROBS_REFUSED, ids=lambda kw: "-".join(f"{k}" for k in kw))
+def test_token_logprobs_refusals(lib, kw):
+    assert logprobs(lib, **kw) == _lib.CLEF_EINVAL
+
+
+def test_token_logprobs_without_rows_is_a_no_op(lib):
+    assert logprobs(lib, rows=0, hidden=None, head=None) == _lib.CLEF_OK
