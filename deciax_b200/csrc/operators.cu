@@ -162,15 +162,16 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
     launch_packed_simt<T, 256>(a, st);
 }
 
-// Runs of vocabulary tiles a row tile is cut into: as many as leave the fewest
-// rounds of tiles on `workers`, where a run costs a quarter of a tile besides
-// (its first columns fill a new list, its state is stored and joined).
-static int logprob_splits(int num_m, int num_n, int workers) {
+// Runs a row tile's vocabulary is cut into: as many as leave the fewest rounds
+// of columns on `workers`, where a run costs 64 columns besides (its first
+// columns fill a new list, its state is stored and joined).
+static int logprob_splits(int num_m, int vocab, int granule, int workers) {
+  const int granules = (vocab + granule - 1) / granule;
   int best = 1;
   long long least = INT64_MAX;
-  for (int s = 1; s <= std::min(num_n, 256); ++s) {
+  for (int s = 1; s <= std::min(granules, kLogprobMaxSplits); ++s) {
     const long long rounds = (static_cast<long long>(num_m) * s + workers - 1) / workers;
-    const long long cost = rounds * (4LL * ((num_n + s - 1) / s) + 1);
+    const long long cost = rounds * (static_cast<long long>((granules + s - 1) / s) * granule + 64);
     if (cost < least) {
       least = cost;
       best = s;
@@ -231,10 +232,10 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
     cfg.numAttrs = 1;
     workers = logprob_pairs<CAP>(dev, cfg);
   }
-  const int bm = pair ? 256 : 128, bn = tc ? 256 : 128;
+  const int bm = pair ? 256 : 128;
   a.num_m = (a.rows + bm - 1) / bm;
-  a.num_n = (a.vocab + bn - 1) / bn;
-  a.splits = logprob_splits(a.num_m, a.num_n, workers);
+  a.granule = tc ? 32 : 128;
+  a.splits = logprob_splits(a.num_m, a.vocab, a.granule, workers);
   const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(a.num_m) * a.splits, workers));
   const size_t states = static_cast<size_t>(a.splits) * a.rows;
   OpScratch scratch(states * (3 + 2 * static_cast<size_t>(a.top)) * 4, st);
@@ -247,13 +248,14 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
     if (tc) {
       const CUtensorMap ta = tmap_bf16(a.hidden, a.rows, a.dim, a.ldh, 128);
       const CUtensorMap tb = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, pair ? 128 : 256);
+      const CUtensorMap tb16 = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, 16);
       if (pair) {
         cfg.gridDim = dim3(2 * grid);
         cfg.dynamicSmemBytes = LogprobShape<true>::smem(a.top);
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprobs_tc_kernel<true, CAP>, ta, tb, a));
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprobs_tc_kernel<true, CAP>, ta, tb, tb16, a));
       } else {
         allow_smem(token_logprobs_tc_kernel<false, CAP>, LogprobShape<false>::smem(kTopMax));
-        token_logprobs_tc_kernel<false, CAP><<<grid, 192, LogprobShape<false>::smem(a.top), st>>>(ta, tb, a);
+        token_logprobs_tc_kernel<false, CAP><<<grid, 192, LogprobShape<false>::smem(a.top), st>>>(ta, tb, tb16, a);
         CUDA_CHECK(cudaGetLastError());
       }
     }
@@ -271,11 +273,15 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   } else {
     if (!tc) simt(token_logprobs_simt_kernel<T, false, CAP>);
   }
+  auto finish = [&](auto kern) {
+    allow_smem(kern, static_cast<size_t>(kLogprobMaxSplits) * kTopMax * 8);
+    kern<<<a.rows, 128, static_cast<size_t>(a.splits) * a.top * 8, st>>>(f);
+    CUDA_CHECK(cudaGetLastError());
+  };
   if (vec)
-    token_logprobs_finish_kernel<T, true, CAP><<<a.rows, 128, 0, st>>>(f);
+    finish(token_logprobs_finish_kernel<T, true, CAP>);
   else
-    token_logprobs_finish_kernel<T, false, CAP><<<a.rows, 128, 0, st>>>(f);
-  CUDA_CHECK(cudaGetLastError());
+    finish(token_logprobs_finish_kernel<T, false, CAP>);
 }
 
 }  // namespace clef

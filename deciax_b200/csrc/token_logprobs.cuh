@@ -7,8 +7,8 @@
 // The [rows, vocab] logits never exist: each vocabulary tile's scores go from
 // the accumulators straight into a running state per row,
 //   m = max z,  s = sum exp(z - m),  t = sum exp(z - m) (z - m)   (log2 units),
-// and a sorted list of the largest x with their ids.  The vocabulary is split
-// into S runs of tiles, so that few rows still fill the GPU; a run of a row
+// and a list of the largest x with their ids.  The vocabulary is split into S
+// runs of columns, so that few rows still fill the GPU; a run of a row
 // tile is one unit of work and leaves its rows' states and lists in scratch.
 // token_logprobs_finish_kernel joins the S states and lists of a row and takes the
 // given tokens' scores from their own dot products.
@@ -24,6 +24,7 @@
 namespace clef {
 
 constexpr int kTopMax = 32;
+constexpr int kLogprobMaxSplits = 256;
 
 struct LogprobArgs {
   const void* hidden;
@@ -32,8 +33,8 @@ struct LogprobArgs {
   int rows, vocab, dim;
   float softcap;
   int top;
-  // units of work: num_m row tiles x splits runs of the num_n vocabulary tiles
-  int num_m, num_n, splits;
+  // units of work: num_m row tiles x splits runs of the vocabulary, cut at multiples of `granule` columns
+  int num_m, splits, granule;
   // scratch: per (split, row) the state, then the list
   float* part_m;
   float* part_s;
@@ -43,8 +44,10 @@ struct LogprobArgs {
   int* status;
 };
 
-__device__ __forceinline__ int split_begin(int split, int num_n, int splits) {
-  return static_cast<int>(static_cast<long long>(num_n) * split / splits);
+// First column of a run.
+__device__ __forceinline__ int run_begin(const LogprobArgs& a, int split) {
+  const int granules = (a.vocab + a.granule - 1) / a.granule;
+  return min(a.vocab, static_cast<int>(static_cast<long long>(granules) * split / a.splits) * a.granule);
 }
 
 template <bool CAP>
@@ -52,10 +55,12 @@ __device__ __forceinline__ float capped(float x, float softcap) {
   return CAP ? softcap * tanhf(x / softcap) : x;
 }
 
-// A row's running state.  m, s, t are in log2 units of z; thr is the smallest x of
-// its list, which lies in shared memory, entry j of row r at [j * 128 + r].
+// A row's running state.  m, s, t are in log2 units of z.  The list of the
+// largest x lies in shared memory, entry j of row r at [j * 128 + r], in no
+// order; its smallest entry (the highest id among equals) is x = thr at `worst`.
 struct RowState {
   float m = -INFINITY, s = 0.f, t = 0.f, thr = -INFINITY;
+  int worst = 0;
 };
 
 __device__ __forceinline__ void list_clear(float* lx, int32_t* lid, int top, int r) {
@@ -65,33 +70,46 @@ __device__ __forceinline__ void list_clear(float* lx, int32_t* lid, int top, int
   }
 }
 
-// Ids arrive in rising order, so an equal score stays behind the entry it equals.
-__device__ __forceinline__ void list_insert(RowState& st, float x, int id, float* lx, int32_t* lid, int top, int r) {
-  int j = top - 1;
-  for (; j > 0 && lx[(j - 1) * 128 + r] < x; --j) {
-    lx[j * 128 + r] = lx[(j - 1) * 128 + r];
-    lid[j * 128 + r] = lid[(j - 1) * 128 + r];
+// x > thr takes the place of the smallest entry.  One pass finds the next one:
+// its loads do not depend on each other, unlike the shifts of a sorted list.
+__device__ __forceinline__ void list_replace(RowState& st, float x, int id, float* lx, int32_t* lid, int top, int r) {
+  lx[st.worst * 128 + r] = x;
+  lid[st.worst * 128 + r] = id;
+  float low = x;
+  int low_id = id, at = st.worst;
+#pragma unroll 4
+  for (int j = 0; j < top; ++j) {
+    const float v = lx[j * 128 + r];
+    const int i = lid[j * 128 + r];
+    if (v < low || (v == low && i > low_id)) low = v, low_id = i, at = j;
   }
-  lx[j * 128 + r] = x;
-  lid[j * 128 + r] = id;
-  st.thr = lx[(top - 1) * 128 + r];
+  st.thr = low;
+  st.worst = at;
+}
+
+__device__ __forceinline__ float max32(const float (&x)[32]) {
+  float p[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int c = 4; c < 32; ++c) p[c & 3] = fmaxf(p[c & 3], x[c]);
+  return fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
 }
 
 // Scores x of columns col .. col + 31, the first `valid` of which exist.
+// Candidates for the list are taken largest first, so that a chunk costs a
+// warp at most `top` rounds (and about one when the list has settled), not one
+// for every lane's every candidate.  Ids rise from chunk to chunk and equal
+// scores of a chunk go by the lowest column: an equal score never displaces.
 template <bool CAP>
-__device__ __forceinline__ void scan32(RowState& st, const float (&x)[32], int col, int valid, float softcap, float* lx,
+__device__ __forceinline__ void scan32(RowState& st, float (&x)[32], int col, int valid, float softcap, float* lx,
                                        int32_t* lid, int top, int r) {
   constexpr float LOG2E = 1.4426950408889634f;
-  float z[32];
-  float px[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (valid < 32) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    const bool in = c < valid;
-    if (in) px[c & 3] = fmaxf(px[c & 3], x[c]);
-    z[c] = CAP ? (in ? capped<CAP>(x[c], softcap) : -INFINITY) : x[c];
+    for (int c = 0; c < 32; ++c)
+      if (c >= valid) x[c] = -INFINITY;
   }
-  const float xmax = fmaxf(fmaxf(px[0], px[1]), fmaxf(px[2], px[3]));
-  const float zmax = capped<CAP>(xmax, softcap) * LOG2E;
+  float best = max32(x);
+  const float zmax = capped<CAP>(best, softcap) * LOG2E;
   if (zmax > st.m) {  // the sums move to the new maximum
     const float step = st.m - zmax, f = exp2f(step);
     st.t = st.s == 0.f ? 0.f : f * fmaf(step, st.s, st.t);
@@ -103,7 +121,7 @@ __device__ __forceinline__ void scan32(RowState& st, const float (&x)[32], int c
   if (valid >= 32) {
 #pragma unroll
     for (int c = 0; c < 32; ++c) {
-      const float d = fmaf(z[c], LOG2E, neg_m);
+      const float d = fmaf(capped<CAP>(x[c], softcap), LOG2E, neg_m);
       const float e = ex2_approx(d);
       ps[c & 3] += e;
       pt[c & 3] = fmaf(d, e, pt[c & 3]);
@@ -112,7 +130,7 @@ __device__ __forceinline__ void scan32(RowState& st, const float (&x)[32], int c
 #pragma unroll
     for (int c = 0; c < 32; ++c)
       if (c < valid) {
-        const float d = fmaf(z[c], LOG2E, neg_m);
+        const float d = fmaf(capped<CAP>(x[c], softcap), LOG2E, neg_m);
         const float e = ex2_approx(d);
         ps[c & 3] += e;
         pt[c & 3] = fmaf(d, e, pt[c & 3]);
@@ -120,22 +138,41 @@ __device__ __forceinline__ void scan32(RowState& st, const float (&x)[32], int c
   }
   st.s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   st.t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
-  if (top > 0 && xmax > st.thr) {
+  if (top > 0) {
+    while (best > st.thr) {
+      int at = 0;
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (c < valid && x[c] > st.thr) list_insert(st, x[c], col + c, lx, lid, top, r);
+      for (int c = 31; c >= 0; --c)
+        if (x[c] == best) at = c;
+      list_replace(st, best, col + at, lx, lid, top, r);
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c == at) x[c] = -INFINITY;
+      best = max32(x);
+    }
   }
 }
 
-__device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, int split, int row, const float* lx,
+// Leaves the state in scratch, and the list in order.
+__device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, int split, int row, float* lx,
                                             const int32_t* lid, int r) {
   const size_t at = static_cast<size_t>(split) * a.rows + row;
   a.part_m[at] = st.m;
   a.part_s[at] = st.s;
   a.part_t[at] = st.t;
+  unsigned taken = 0u;  // top <= 32
   for (int j = 0; j < a.top; ++j) {
-    a.list_x[at * a.top + j] = lx[j * 128 + r];
-    a.list_id[at * a.top + j] = lid[j * 128 + r];
+    float x = -INFINITY;
+    int id = INT32_MAX, from = -1;
+#pragma unroll 4
+    for (int i = 0; i < a.top; ++i) {
+      const float v = lx[i * 128 + r];
+      const int vi = lid[i * 128 + r];
+      if (!((taken >> i) & 1u) && vi >= 0 && (v > x || (v == x && vi < id))) x = v, id = vi, from = i;
+    }
+    if (from >= 0) taken |= 1u << from;
+    a.list_x[at * a.top + j] = x;
+    a.list_id[at * a.top + j] = from >= 0 ? id : -1;
   }
 }
 
@@ -185,13 +222,12 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
   const int lr = tid >> 1, lk = (tid & 1) * 8;  // row and first k this thread loads
   for (int unit = blockIdx.x; unit < a.num_m * a.splits; unit += gridDim.x) {
     const int m0 = unit % a.num_m * 128, split = unit / a.num_m;
-    const int n_end = split_begin(split + 1, a.num_n, a.splits);
+    const int n_end = run_begin(a, split + 1);
     RowState st;
     if (tid < 128) list_clear(lx, lid, a.top, tid);
     const T* pa = static_cast<const T*>(a.hidden) + (m0 + lr) * a.ldh;
     const bool la = m0 + lr < a.rows;
-    for (int n = split_begin(split, a.num_n, a.splits); n < n_end; ++n) {
-      const int n0 = n * 128;
+    for (int n0 = run_begin(a, split); n0 < n_end; n0 += 128) {
       const T* pb = static_cast<const T*>(a.head) + static_cast<long long>(n0 + lr) * a.ldw;
       const bool lb = n0 + lr < a.vocab;
       float va[8], vb[8], acc[8][8] = {};
@@ -259,81 +295,107 @@ struct FinishArgs {
   float* top_logprobs;
 };
 
-// One block a row: warp 0 joins states and lists, then the warps take the
-// targets in turn, a dot product each.
+// One block a row: all threads join the states and stage the lists, then warp 0
+// joins the lists while the others take the targets' dot products.
 template <typename T, bool VEC, bool CAP>
 __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid_constant__ FinishArgs f) {
   constexpr float LN2 = 0.6931471805599453f;
+  constexpr int kOwn = kLogprobMaxSplits / 32;
   const LogprobArgs& a = f.l;
-  __shared__ float s_lse;
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    float m = -INFINITY;
-    for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, a.part_m[static_cast<size_t>(i) * a.rows + row]);
-    m = warp_max(m);
-    float s = 0.f, t = 0.f;
-    for (int i = lane; i < a.splits; i += 32) {
-      const size_t at = static_cast<size_t>(i) * a.rows + row;
-      const float step = a.part_m[at] - m, w = exp2f(step), si = a.part_s[at];
-      s = fmaf(w, si, s);
-      if (w != 0.f) t = fmaf(w, fmaf(step, si, a.part_t[at]), t);
+  extern __shared__ float fin_x[];  // [splits * top], then their ids
+  int32_t* fin_id = reinterpret_cast<int32_t*>(fin_x + a.splits * a.top);
+  __shared__ float s_red[3][4];
+  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float pm[kLogprobMaxSplits / 128], ps[kLogprobMaxSplits / 128], pt[kLogprobMaxSplits / 128];
+  float m = -INFINITY;
+#pragma unroll
+  for (int o = 0; o < kLogprobMaxSplits / 128; ++o) {
+    const int i = tid + 128 * o;
+    const size_t at = static_cast<size_t>(i) * a.rows + row;
+    const bool in = i < a.splits;
+    pm[o] = in ? a.part_m[at] : -INFINITY;
+    ps[o] = in ? a.part_s[at] : 0.f;
+    pt[o] = in ? a.part_t[at] : 0.f;
+    m = fmaxf(m, pm[o]);
+  }
+  for (int e = tid; e < a.splits * a.top; e += 128) {
+    const size_t at = (static_cast<size_t>(e / a.top) * a.rows + row) * a.top + e % a.top;
+    fin_x[e] = a.list_x[at];
+    fin_id[e] = a.list_id[at];
+  }
+  m = warp_max(m);
+  if (lane == 0) s_red[0][warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int o = 0; o < kLogprobMaxSplits / 128; ++o) {
+    const float step = pm[o] - m, w = exp2f(step);
+    s = fmaf(w, ps[o], s);
+    if (w != 0.f) t = fmaf(w, fmaf(step, ps[o], pt[o]), t);
+  }
+  s = warp_sum(s);
+  t = warp_sum(t);
+  if (lane == 0) s_red[1][warp] = s, s_red[2][warp] = t;
+  __syncthreads();
+  s = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  t = (s_red[2][0] + s_red[2][1]) + (s_red[2][2] + s_red[2][3]);
+  const float lse = (m + log2f(s)) * LN2;
+  if (tid == 0 && f.entropy) f.entropy[row] = logf(s) - LN2 * (t / s);
+  if (warp == 0 && a.top > 0) {
+    // lane i owns the lists of splits i, i + 32, ..; each round takes the
+    // largest of the lanes' heads, the lowest id among equals
+    float hx[kOwn];
+    int hid[kOwn], head[kOwn];
+    auto load_head = [&](int o) {
+      const int i = lane + 32 * o;
+      const bool in = i < a.splits && head[o] < a.top;
+      const int id = in ? fin_id[i * a.top + head[o]] : -1;
+      hx[o] = id >= 0 ? fin_x[i * a.top + head[o]] : -INFINITY;
+      hid[o] = id >= 0 ? id : INT32_MAX;
+    };
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      head[o] = 0;
+      load_head(o);
     }
-    s = warp_sum(s);
-    t = warp_sum(t);
-    const float lse = (m + log2f(s)) * LN2;
-    if (lane == 0) {
-      s_lse = lse;
-      if (f.entropy) f.entropy[row] = logf(s) - LN2 * (t / s);
-    }
-    if (a.top > 0) {
-      // lane i owns the lists of splits i, i + 32, ..; each round takes the
-      // largest of the lanes' heads, the lowest id among equals
-      constexpr int kOwn = 8;  // splits <= 256
-      int head[kOwn] = {};
-      for (int j = 0; j < a.top; ++j) {
-        float bx = -INFINITY;
-        int bid = INT32_MAX, own = -1;
+    for (int j = 0; j < a.top; ++j) {
+      float bx = hx[0];
+      int bid = hid[0];
 #pragma unroll
-        for (int o = 0; o < kOwn; ++o) {
-          const int i = lane + 32 * o;
-          if (i < a.splits && head[o] < a.top) {
-            const size_t at = (static_cast<size_t>(i) * a.rows + row) * a.top + head[o];
-            const int id = a.list_id[at];
-            const float x = a.list_x[at];
-            if (id >= 0 && (x > bx || (x == bx && id < bid))) bx = x, bid = id, own = o;
-          }
-        }
-        float wx = bx;
-        int wid = bid;
+      for (int o = 1; o < kOwn; ++o)
+        if (hx[o] > bx || (hx[o] == bx && hid[o] < bid)) bx = hx[o], bid = hid[o];
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) {
-          const float ox = __shfl_xor_sync(0xffffffffu, wx, w);
-          const int oid = __shfl_xor_sync(0xffffffffu, wid, w);
-          if (ox > wx || (ox == wx && oid < wid)) wx = ox, wid = oid;
-        }
-        if (own >= 0 && bid == wid) {
+      for (int w = 16; w > 0; w >>= 1) {
+        const float ox = __shfl_xor_sync(0xffffffffu, bx, w);
+        const int oid = __shfl_xor_sync(0xffffffffu, bid, w);
+        if (ox > bx || (ox == bx && oid < bid)) bx = ox, bid = oid;
+      }
+      const bool some = bid != INT32_MAX;
 #pragma unroll
-          for (int o = 0; o < kOwn; ++o)
-            if (o == own) ++head[o];
+      for (int o = 0; o < kOwn; ++o)
+        if (some && hid[o] == bid) {  // ids are unique: one lane, one list
+          ++head[o];
+          load_head(o);
         }
-        if (lane == 0) {
-          const bool some = wid != INT32_MAX;
-          f.top_ids[static_cast<size_t>(row) * a.top + j] = some ? wid : -1;
-          f.top_logprobs[static_cast<size_t>(row) * a.top + j] = some ? capped<CAP>(wx, a.softcap) - lse : -INFINITY;
-        }
+      if (lane == 0) {
+        f.top_ids[static_cast<size_t>(row) * a.top + j] = some ? bid : -1;
+        f.top_logprobs[static_cast<size_t>(row) * a.top + j] = some ? capped<CAP>(bx, a.softcap) - lse : -INFINITY;
       }
     }
   }
-  __syncthreads();
-  const float lse = s_lse;
+  // without lists warp 0 takes its share of the targets
+  const int first = a.top > 0 ? 1 : 0;
+  if (warp < first) return;
   const T* h = static_cast<const T*>(a.hidden) + row * a.ldh;
-  for (int c = warp; c < f.n_targets; c += 4) {
+  for (int c = warp - first; c < f.n_targets; c += 4 - first) {
     const size_t at = static_cast<size_t>(row) * f.n_targets + c;
     const int id = f.targets[at];
     float x = 0.f;
     if (id >= 0 && id < a.vocab) {
       const T* w = static_cast<const T*>(a.head) + id * a.ldw;
       float p[8] = {};
+#pragma unroll 4
       for (int k = lane * 8; k < a.dim; k += 256) {
         float u[8], v[8];
         load8<T, VEC>(h, k, a.dim, true, u);

@@ -8,8 +8,10 @@
 // PAIR (more than 128 rows): CTA pairs on 256 rows x 256 columns, each CTA
 // loading half of both operands; otherwise one CTA on 128 rows x 256 columns,
 // where the head's bytes are the bound and a pair would only wait for its peer.
-// A unit is one row tile and one run of vocabulary tiles; units of the same run
-// are neighbours, so the row tiles that read it share it in L2.
+// A unit is one row tile and one run of columns; units of the same run are
+// neighbours, so the row tiles that read it share it in L2.  Runs end at any
+// multiple of 32 columns: their last tile is narrower, its head rows loaded 16
+// at a time, so that every worker gets the same number of columns.
 #pragma once
 
 #include "common.cuh"
@@ -28,13 +30,16 @@ struct LogprobShape {
   static constexpr size_t smem(int top) { return 1024 + STAGES * (A_BYTES + B_BYTES) + 256 + 128 * 8 * static_cast<size_t>(top); }
 };
 
+// Columns the MMA of the tile at c computes: the run's last tile is as narrow
+// as a multiple of 32 can be (the instruction's step for a pair).
+__device__ __forceinline__ int tile_width(int c, int c_end) { return min(256, (c_end - c + 31) / 32 * 32); }
+
 template <bool PAIR, bool CAP>
 __global__ void __launch_bounds__(192, 1)
     token_logprobs_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
-                             const __grid_constant__ LogprobArgs args) {
+                             const __grid_constant__ CUtensorMap tma_b16, const __grid_constant__ LogprobArgs args) {
   using S = LogprobShape<PAIR>;
   constexpr int BM = S::BM, BN = S::BN, BK = S::BK, STAGES = S::STAGES;
-  constexpr uint32_t IDESC = idesc_bf16_f32(BM, BN);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -60,6 +65,7 @@ __global__ void __launch_bounds__(192, 1)
   if (threadIdx.x == 0) {
     prefetch_tmap(&tma_a);
     prefetch_tmap(&tma_b);
+    prefetch_tmap(&tma_b16);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -95,22 +101,32 @@ __global__ void __launch_bounds__(192, 1)
       long long issued = 0;
       for (int unit = worker; unit < units && !*abort_flag; unit += workers) {
         const int m = unit % args.num_m, split = unit / args.num_m;
-        const int n_end = split_begin(split + 1, args.num_n, args.splits);
-        for (int n = split_begin(split, args.num_n, args.splits); n < n_end && !*abort_flag; ++n) {
+        const int c_end = run_begin(args, split + 1);
+        for (int c = run_begin(args, split); c < c_end && !*abort_flag; c += BN) {
+          const int w = tile_width(c, c_end);
+          // the head rows this CTA loads: all of the tile's, or its half of them
+          const int rows = PAIR ? w / 2 : w, first = PAIR ? c + static_cast<int>(rank) * rows : c;
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!mbar_wait(&empty[stage], phase ^ 1, args.status, kTimeoutProducer) || *abort_flag) {
               *abort_flag = 1;
               break;
             }
+            uint8_t* dst = sB + stage * S::B_BYTES;
             if constexpr (PAIR) {
-              if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (S::A_BYTES + S::B_BYTES));
+              if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::A_BYTES + w * BK * 2);
               const uint32_t bar = full0 + stage * 8;
-              tma_load_2d_pair(sA + stage * S::A_BYTES, &tma_a, bar, kb * BK, m * BM + rank * 128);
-              tma_load_2d_pair(sB + stage * S::B_BYTES, &tma_b, bar, kb * BK, n * BN + rank * 128);
+              tma_load_2d_pair(sA + stage * S::A_BYTES, &tma_a, bar, kb * BK, m * BM + static_cast<int>(rank) * 128);
+              if (w == BN)
+                tma_load_2d_pair(dst, &tma_b, bar, kb * BK, first);
+              else
+                for (int i = 0; i < rows; i += 16) tma_load_2d_pair(dst + i * 128, &tma_b16, bar, kb * BK, first + i);
             } else {
-              mbar_arrive_expect_tx(&full[stage], S::A_BYTES + S::B_BYTES);
+              mbar_arrive_expect_tx(&full[stage], S::A_BYTES + w * BK * 2);
               tma_load_2d(sA + stage * S::A_BYTES, &tma_a, &full[stage], kb * BK, m * BM);
-              tma_load_2d(sB + stage * S::B_BYTES, &tma_b, &full[stage], kb * BK, n * BN);
+              if (w == BN)
+                tma_load_2d(dst, &tma_b, &full[stage], kb * BK, first);
+              else
+                for (int i = 0; i < rows; i += 16) tma_load_2d(dst + i * 128, &tma_b16, &full[stage], kb * BK, first + i);
             }
             ++issued;
             if (++stage == STAGES) {
@@ -141,9 +157,10 @@ __global__ void __launch_bounds__(192, 1)
       bool ok = true;
       for (int unit = worker; ok && unit < units; unit += workers) {
         const int split = unit / args.num_m;
-        const int n_end = split_begin(split + 1, args.num_n, args.splits);
-        for (int n = split_begin(split, args.num_n, args.splits); ok && n < n_end; ++n, ++local) {
+        const int c_end = run_begin(args, split + 1);
+        for (int c = run_begin(args, split); ok && c < c_end; c += BN, ++local) {
           const int acc = local & 1;
+          const uint32_t idesc = idesc_bf16_f32(BM, tile_width(c, c_end));
           ok = mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, args.status, kTimeoutMma) && !*abort_flag;
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * BN;
@@ -158,10 +175,10 @@ __global__ void __launch_bounds__(192, 1)
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k) {
               if constexpr (PAIR)
-                umma_bf16_pair(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), IDESC,
+                umma_bf16_pair(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), idesc,
                                (kb | k) != 0 ? 1u : 0u);
               else
-                umma_bf16(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), IDESC,
+                umma_bf16(d_tmem, smem_desc_k128(a_addr + k * 32), smem_desc_k128(b_addr + k * 32), idesc,
                           (kb | k) != 0 ? 1u : 0u);
             }
             if constexpr (PAIR)
@@ -196,12 +213,12 @@ __global__ void __launch_bounds__(192, 1)
     bool ok = true;
     for (int unit = worker; ok && unit < units; unit += workers) {
       const int m = unit % args.num_m, split = unit / args.num_m;
-      const int n_end = split_begin(split + 1, args.num_n, args.splits);
+      const int c_end = run_begin(args, split + 1);
       const int row = m * BM + static_cast<int>(rank) * 128 + r;
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
       list_clear(lx, lid, args.top, r);
-      for (int n = split_begin(split, args.num_n, args.splits); n < n_end; ++n, ++local) {
+      for (int c0 = run_begin(args, split); c0 < c_end; c0 += BN, ++local) {
         const int acc = local & 1;
         ok = mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue);
         __syncwarp();
@@ -213,7 +230,7 @@ __global__ void __launch_bounds__(192, 1)
         tc_fence_after();
         const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
         if (any) {
-          const int cols = min(BN, args.vocab - n * BN);
+          const int cols = min(BN, c_end - c0);
 #pragma unroll 1
           for (int c = 0; c < cols; c += 32) {
             uint32_t v[32];
@@ -222,7 +239,7 @@ __global__ void __launch_bounds__(192, 1)
             float x[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
-            if (row < args.rows) scan32<CAP>(st, x, n * BN + c, cols - c, args.softcap, lx, lid, args.top, r);
+            if (row < args.rows) scan32<CAP>(st, x, c0 + c, cols - c, args.softcap, lx, lid, args.top, r);
             __syncwarp();
           }
         }
