@@ -162,22 +162,27 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
     launch_packed_simt<T, 256>(a, st);
 }
 
-// Runs a row tile's vocabulary is cut into: as many as leave the fewest rounds
-// of columns on `workers`, where a run costs 64 columns besides (its first
-// columns fill a new list, its state is stored and joined).
-static int logprob_splits(int num_m, int vocab, int granule, int workers) {
-  const int granules = (vocab + granule - 1) / granule;
-  int best = 1;
+// Cuts the vocabulary into runs of equal columns: as many as leave the fewest
+// rounds of columns on `workers`, where a run costs 64 columns besides (its
+// first columns fill a new list, its state is stored and joined).  A run is a
+// multiple of `step` columns and, with equal_tiles, of its tile.
+static void logprob_runs(LogprobArgs& a, int tile, int step, bool equal_tiles, int workers) {
   long long least = INT64_MAX;
-  for (int s = 1; s <= std::min(granules, kLogprobMaxSplits); ++s) {
-    const long long rounds = (static_cast<long long>(num_m) * s + workers - 1) / workers;
-    const long long cost = rounds * (static_cast<long long>((granules + s - 1) / s) * granule + 64);
+  for (int s = 1; s <= kLogprobMaxSplits; ++s) {
+    const long long share = (static_cast<long long>(a.vocab) + s - 1) / s;  // columns of a run
+    const long long tiles = (share + tile - 1) / tile;
+    const long long width = equal_tiles ? ((share + tiles - 1) / tiles + step - 1) / step * step : tile;
+    const long long run = equal_tiles ? tiles * width : (share + step - 1) / step * step;
+    const long long splits = (a.vocab + run - 1) / run;
+    const long long cost = (a.num_m * splits + workers - 1) / workers * (run + 64);
     if (cost < least) {
       least = cost;
-      best = s;
+      a.splits = static_cast<int>(splits);
+      a.run = static_cast<int>(run);
+      a.tile = static_cast<int>(width);
     }
+    if (share <= step) break;
   }
-  return best;
 }
 
 // Stream-ordered scratch of one call, freed on the stream when the call's kernels are enqueued.
@@ -234,8 +239,12 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   }
   const int bm = pair ? 256 : 128;
   a.num_m = (a.rows + bm - 1) / bm;
-  a.granule = tc ? 32 : 128;
-  a.splits = logprob_splits(a.num_m, a.vocab, a.granule, workers);
+  if (!tc)
+    logprob_runs(a, 128, 128, false, workers);
+  else if (pair)
+    logprob_runs(a, 256, 32, false, workers);
+  else
+    logprob_runs(a, 256, 8, true, workers);
   const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(a.num_m) * a.splits, workers));
   const size_t states = static_cast<size_t>(a.splits) * a.rows;
   OpScratch scratch(states * (3 + 2 * static_cast<size_t>(a.top)) * 4, st);
@@ -246,8 +255,9 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   a.list_id = reinterpret_cast<int32_t*>(a.list_x + states * a.top);
   if constexpr (sizeof(T) == 2) {
     if (tc) {
-      const CUtensorMap ta = tmap_bf16(a.hidden, a.rows, a.dim, a.ldh, 128);
-      const CUtensorMap tb = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, pair ? 128 : 256);
+      a.copies = a.rows > 64 ? 1 : a.rows > 32 ? 2 : 4;
+      const CUtensorMap ta = tmap_bf16(a.hidden, a.rows, a.dim, a.ldh, hidden_box(a.rows));
+      const CUtensorMap tb = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, pair ? 128 : a.tile);
       const CUtensorMap tb16 = tmap_bf16(a.head, a.vocab, a.dim, a.ldw, 16);
       if (pair) {
         cfg.gridDim = dim3(2 * grid);
@@ -275,8 +285,18 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   }
   auto finish = [&](auto kern) {
     allow_smem(kern, static_cast<size_t>(kLogprobMaxSplits) * kTopMax * 8);
-    kern<<<a.rows, 128, static_cast<size_t>(a.splits) * a.top * 8, st>>>(f);
-    CUDA_CHECK(cudaGetLastError());
+    // it may start while the kernel before it ends, and waits for that one itself
+    cudaLaunchConfig_t fin = {};
+    cudaLaunchAttribute early[1];
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[0].val.programmaticStreamSerializationAllowed = 1;
+    fin.gridDim = dim3(a.rows);
+    fin.blockDim = dim3(128);
+    fin.dynamicSmemBytes = static_cast<size_t>(a.splits) * a.top * 8;
+    fin.stream = st;
+    fin.attrs = early;
+    fin.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&fin, kern, f));
   };
   if (vec)
     finish(token_logprobs_finish_kernel<T, true, CAP>);

@@ -33,8 +33,9 @@ struct LogprobArgs {
   int rows, vocab, dim;
   float softcap;
   int top;
-  // units of work: num_m row tiles x splits runs of the vocabulary, cut at multiples of `granule` columns
-  int num_m, splits, granule;
+  // units of work: num_m row tiles x `splits` runs of `run` columns, in tiles of `tile`
+  int num_m, splits, run, tile;
+  int copies;  // tensor cores, at most 32 (64) rows: the row tile holds them four times (twice)
   // scratch: per (split, row) the state, then the list
   float* part_m;
   float* part_s;
@@ -44,10 +45,9 @@ struct LogprobArgs {
   int* status;
 };
 
-// First column of a run.
+// First column of a run (one past the last run: the end).
 __device__ __forceinline__ int run_begin(const LogprobArgs& a, int split) {
-  const int granules = (a.vocab + a.granule - 1) / a.granule;
-  return min(a.vocab, static_cast<int>(static_cast<long long>(granules) * split / a.splits) * a.granule);
+  return static_cast<int>(min(static_cast<long long>(a.vocab), static_cast<long long>(split) * a.run));
 }
 
 template <bool CAP>
@@ -150,6 +150,22 @@ __device__ __forceinline__ void scan32(RowState& st, float (&x)[32], int col, in
         if (c == at) x[c] = -INFINITY;
       best = max32(x);
     }
+  }
+}
+
+// Joins thread r2's state and list (in shared memory) into thread r's.
+__device__ __forceinline__ void join_state(RowState& st, float m, float s, float t, int r2, float* lx, int32_t* lid,
+                                           int top, int r) {
+  const float mx = fmaxf(st.m, m);
+  const float d0 = st.m - mx, d1 = m - mx, w0 = exp2f(d0), w1 = exp2f(d1);
+  // a side without columns has m = -inf, s = t = 0: it weighs nothing
+  st.t = (w0 == 0.f ? 0.f : w0 * fmaf(d0, st.s, st.t)) + (w1 == 0.f ? 0.f : w1 * fmaf(d1, s, t));
+  st.s = w0 * st.s + w1 * s;
+  st.m = mx;
+  for (int j = 0; j < top; ++j) {
+    const float x = lx[j * 128 + r2];
+    const int id = lid[j * 128 + r2];
+    if (id >= 0 && (x > st.thr || (x == st.thr && id < lid[st.worst * 128 + r]))) list_replace(st, x, id, lx, lid, top, r);
   }
 }
 
@@ -295,8 +311,37 @@ struct FinishArgs {
   float* top_logprobs;
 };
 
-// One block a row: all threads join the states and stage the lists, then warp 0
-// joins the lists while the others take the targets' dot products.
+// x of target c of a row: its own dot product, by a warp.
+template <typename T, bool VEC>
+__device__ __forceinline__ float target_score(const FinishArgs& f, int row, int c, int lane) {
+  const LogprobArgs& a = f.l;
+  const int id = f.targets[static_cast<size_t>(row) * f.n_targets + c];
+  if (id < 0 || id >= a.vocab) return 0.f;
+  const T* h = static_cast<const T*>(a.hidden) + row * a.ldh;
+  const T* w = static_cast<const T*>(a.head) + id * a.ldw;
+  float p[8] = {};
+#pragma unroll 4
+  for (int k = lane * 8; k < a.dim; k += 256) {
+    float u[8], v[8];
+    load8<T, VEC>(h, k, a.dim, true, u);
+    load8<T, VEC>(w, k, a.dim, true, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = fmaf(u[j], v[j], p[j]);
+  }
+  return warp_sum(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+}
+
+// A padded slot (negative id) gives 0, a token that does not exist NaN.
+template <bool CAP>
+__device__ __forceinline__ void store_logprob(const FinishArgs& f, int row, int c, float x, float lse, int lane) {
+  const size_t at = static_cast<size_t>(row) * f.n_targets + c;
+  const int id = f.targets[at];
+  if (lane == 0)
+    f.logprobs[at] = id < 0 ? 0.f : id >= f.l.vocab ? __int_as_float(0x7fffffff) : capped<CAP>(x, f.l.softcap) - lse;
+}
+
+// One block a row: each warp takes its targets' dot products, all threads join
+// the states and stage the lists, warp 0 joins the lists.
 template <typename T, bool VEC, bool CAP>
 __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid_constant__ FinishArgs f) {
   constexpr float LN2 = 0.6931471805599453f;
@@ -306,6 +351,14 @@ __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid
   int32_t* fin_id = reinterpret_cast<int32_t*>(fin_x + a.splits * a.top);
   __shared__ float s_red[3][4];
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // The targets' products need nothing of the kernel before: they run while it
+  // ends.  Each of the first kHeld stays with its warp until lse is known.
+  constexpr int kHeld = 2;
+  float held[kHeld];
+#pragma unroll
+  for (int o = 0; o < kHeld; ++o)
+    held[o] = warp + 4 * o < f.n_targets ? target_score<T, VEC>(f, row, warp + 4 * o, lane) : 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float pm[kLogprobMaxSplits / 128], ps[kLogprobMaxSplits / 128], pt[kLogprobMaxSplits / 128];
   float m = -INFINITY;
 #pragma unroll
@@ -346,7 +399,7 @@ __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid
     // lane i owns the lists of splits i, i + 32, ..; each round takes the
     // largest of the lanes' heads, the lowest id among equals
     float hx[kOwn];
-    int hid[kOwn], head[kOwn];
+    int hid[kOwn], head[kOwn] = {};
     auto load_head = [&](int o) {
       const int i = lane + 32 * o;
       const bool in = i < a.splits && head[o] < a.top;
@@ -356,7 +409,6 @@ __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid
     };
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) {
-      head[o] = 0;
       load_head(o);
     }
     for (int j = 0; j < a.top; ++j) {
@@ -384,32 +436,11 @@ __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid
       }
     }
   }
-  // without lists warp 0 takes its share of the targets
-  const int first = a.top > 0 ? 1 : 0;
-  if (warp < first) return;
-  const T* h = static_cast<const T*>(a.hidden) + row * a.ldh;
-  for (int c = warp - first; c < f.n_targets; c += 4 - first) {
-    const size_t at = static_cast<size_t>(row) * f.n_targets + c;
-    const int id = f.targets[at];
-    float x = 0.f;
-    if (id >= 0 && id < a.vocab) {
-      const T* w = static_cast<const T*>(a.head) + id * a.ldw;
-      float p[8] = {};
-#pragma unroll 4
-      for (int k = lane * 8; k < a.dim; k += 256) {
-        float u[8], v[8];
-        load8<T, VEC>(h, k, a.dim, true, u);
-        load8<T, VEC>(w, k, a.dim, true, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = fmaf(u[j], v[j], p[j]);
-      }
-      x = warp_sum(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
-      x = capped<CAP>(x, a.softcap) - lse;
-    } else if (id >= a.vocab) {
-      x = __int_as_float(0x7fffffff);  // NaN: no such token
-    }
-    if (lane == 0) f.logprobs[at] = x;
-  }
+  for (int o = 0; o < kHeld; ++o)
+    if (warp + 4 * o < f.n_targets) store_logprob<CAP>(f, row, warp + 4 * o, held[o], lse, lane);
+  for (int c = warp + 4 * kHeld; c < f.n_targets; c += 4)
+    store_logprob<CAP>(f, row, c, target_score<T, VEC>(f, row, c, lane), lse, lane);
 }
 
 }  // namespace clef

@@ -8,12 +8,17 @@
 // PAIR (more than 128 rows): CTA pairs on 256 rows x 256 columns, each CTA
 // loading half of both operands; otherwise one CTA on 128 rows x 256 columns,
 // where the head's bytes are the bound and a pair would only wait for its peer.
+// At most 32 (64) rows lie in the tile four times (twice), and the warps share
+// each row's columns instead of leaving them to one.
 // A unit is one row tile and one run of columns; units of the same run are
-// neighbours, so the row tiles that read it share it in L2.  Runs end at any
-// multiple of 32 columns: their last tile is narrower, its head rows loaded 16
-// at a time, so that every worker gets the same number of columns.
+// neighbours, so the row tiles that read it share it in L2.  Every worker gets
+// the same number of columns.  Pairs cut a run into tiles of 256 and a narrower
+// last one (head rows by 16: their MMAs are the bound); one CTA, bound by the
+// head's bytes, cuts it into equal tiles of any multiple of 8 columns, one box
+// each (a last tile in boxes of 16 rows made one row 30 us slower).
 #pragma once
 
+#include "attention_sm100.cuh"
 #include "common.cuh"
 #include "gemm2_sm100.cuh"
 #include "token_logprobs.cuh"
@@ -30,9 +35,18 @@ struct LogprobShape {
   static constexpr size_t smem(int top) { return 1024 + STAGES * (A_BYTES + B_BYTES) + 256 + 128 * 8 * static_cast<size_t>(top); }
 };
 
-// Columns the MMA of the tile at c computes: the run's last tile is as narrow
-// as a multiple of 32 can be (the instruction's step for a pair).
-__device__ __forceinline__ int tile_width(int c, int c_end) { return min(256, (c_end - c + 31) / 32 * 32); }
+// Columns the MMA of the tile at c computes, in the instruction's steps of 32
+// for a pair and 16 for one CTA.
+template <bool PAIR>
+__device__ __forceinline__ int tile_width(const LogprobArgs& a, int c, int c_end) {
+  return PAIR ? min(256, (c_end - c + 31) / 32 * 32) : (a.tile + 15) / 16 * 16;
+}
+
+// Rows of the box that loads hidden states: a box much taller than the rows
+// that exist costs the TMA unit their zeros (one row of 128: 430 us for the
+// head's 1.8 GB, against 308 us with 8 of 128).  The tile's other rows hold
+// whatever shared memory held; their scores are never read.
+__host__ __device__ inline int hidden_box(int rows) { return rows > 64 ? 128 : rows > 32 ? 64 : rows > 8 ? 32 : 8; }
 
 template <bool PAIR, bool CAP>
 __global__ void __launch_bounds__(192, 1)
@@ -54,6 +68,7 @@ __global__ void __launch_bounds__(192, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* lx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);
   int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * args.top);
+  __shared__ float3 state[PAIR ? 1 : 128];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -95,6 +110,7 @@ __global__ void __launch_bounds__(192, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      const int a_box = hidden_box(args.rows);
       const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : 0;
       int stage = 0;
       uint32_t phase = 0;
@@ -102,9 +118,9 @@ __global__ void __launch_bounds__(192, 1)
       for (int unit = worker; unit < units && !*abort_flag; unit += workers) {
         const int m = unit % args.num_m, split = unit / args.num_m;
         const int c_end = run_begin(args, split + 1);
-        for (int c = run_begin(args, split); c < c_end && !*abort_flag; c += BN) {
-          const int w = tile_width(c, c_end);
-          // the head rows this CTA loads: all of the tile's, or its half of them
+        for (int c = run_begin(args, split); c < c_end && !*abort_flag; c += args.tile) {
+          // head rows of this tile: pairs load half of them each
+          const int w = PAIR ? tile_width<PAIR>(args, c, c_end) : args.tile;
           const int rows = PAIR ? w / 2 : w, first = PAIR ? c + static_cast<int>(rank) * rows : c;
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!mbar_wait(&empty[stage], phase ^ 1, args.status, kTimeoutProducer) || *abort_flag) {
@@ -121,12 +137,10 @@ __global__ void __launch_bounds__(192, 1)
               else
                 for (int i = 0; i < rows; i += 16) tma_load_2d_pair(dst + i * 128, &tma_b16, bar, kb * BK, first + i);
             } else {
-              mbar_arrive_expect_tx(&full[stage], S::A_BYTES + w * BK * 2);
-              tma_load_2d(sA + stage * S::A_BYTES, &tma_a, &full[stage], kb * BK, m * BM);
-              if (w == BN)
-                tma_load_2d(dst, &tma_b, &full[stage], kb * BK, first);
-              else
-                for (int i = 0; i < rows; i += 16) tma_load_2d(dst + i * 128, &tma_b16, &full[stage], kb * BK, first + i);
+              mbar_arrive_expect_tx(&full[stage], args.copies * a_box * BK * 2 + w * BK * 2);
+              for (int i = 0; i < args.copies; ++i)
+                tma_load_2d(sA + stage * S::A_BYTES + i * (BM / args.copies) * 128, &tma_a, &full[stage], kb * BK, m * BM);
+              tma_load_2d(dst, &tma_b, &full[stage], kb * BK, first);
             }
             ++issued;
             if (++stage == STAGES) {
@@ -158,9 +172,9 @@ __global__ void __launch_bounds__(192, 1)
       for (int unit = worker; ok && unit < units; unit += workers) {
         const int split = unit / args.num_m;
         const int c_end = run_begin(args, split + 1);
-        for (int c = run_begin(args, split); ok && c < c_end; c += BN, ++local) {
+        for (int c = run_begin(args, split); ok && c < c_end; c += args.tile, ++local) {
           const int acc = local & 1;
-          const uint32_t idesc = idesc_bf16_f32(BM, tile_width(c, c_end));
+          const uint32_t idesc = idesc_bf16_f32(BM, tile_width<PAIR>(args, c, c_end));
           ok = mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, args.status, kTimeoutMma) && !*abort_flag;
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * BN;
@@ -208,17 +222,20 @@ __global__ void __launch_bounds__(192, 1)
     }
   } else {
     const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter; row within the CTA's 128
+    // with copies, this warp's rows are seen by others too: each takes every copies-th 32 columns
+    const int copies = PAIR ? 1 : args.copies, rows_seen = 128 / copies;
+    const int share = r / rows_seen;
     const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
     int local = 0;
     bool ok = true;
     for (int unit = worker; ok && unit < units; unit += workers) {
       const int m = unit % args.num_m, split = unit / args.num_m;
       const int c_end = run_begin(args, split + 1);
-      const int row = m * BM + static_cast<int>(rank) * 128 + r;
+      const int row = m * BM + static_cast<int>(rank) * 128 + r - share * rows_seen;
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
       list_clear(lx, lid, args.top, r);
-      for (int c0 = run_begin(args, split); c0 < c_end; c0 += BN, ++local) {
+      for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
         const int acc = local & 1;
         ok = mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue);
         __syncwarp();
@@ -230,9 +247,9 @@ __global__ void __launch_bounds__(192, 1)
         tc_fence_after();
         const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
         if (any) {
-          const int cols = min(BN, c_end - c0);
+          const int cols = min(args.tile, c_end - c0);
 #pragma unroll 1
-          for (int c = 0; c < cols; c += 32) {
+          for (int c = 32 * share; c < cols; c += 32 * copies) {
             uint32_t v[32];
             tmem_ld32(taddr + c, v);
             tmem_wait_ld();
@@ -252,10 +269,25 @@ __global__ void __launch_bounds__(192, 1)
             mbar_arrive(&tempty[acc]);
         }
       }
-      if (ok && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+      if constexpr (!PAIR) {
+        if (copies > 1) {
+          // the shares of a row meet in the first one's thread
+          state[r] = make_float3(st.m, st.s, st.t);
+          ok = !bar_red_or(1, 128, !ok);  // a failed wait ends every warp's loop together
+          if (ok && share == 0 && row < args.rows)
+            for (int i = 1; i < copies; ++i) {
+              const int r2 = r + i * rows_seen;
+              const float3 o = state[r2];
+              join_state(st, o.x, o.y, o.z, r2, lx, lid, args.top, r);
+            }
+        }
+      }
+      if (ok && share == 0 && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+      if (!PAIR && copies > 1) asm volatile("bar.sync 1, 128;" ::: "memory");  // the lists may be cleared
     }
   }
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();  // no CTA frees TMEM while its pair may still use it
