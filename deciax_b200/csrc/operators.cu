@@ -78,10 +78,33 @@ static void rope_frequencies(RopeAxesArgs& a, int rot, double theta, int axes, c
   }
 }
 
+template <typename T, int LANES>
+static void launch_rope(const RopeAxesArgs& a, cudaStream_t st) {
+  // a block's tokens share one computation of cos and sin; few tokens spread over the SMs instead
+  const int span = std::max(1, std::min(4, a.tokens / (4 * sm_count(current_device()))));
+  const int grid = (a.tokens + span - 1) / span;
+  rope_axes_kernel<T, LANES><<<grid, 256, sizeof(float2) * span * a.half, st>>>(a, span);
+}
+
 template <typename T>
 static void rope_axes(const RopeAxesArgs& a, cudaStream_t st) {
-  const long long items = static_cast<long long>(a.tokens) * (a.heads[0] + a.heads[1]);
-  rope_axes_any_kernel<T><<<static_cast<int>((items + 7) / 8), 256, 8 * a.d * sizeof(float), st>>>(a);
+  constexpr int kVec = 16 / sizeof(T);
+  bool vec = a.d % 16 == 0 && a.half % 8 == 0;
+  for (int i = 0; i < 2; ++i)
+    if (a.heads[i])
+      vec = vec && aligned16(a.x[i]) && aligned16(a.out[i]) && (!a.w[i] || aligned16(a.w[i])) && a.ldx[i] % kVec == 0 &&
+            a.ldo[i] % kVec == 0 && (a.heads[i] == 1 || (a.hsx[i] % kVec == 0 && a.hso[i] % kVec == 0));
+  if (vec) {
+    if (a.d <= 64)
+      launch_rope<T, 4>(a, st);
+    else if (a.d <= 128)
+      launch_rope<T, 8>(a, st);
+    else
+      launch_rope<T, 16>(a, st);
+  } else {
+    const long long items = static_cast<long long>(a.tokens) * (a.heads[0] + a.heads[1]);
+    rope_axes_any_kernel<T><<<static_cast<int>((items + 7) / 8), 256, 8 * a.d * sizeof(float), st>>>(a);
+  }
   CUDA_CHECK(cudaGetLastError());
 }
 
