@@ -52,6 +52,18 @@ static void require_on_device(std::initializer_list<const void*> pointers) {
   }
 }
 
+// Dynamic shared memory beyond the default is a per-device attribute of a kernel.
+template <typename K>
+static void allow_smem(K kern, size_t bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  const std::pair<int, const void*> key{current_device(), reinterpret_cast<const void*>(kern)};
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count(key)) return;
+  CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  done.insert(key);
+}
+
 static int size_of(int dtype) {
   REQUIRE(dtype == CLEF_DTYPE_BF16 || dtype == CLEF_DTYPE_F32, "dtype must be CLEF_DTYPE_BF16 or CLEF_DTYPE_F32");
   return dtype == CLEF_DTYPE_BF16 ? 2 : 4;
@@ -61,10 +73,11 @@ static void rope_frequencies(RopeAxesArgs& a, int rot, double theta, int axes, c
                              int interleaved) {
   const int half = rot / 2;
   a.half = half;
-  for (int i = 0; i < half; ++i) {
-    const long double turn = std::pow(static_cast<long double>(theta), static_cast<long double>(-2 * i) / rot) /
-                             6.283185307179586476925286766559L;
-    a.turn[i] = static_cast<unsigned long long>(std::ldexp(turn, 64));
+  // powers by repeated products of one 64-bit-mantissa root: off by 2^-57 at most
+  const long double step = std::pow(static_cast<long double>(theta), -2.0L / rot);
+  long double turn = 18446744073709551616.0L / 6.283185307179586476925286766559L;  // 2^64 / 2 pi
+  for (int i = 0; i < half; ++i, turn *= step) {
+    a.turn[i] = static_cast<unsigned long long>(turn);
     a.axis[i] = 0;
   }
   if (axes == 1) return;
@@ -80,27 +93,34 @@ static void rope_frequencies(RopeAxesArgs& a, int rot, double theta, int axes, c
 
 template <typename T, int LANES>
 static void launch_rope(const RopeAxesArgs& a, cudaStream_t st) {
-  // a block's tokens share one computation of cos and sin; few tokens spread over the SMs instead
-  const int span = std::max(1, std::min(4, a.tokens / (4 * sm_count(current_device()))));
-  const int grid = (a.tokens + span - 1) / span;
-  rope_axes_kernel<T, LANES><<<grid, 256, sizeof(float2) * span * a.half, st>>>(a, span);
+  // all heads in one block where 512 threads hold them, else in groups of equal size
+  const int heads = a.heads[0] + a.heads[1], groups = (heads * LANES + 511) / 512;
+  const int threads = ((heads + groups - 1) / groups * LANES + 31) / 32 * 32;
+  // a block's tokens share its weights and the start of its pipeline; few tokens spread over the SMs instead
+  const int span = std::max(1, std::min(16, static_cast<int>(static_cast<long long>(a.tokens) * groups /
+                                                             (12 * sm_count(current_device())))));
+  const size_t smem = RopeShape<T>::ring(threads) + sizeof(float2) * span * a.half;
+  allow_smem(rope_axes_kernel<T, LANES>, RopeShape<T>::ring(512) + sizeof(float2) * 16 * kRopeMaxHalf);
+  rope_axes_kernel<T, LANES><<<dim3((a.tokens + span - 1) / span, groups), threads, smem, st>>>(a, span);
 }
 
 template <typename T>
 static void rope_axes(const RopeAxesArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  bool vec = a.d % 16 == 0 && a.half % 8 == 0;
+  bool vec = a.d % (2 * kVec) == 0 && a.half % kVec == 0;
   for (int i = 0; i < 2; ++i)
     if (a.heads[i])
       vec = vec && aligned16(a.x[i]) && aligned16(a.out[i]) && (!a.w[i] || aligned16(a.w[i])) && a.ldx[i] % kVec == 0 &&
             a.ldo[i] % kVec == 0 && (a.heads[i] == 1 || (a.hsx[i] % kVec == 0 && a.hso[i] % kVec == 0));
   if (vec) {
-    if (a.d <= 64)
+    if (a.d <= 8 * kVec)
       launch_rope<T, 4>(a, st);
-    else if (a.d <= 128)
+    else if (a.d <= 16 * kVec)
       launch_rope<T, 8>(a, st);
-    else
+    else if (a.d <= 32 * kVec)
       launch_rope<T, 16>(a, st);
+    else
+      launch_rope<T, 32>(a, st);
   } else {
     const long long items = static_cast<long long>(a.tokens) * (a.heads[0] + a.heads[1]);
     rope_axes_any_kernel<T><<<static_cast<int>((items + 7) / 8), 256, 8 * a.d * sizeof(float), st>>>(a);
@@ -122,18 +142,6 @@ static CUtensorMap tmap_bf16_heads(const void* ptr, int tokens, int heads, int d
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(CLEF_EINVAL, "cuTensorMapEncodeTiled rejected an attention operand");
   return m;
-}
-
-// Dynamic shared memory beyond the default is a per-device attribute of a kernel.
-template <typename K>
-static void allow_smem(K kern, size_t bytes) {
-  static std::mutex mu;
-  static std::set<std::pair<int, const void*>> done;
-  const std::pair<int, const void*> key{current_device(), reinterpret_cast<const void*>(kern)};
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count(key)) return;
-  CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-  done.insert(key);
 }
 
 template <typename T, int DP>

@@ -84,9 +84,8 @@ __global__ void __launch_bounds__(256) rope_axes_any_kernel(const __grid_constan
   for (int i = 2 * a.half + lane; i < a.d; i += 32) out[i] = from_f32<T>(row[i]);
 }
 
-// Eight consecutive elements.
-__device__ __forceinline__ void load_vec8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+// The elements of a 16-byte vector as floats, and back.
+__device__ __forceinline__ void unpack16(const uint4 u, float (&v)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -94,86 +93,112 @@ __device__ __forceinline__ void load_vec8(const __nv_bfloat16* p, float (&v)[8])
     v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ void load_vec8(const float* p, float (&v)[8]) {
-  *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-  *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+__device__ __forceinline__ void unpack16(const uint4 u, float (&v)[4]) {
+  v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
 }
-__device__ __forceinline__ void store_vec8(__nv_bfloat16* p, const float (&v)[8]) {
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) =
       make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
-__device__ __forceinline__ void store_vec8(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v);
-  *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(v + 4);
+__device__ __forceinline__ void store16(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// 16-byte aligned rows, d and rot multiples of 16: a block takes `span` tokens.
-// Their cos and sin are computed once, into shared memory, while the first
-// rows load; then LANES lanes hold a head row, each an element run of 8 and the
-// run its rotation pairs it with (or two runs behind the rotated part), so that
-// a row is read and written once by 16-byte accesses and its norm is one
-// reduction over the lanes.  HBM bound; the next row of a lane loads while the
-// current one is computed.
+template <typename T>
+struct RopeShape {
+  static constexpr int V = 16 / sizeof(T);  // elements of a 16-byte vector
+  static constexpr int DEPTH = 4;           // rows a lane has on the way, the current one among them
+  static constexpr size_t ring(int threads) { return static_cast<size_t>(DEPTH) * 2 * threads * sizeof(uint4); }
+};
+
+// 16-byte aligned rows, d and rot multiples of two vectors: LANES lanes hold a
+// head row, each a 16-byte vector and the one its rotation pairs it with (or two
+// behind the rotated part, as far apart as keeps neighbours adjacent), so that a
+// row is read and written once by whole sectors and its norm is one reduction
+// over the lanes.  A lane keeps its head
+// and walks the block's `span` tokens, so the weights stay in registers and a
+// row costs no index arithmetic (a walk over (token, head) pairs issued 2.6
+// times the instructions and was bound by them at 4.8 TB/s).  cos and sin of
+// the block's tokens are computed once, while the first rows load.  HBM bound:
+// rows come by asynchronous copies, DEPTH on the way, into slots of shared
+// memory that only their lane reads, so nothing waits at a barrier.
+// grid (token spans, head groups of blockDim / LANES).
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int span) {
-  extern __shared__ float2 rope_cs[];  // [span][half]
-  constexpr int SLOTS = 256 / LANES;   // head rows in flight in the block
-  const int tid = threadIdx.x, j = tid % LANES;
+__global__ void __launch_bounds__(512) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int span) {
+  using S = RopeShape<T>;
+  constexpr int V = S::V;
+  extern __shared__ uint4 rope_ring[];  // [DEPTH][2][threads], then cos, sin [span][half]
+  const int threads = blockDim.x, tid = threadIdx.x, j = tid % LANES;
+  float2* rope_cs = reinterpret_cast<float2*>(rope_ring + S::DEPTH * 2 * threads);
   const int t0 = blockIdx.x * span, n = min(span, a.tokens - t0);
-  const int heads = a.heads[0] + a.heads[1];
-  const bool active = j < a.d / 16;
-  const bool turns = j < a.half / 8;
-  const int lo_at = turns ? 8 * j : 2 * a.half + 16 * (j - a.half / 8);
-  const int hi_at = turns ? lo_at + a.half : lo_at + 8;
-  int t = (tid / LANES) / heads, h = (tid / LANES) % heads;
-  float lo[8] = {}, hi[8] = {};
-  auto load = [&](int t, int h, float (&lo)[8], float (&hi)[8]) {
-    if (t < n && active) {
-      const int which = h >= a.heads[0];
-      const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + (t0 + t) * (which ? a.ldx[1] : a.ldx[0]) +
-                   (which ? (h - a.heads[0]) * a.hsx[1] : h * a.hsx[0]);
-      load_vec8(x + lo_at, lo);
-      load_vec8(x + hi_at, hi);
+  int h = blockIdx.y * (threads / LANES) + tid / LANES;
+  const bool live = h < a.heads[0] + a.heads[1] && j < a.d / (2 * V);  // lanes behind the heads or the row's end
+  const int which = h >= a.heads[0];
+  if (which) h -= a.heads[0];
+  const bool turns = j < a.half / V;
+  const int lo_at = turns ? V * j : a.half + V * j;  // behind the rotated part: 2 half + V (j - half / V)
+  const int hi_at = lo_at + (turns ? a.half : a.d / 2 - a.half);
+  const long long ldx = which ? a.ldx[1] : a.ldx[0], ldo = which ? a.ldo[1] : a.ldo[0];
+  const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + t0 * ldx + h * (which ? a.hsx[1] : a.hsx[0]);
+  T* out = static_cast<T*>(which ? a.out[1] : a.out[0]) + t0 * ldo + h * (which ? a.hso[1] : a.hso[0]);
+  const T* w = static_cast<const T*>(which ? a.w[1] : a.w[0]);
+  int fill = 0;
+  auto fetch = [&](int t) {  // the row of token t, into slot `fill`
+    if (live && t < n) {
+      uint4* dst = rope_ring + fill * 2 * threads + tid;
+      cp_async16(dst, x + lo_at, true);
+      cp_async16(dst + threads, x + hi_at, true);
+      x += ldx;
     }
+    cp_async_commit();
+    if (++fill == S::DEPTH) fill = 0;
   };
-  load(t, h, lo, hi);
-  for (int e = tid; e < n * a.half; e += 256) {
-    const int i = e % a.half;
-    rope_cs[e] = rope_cos_sin(a.pos[a.axis[i] * a.ldp + t0 + e / a.half], a.turn[i]);
+#pragma unroll
+  for (int i = 0; i < S::DEPTH - 1; ++i) fetch(i);
+  float wl[V], wh[V];  // 1 + w of this lane's vectors
+#pragma unroll
+  for (int e = 0; e < V; ++e) wl[e] = wh[e] = 1.f;
+  if (live && w) {
+    unpack16(*reinterpret_cast<const uint4*>(w + lo_at), wl);
+    unpack16(*reinterpret_cast<const uint4*>(w + hi_at), wh);
+#pragma unroll
+    for (int e = 0; e < V; ++e) wl[e] += 1.f, wh[e] += 1.f;
+  }
+  for (int e = tid; e < n * a.half; e += threads) {
+    // a lane reads two pairs at a time: the lanes' two lie side by side
+    const int t = e / a.half, i = e % a.half;
+    rope_cs[t * a.half + (i % V / 2 * (a.half / V) + i / V) * 2 + (i & 1)] =
+        rope_cos_sin(a.pos[a.axis[i] * a.ldp + t0 + t], a.turn[i]);
   }
   __syncthreads();
-  while (__any_sync(0xffffffffu, t < n)) {
-    int t_next = t, h_next = h + SLOTS;
-    while (h_next >= heads) {
-      h_next -= heads;
-      ++t_next;
-    }
-    float lo_next[8] = {}, hi_next[8] = {};
-    load(t_next, h_next, lo_next, hi_next);
-    const int which = h >= a.heads[0];
-    const T* w = static_cast<const T*>(which ? a.w[1] : a.w[0]);
+  const float inv_d = 1.f / static_cast<float>(a.d);
+  int take = 0;
+  for (int t = 0; t < n; ++t) {
+    fetch(t + S::DEPTH - 1);
+    cp_async_wait<S::DEPTH - 1>();
+    float lo[V], hi[V];
+    const uint4* src = rope_ring + take * 2 * threads + tid;
+    unpack16(src[0], lo);
+    unpack16(src[threads], hi);
+    if (++take == S::DEPTH) take = 0;
     float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+    for (int e = 0; e < V; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+    if (!live) ss = 0.f;  // nothing was fetched
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (t < n && active) {
-      if (w) {
-        const float r = rsqrtf(ss / static_cast<float>(a.d) + a.eps);
-        float wl[8], wh[8];
-        load_vec8(w + lo_at, wl);
-        load_vec8(w + hi_at, wh);
+    const float r = w ? rsqrtf(ss * inv_d + a.eps) : 1.f;
+    if (live) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          lo[e] *= r * (1.f + wl[e]);
-          hi[e] *= r * (1.f + wh[e]);
-        }
+      for (int e = 0; e < V; ++e) {
+        lo[e] *= r * wl[e];
+        hi[e] *= r * wh[e];
       }
       if (turns) {
-        const float4* cs = reinterpret_cast<const float4*>(rope_cs + t * a.half + 8 * j);
+        const float4* cs = reinterpret_cast<const float4*>(rope_cs + t * a.half) + j;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 c = cs[e];  // cos, sin of two pairs
+        for (int e = 0; e < V / 2; ++e) {
+          const float4 c = cs[e * (a.half / V)];  // cos, sin of two pairs
           const float l0 = lo[2 * e], h0 = hi[2 * e], l1 = lo[2 * e + 1], h1 = hi[2 * e + 1];
           lo[2 * e] = l0 * c.x - h0 * c.y;
           hi[2 * e] = h0 * c.x + l0 * c.y;
@@ -181,18 +206,10 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
           hi[2 * e + 1] = h1 * c.z + l1 * c.w;
         }
       }
-      T* out = static_cast<T*>(which ? a.out[1] : a.out[0]) + (t0 + t) * (which ? a.ldo[1] : a.ldo[0]) +
-               (which ? (h - a.heads[0]) * a.hso[1] : h * a.hso[0]);
-      store_vec8(out + lo_at, lo);
-      store_vec8(out + hi_at, hi);
+      store16(out + lo_at, lo);
+      store16(out + hi_at, hi);
+      out += ldo;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = lo_next[e];
-      hi[e] = hi_next[e];
-    }
-    t = t_next;
-    h = h_next;
   }
 }
 
