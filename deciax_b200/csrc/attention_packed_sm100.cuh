@@ -14,8 +14,8 @@
 // Key tiles are aligned to the query tile's end, so the diagonal is the last
 // tile (the last two at 64 keys) and only tiles that reach below some row's
 // first key need a mask besides.  The maximum moves, and O is rescaled, only
-// when it grows by more than 2^8; a row that saw no key yet has O = 0 written
-// rather than scaled, so what foreign tiles left there is gone.
+// when it grows by more than 2^8.  A part of a tile that every row of a warp
+// masks leaves P = 0 and nothing else.
 //
 // Differs from attention_sm100.cuh in what bounds a row's keys, and in the
 // rounding: the sigmoid gate multiplies in FP32 and the result is rounded once.
@@ -48,18 +48,57 @@ struct AttnPackedMaps {
   CUtensorMap q, k, v, gate, out;
 };
 
-// The last s in [0, n) with cu[s] <= row (cu[0] <= row), by a whole warp: 32 probes a round.
-__device__ __forceinline__ int packed_seq_warp(const int32_t* cu, int n, int row, int lane) {
+// The last s in [0, n) with cu[s] <= row, by a whole warp, 32 probes a round
+// (0 where there is none).  `start` gets cu[s].
+__device__ __forceinline__ int packed_seq_warp(const int32_t* cu, int n, int row, int lane, int& start) {
   int lo = 0;
-  while (n > 1) {
+  start = 0;
+  do {
     const int step = (n + 31) >> 5;
     const int at = lane * step;
-    const unsigned hit = __ballot_sync(0xffffffffu, at < n && cu[lo + at] <= row);
+    const int c = at < n ? cu[lo + at] : INT32_MAX;
+    const unsigned hit = __ballot_sync(0xffffffffu, c <= row);
     const int j = hit ? 31 - __clz(hit) : 0;
+    start = __shfl_sync(0xffffffffu, c, j);
     lo += j * step;
     n = min(step, n - j * step);
-  }
+  } while (n > 1);
   return lo;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Sigmoids of 32 gates (bf16).  Two share one reciprocal, 1/a = b / (ab): the
+// special-function unit, at 16 results a cycle and SM, bounds the epilogue.
+// The product of two sums 1 + e^-g stays finite while -g log2 e <= 63; a row
+// with a gate below -43, or NaN, takes a reciprocal for each.
+__device__ __forceinline__ void sigmoid32(const uint4 (&gq)[4], float (&sg)[32]) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t gw[4] = {gq[q].x, gq[q].y, gq[q].z, gq[q].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sg[8 * q + 2 * e] = __uint_as_float(gw[e] << 16) * -1.4426950408889634f;
+      sg[8 * q + 2 * e + 1] = __uint_as_float(gw[e] & 0xffff0000u) * -1.4426950408889634f;
+      top = max_nan(top, max_nan(sg[8 * q + 2 * e], sg[8 * q + 2 * e + 1]));
+    }
+  }
+  if (top <= 63.f) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float a = 1.f + ex2_approx(sg[e]), b = 1.f + ex2_approx(sg[e + 1]);
+      const float r = rcp_approx(a * b);
+      sg[e] = r * b;
+      sg[e + 1] = r * a;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) sg[e] = rcp_approx(1.f + ex2_approx(sg[e]));
+  }
 }
 
 template <int D>
@@ -106,9 +145,10 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   float* xbuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);  // softmax parts' exchange
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int first, total;
-  packed_extent(a, first, total);
   const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
+  int first, total, seq_start = 0;
+  packed_extent(a, first, total);
+  if (warp == 2) packed_seq_warp(a.cu, a.n_seqs, q0, lane, seq_start);  // beside the loads of the extent
   const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
   if (q_first >= q_end) return;  // no row of this tile belongs to a sequence
   const int hk = h / (a.H / a.Hk);
@@ -136,8 +176,11 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     tmem_relinquish();
   }
   if (warp == 2) {
-    const int s = packed_seq_warp(a.cu, a.n_seqs, q_first, lane);
-    if (lane == 0) *s_begin = packed_first_key(a, q_first, s, s);
+    if (q_first != q0) {  // the first sequence starts inside the tile
+      seq_start = first;
+    }
+    const int start = min(max(seq_start, 0), q_first);
+    if (lane == 0) *s_begin = a.window > 0 ? max(start, q_first - a.window + 1) : start;
   }
   tc_fence_before();
   __syncthreads();
@@ -298,11 +341,13 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     {
       const int w0 = max(q0 + q4 * 32, q_first), w1 = min(q0 + q4 * 32 + 31, q_end - 1);
       if (w0 <= w1) {
-        const int s0 = packed_seq_warp(a.cu, a.n_seqs, w0, lane), s1 = packed_seq_warp(a.cu, a.n_seqs, w1, lane);
+        int start;
+        const int s0 = packed_seq_warp(a.cu, a.n_seqs, w0, lane, start), s1 = packed_seq_warp(a.cu, a.n_seqs, w1, lane, start);
         if (live) lo = packed_first_key(a, row, s0, s1);
       }
     }
-    const int lo_max = __reduce_max_sync(0xffffffffu, lo);
+    // over the warp's rows: keys below lo_min or above its last row are masked for all of them
+    const int lo_max = __reduce_max_sync(0xffffffffu, lo), lo_min = __reduce_min_sync(0xffffffffu, lo);
     const uint32_t t_lane = static_cast<uint32_t>(q4 * 32) << 16;
     const float scale = rsqrtf(static_cast<float>(a.d));
     const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
@@ -337,23 +382,30 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         tc_fence_before();
         mbar_arrive(&sfree[s]);
       }
+      // every key of this part is masked for every row of the warp: short sequences, a window's edge
+      const bool none = k0 > q0 + q4 * 32 + 31 || k0 + BKP - 1 < lo_min;
       if constexpr (CAP) {
+        if (!none) {
 #pragma unroll
-        for (int c = 0; c < BKP; ++c)
-          sr[c] = __float_as_uint(packed_score(__uint_as_float(sr[c]), scale, a.softcap));
+          for (int c = 0; c < BKP; ++c)
+            sr[c] = __float_as_uint(packed_score(__uint_as_float(sr[c]), scale, a.softcap));
+        }
       }
-      if (k0 + BKP - 1 > q0 + q4 * 32 || k0 < lo_max) {  // some key of this part is masked for some row of the warp
-        const int top = row - k0, low = lo - k0;
+      float mt = -INFINITY;
+      if (!none) {
+        if (k0 + BKP - 1 > q0 + q4 * 32 || k0 < lo_max) {  // some key of this part is masked for some row of the warp
+          const int top = row - k0, low = lo - k0;
 #pragma unroll
-        for (int c = 0; c < BKP; ++c) sr[c] = c >= low && c <= top ? sr[c] : 0xff800000u;  // -inf
+          for (int c = 0; c < BKP; ++c) sr[c] = c >= low && c <= top ? sr[c] : 0xff800000u;  // -inf
+        }
+        // Row max with 8 independent partial maxima (short dependency chains).
+        float pm[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sr[e]);
+#pragma unroll
+        for (int c = 8; c < BKP; ++c) pm[c & 7] = fmaxf(pm[c & 7], __uint_as_float(sr[c]));
+        mt = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
       }
-      // Row max with 8 independent partial maxima (short dependency chains).
-      float pm[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sr[e]);
-#pragma unroll
-      for (int c = 8; c < BKP; ++c) pm[c & 7] = fmaxf(pm[c & 7], __uint_as_float(sr[c]));
-      float mt = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
       if constexpr (NP > 1) {
         // both parts of a row end with the same maximum, bit for bit
         xbuf[(s * NP + part) * 128 + r] = mt;
@@ -365,9 +417,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         for (int p = 0; p < NP; ++p) mt = fmaxf(mt, xbuf[(s * NP + p) * 128 + r]);
       }
       const float mn = fmaxf(m, mt * scale_log2);
-      if (t == 0) {
-        m = mn;
-      } else {
+      if (m == -INFINITY) m = mn;  // the row's first keys: its O and l are zero
+      {
         // the parts of a row see the same m and mn, so they decide alike
         const bool need = mn > m + 8.f;
         if (__any_sync(0xffffffffu, need)) {
@@ -384,7 +435,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
             }
           }
           tc_fence_after();
-          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);  // 0 for a row's first keys
+          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
           m = mn;
           l *= corr;
 #pragma unroll 1
@@ -393,7 +444,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
             tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = corr == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * corr);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
             tmem_st32(tmem + t_lane + Sh::O_COL + c, o);
           }
           tmem_wait_st();
@@ -419,6 +470,10 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 #pragma unroll
         for (int w = 0; w < NWP / 2; ++w) {
           uint32_t pw[32];
+          if (none) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pw[e] = 0u;
+          } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int c = 64 * w + 2 * e;
@@ -428,12 +483,17 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
             ps[(c + 1) & 7] += p1;
             pw[e] = pack_bf16x2(p0, p1);
           }
+          }
           tmem_st32(tmem + t_lane + Sh::S_COL + s * BK + c0 / 2 + 32 * w, pw);
         }
         tmem_wait_st();
       } else {
         // row r of the swizzled [128 x 64] P tile in shared memory (one part)
         uint8_t* prow = sP + s * Sh::P_BYTES + r * 128;
+        if (none) {
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) *reinterpret_cast<uint4*>(prow + (ch << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        } else {
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
           uint32_t w[4];
@@ -446,6 +506,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
             w[e] = pack_bf16x2(p0, p1);
           }
           *reinterpret_cast<uint4*>(prow + ((ch ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
         }
         fence_async_smem();
       }
@@ -471,55 +532,63 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // rows come from the same layout in the K stages.
     const bool fin = ok && mbar_wait(ofinal, 0, a.status, kTimeoutAttention);
     const bool have_gate = fin && a.gate && mbar_wait(gfull, 0, a.status, kTimeoutAttention);
-    __syncwarp();
-    if (__all_sync(0xffffffffu, fin && (have_gate || !a.gate))) {
+    // Phase 2: a tile of sequence rows only leaves through TMA bulk stores, each
+    // 64-column atom as soon as its rows are staged; otherwise the rows leave
+    // through coalesced 16-byte stores at the end, and rows outside the
+    // sequences stay as they were.
+    const bool whole = q_first == q0 && q_end == q0 + BQ;
+    const bool out_ok = !bar_red_or(1, NT, !(fin && (have_gate || !a.gate)));  // every softmax warp agrees
+    if (out_ok) {
       tc_fence_after();
       const float inv = 1.f / l;
       bool bad = false;
 #pragma unroll 1
-      for (int c = part * DP; c < (part + 1) * DP; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
-        tmem_wait_ld();
+      for (int at = part * (DP / 64); at < (part + 1) * (DP / 64); ++at) {
+#pragma unroll 1
+        for (int c = at * 64; c < at * 64 + 64; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
+          const uint32_t base = at * (BQ * 128) + r * 128;
+          auto place = [&](int v4) { return base + (((((c >> 3) + v4) & 7) ^ (r & 7)) << 4); };
+          float sg[32];
+          if (a.gate) {  // while O is on its way
+            uint4 gq[4];
 #pragma unroll
-        for (int v4 = 0; v4 < 4; ++v4) {
-          const int chunk = (c >> 3) + v4;
-          const uint32_t off = (chunk >> 3) * (BQ * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-          float y[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
-            bad |= y[e] != y[e];
+            for (int v4 = 0; v4 < 4; ++v4) gq[v4] = *reinterpret_cast<const uint4*>(sK + place(v4));
+            sigmoid32(gq, sg);
           }
-          if (a.gate) {
-            const uint4 gq = *reinterpret_cast<const uint4*>(sK + off);
-            const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[2 * e] *= sigmoid_fast(__uint_as_float(gw[e] << 16));
-              y[2 * e + 1] *= sigmoid_fast(__uint_as_float(gw[e] & 0xffff0000u));
+          for (int v4 = 0; v4 < 4; ++v4) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
+              bad |= y[e] != y[e];
+              if (a.gate) y[e] *= sg[v4 * 8 + e];
             }
+            *reinterpret_cast<uint4*>(sQ + place(v4)) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                                   pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
           }
-          *reinterpret_cast<uint4*>(sQ + off) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                                                           pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+        }
+        if (whole && at * 64 < a.d) {
+          fence_async_smem();  // generic-proxy writes -> visible to the TMA engine
+          if (part == 0)  // the four warps of this part
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+          else
+            asm volatile("bar.sync 3, 128;" ::: "memory");
+          if (r == 0) {
+            for (int half = 0; half < 2; ++half)
+              tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
+            tma_store_commit();
+          }
         }
       }
       const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
       if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
-    }
-    fence_async_smem();  // generic-proxy writes -> visible to the TMA engine
-    asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");  // every softmax warp
-    // Phase 2: a tile of sequence rows only leaves through TMA bulk stores;
-    // otherwise its rows leave through coalesced 16-byte stores, and rows
-    // outside the sequences stay as they were.
-    const int tid = static_cast<int>(threadIdx.x) - 64;
-    if (!*abort_flag) {
-      if (q_first == q0 && q_end == q0 + BQ) {
-        if (tid == 0) {
-          for (int at = 0; at < ATOMS && at * 64 < a.d; ++at)
-            for (int half = 0; half < 2; ++half)
-              tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
-          tma_store_commit();
+      asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");  // every softmax warp
+      if (whole) {
+        if (r == 0) {
           // the staging buffer must outlive the copy; a row that is computed again must find it done
           if (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3])
             tma_store_wait_all();
@@ -528,7 +597,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         }
       } else {
         const int chunks = a.d / 8;
-        for (int idx = tid; idx < BQ * chunks; idx += NT) {
+        for (int idx = static_cast<int>(threadIdx.x) - 64; idx < BQ * chunks; idx += NT) {
           const int rr = idx / chunks, ch = idx % chunks;
           if (q0 + rr < q_first || q0 + rr >= q_end) continue;
           *reinterpret_cast<uint4*>(a.out + (q0 + rr) * a.ldo + h * a.hso + ch * 8) =
