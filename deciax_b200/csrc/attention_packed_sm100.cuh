@@ -2,20 +2,24 @@
 // cores: bf16 operands with 16-byte aligned rows, head size a multiple of 8 up
 // to 256 (computed as 64, 128 or 256: TMA reads zeros past the head's end).
 //
-// One CTA = 128 consecutive packed rows of one query head:
+// One CTA = 128 consecutive packed rows of one query head, 320 threads:
 //   warp 0      TMA producer: the Q tile, then K and V tiles through one ring
 //               each, then the gate tile into the K stages.
 //   warp 1      issues tcgen05.mma: S_t = Q K_t^T into one of two TMEM
 //               buffers, then O += P_{t-1} V_{t-1}.
-//   the others  softmax: thread r owns query row r (two warps a row at D =
-//               256, half of each key tile apiece): mask, running maximum and
-//               sum, P back over its S buffer in tensor memory (D >= 128) or
-//               into shared memory, at the end O / l * sigmoid(gate).
-// Key tiles are aligned to the query tile's end, so the diagonal is the last
-// tile (the last two at 64 keys) and only tiles that reach below some row's
-// first key need a mask besides.  The maximum moves, and O is rescaled, only
-// when it grows by more than 2^8.  A part of a tile that every row of a warp
-// masks leaves P = 0 and nothing else.
+//   warps 2..9  softmax, two warps a row (part 0 and 1: half of every key tile
+//               and half of O's columns each): mask, running maximum and sum, P
+//               as bf16 back over its S buffer, the A operand of P.V; at the end
+//               O / l * sigmoid(gate).
+// Key tiles are taken from the diagonal down.  The first one then lies beside
+// the query tile: it loads with the queries, before the tile knows where its
+// first row's sequence starts, and every row meets its own key at once.  Only
+// the diagonal and tiles that reach below some row's first key need a mask.
+// The maximum moves, and O is rescaled, only when it grows by more than 2^8.
+// A part of a tile that every row of a warp masks leaves P = 0 and nothing else.
+//
+// D = 256: 128-key tiles, one CTA an SM (Q, K and V stages fill shared memory,
+// two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs.
 //
 // Differs from attention_sm100.cuh in what bounds a row's keys, and in the
 // rounding: the sigmoid gate multiplies in FP32 and the result is rounded once.
@@ -71,14 +75,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// Sigmoids of 32 gates (bf16).  Two share one reciprocal, 1/a = b / (ab): the
+// Sigmoids of 8 Q gates (bf16).  Two share one reciprocal, 1/a = b / (ab): the
 // special-function unit, at 16 results a cycle and SM, bounds the epilogue.
 // The product of two sums 1 + e^-g stays finite while -g log2 e <= 63; a row
 // with a gate below -43, or NaN, takes a reciprocal for each.
-__device__ __forceinline__ void sigmoid32(const uint4 (&gq)[4], float (&sg)[32]) {
+template <int Q>
+__device__ __forceinline__ void sigmoids(const uint4 (&gq)[Q], float (&sg)[8 * Q]) {
   float top = -INFINITY;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < Q; ++q) {
     const uint32_t gw[4] = {gq[q].x, gq[q].y, gq[q].z, gq[q].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -89,7 +94,7 @@ __device__ __forceinline__ void sigmoid32(const uint4 (&gq)[4], float (&sg)[32])
   }
   if (top <= 63.f) {
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
+    for (int e = 0; e < 8 * Q; e += 2) {
       const float a = 1.f + ex2_approx(sg[e]), b = 1.f + ex2_approx(sg[e + 1]);
       const float r = rcp_approx(a * b);
       sg[e] = r * b;
@@ -97,15 +102,43 @@ __device__ __forceinline__ void sigmoid32(const uint4 (&gq)[4], float (&sg)[32])
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) sg[e] = rcp_approx(1.f + ex2_approx(sg[e]));
+    for (int e = 0; e < 8 * Q; ++e) sg[e] = rcp_approx(1.f + ex2_approx(sg[e]));
   }
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 template <int D>
-struct AttnPackedTcShape : AttnTcShape<D> {
-  using S = AttnTcShape<D>;
-  static constexpr int CTAS = D <= 128 ? 2 : 1;  // per SM: shared memory and 256 TMEM columns each
-  static_assert(CTAS * (S::SMEM + 1024) <= 228 * 1024, "shared memory");
+struct AttnPackedTcShape {
+  static constexpr int BQ = 128, BK = D == 256 ? 128 : 64, ATOMS = D / 64;
+  static constexpr int KST = D == 256 ? 1 : 2;   // K and V stages each
+  static constexpr int NP = 2;                   // softmax warps a row
+  static constexpr int CTAS = D == 256 ? 1 : 2;  // per SM
+  static constexpr int THREADS = 64 + 128 * NP;
+  static constexpr uint32_t Q_BYTES = BQ * D * 2;   // ATOMS x [128 rows x 128 B]
+  static constexpr uint32_t KV_BYTES = BK * D * 2;  // ATOMS x [BK rows x 128 B]
+  static constexpr uint32_t TMEM_COLS = D + 2 * BK <= 256 ? 256 : 512;
+  static constexpr uint32_t S_COL = 0, O_COL = 2 * BK;  // S buffers at 0 and BK, O after them
+  static constexpr uint32_t XCH_BYTES = 3 * NP * 128 * 4;  // row maxima [2][NP][128], sums [NP][128]
+  static constexpr size_t SMEM = 1024 + Q_BYTES + 2 * KST * KV_BYTES + 256 + XCH_BYTES;
+  static_assert(D + 2 * BK <= 512 && CTAS * TMEM_COLS <= 512, "tensor memory");
+  static_assert(Q_BYTES <= KST * KV_BYTES, "the gate tile is loaded into the K stages");
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
 template <int D, bool CAP>
@@ -123,8 +156,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + Sh::Q_BYTES;          // KST stages
   uint8_t* sV = sK + KST * Sh::KV_BYTES;   // KST stages
-  uint8_t* sP = sV + KST * Sh::KV_BYTES;   // 2 buffers (none when P lives in tensor memory)
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + (Sh::P_TMEM ? 0 : 2 * Sh::P_BYTES));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + KST * Sh::KV_BYTES);
   uint64_t* qfull = bars;
   uint64_t* kfull = bars + 1;
   uint64_t* kempty = bars + 3;
@@ -133,12 +165,11 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   uint64_t* sfull = bars + 9;
   uint64_t* sfree = bars + 11;
   uint64_t* pfull = bars + 13;
-  uint64_t* pempty = bars + 15;
-  uint64_t* ofull = bars + 17;
-  uint64_t* ofinal = bars + 18;
-  uint64_t* drain = bars + 19;
-  uint64_t* gfull = bars + 20;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* ofull = bars + 15;
+  uint64_t* ofinal = bars + 16;
+  uint64_t* drain = bars + 17;
+  uint64_t* gfull = bars + 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_begin = abort_flag + 1;  // first key of the tile's first row
   uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out NaN
@@ -146,18 +177,16 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
-  int first, total, seq_start = 0;
-  packed_extent(a, first, total);
-  if (warp == 2) packed_seq_warp(a.cu, a.n_seqs, q0, lane, seq_start);  // beside the loads of the extent
-  const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
-  if (q_first >= q_end) return;  // no row of this tile belongs to a sequence
   const int hk = h / (a.H / a.Hk);
-
+  // tile t holds keys k_end - (t + 1) BK .., possibly below the buffer (read as zero)
+  const int k_end = q0 + BQ;
+  auto load_tile = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row, int rows) {
+    for (int at = 0; at < ATOMS; ++at)
+      for (int bx = 0; bx < rows; bx += 64)
+        tma_load_3d(dst + at * (rows * 128) + bx * 128, map, bar, at * 64, head, row + bx);
+  };
   if (threadIdx.x == 0) {
-    prefetch_tmap(&maps.q);
-    prefetch_tmap(&maps.k);
-    prefetch_tmap(&maps.v);
-    for (int i = 0; i < 21; ++i) {
+    for (int i = 0; i < 19; ++i) {
       const bool softmax_arrives = (i >= 11 && i < 15);  // sfree[2], pfull[2]: one arrive per softmax thread
       mbar_init(&bars[i], softmax_arrives ? 128 * Sh::NP : 1);
     }
@@ -165,20 +194,29 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     s_nan[0] = s_nan[1] = s_nan[2] = s_nan[3] = 0u;
     fence_barrier_init();
     fence_async_smem();
-    // the query rows do not wait for the key range
+    // the queries and the first keys wait for nothing
     mbar_arrive_expect_tx(qfull, Sh::Q_BYTES);
-    for (int at = 0; at < ATOMS; ++at)
-      for (int half = 0; half < 2; ++half)
-        tma_load_3d(sQ + at * (BQ * 128) + half * (64 * 128), &maps.q, qfull, at * 64, h, q0 + half * 64);
+    load_tile(sQ, &maps.q, qfull, h, q0, BQ);
+    mbar_arrive_expect_tx(&kfull[0], Sh::KV_BYTES);
+    load_tile(sK, &maps.k, &kfull[0], hk, k_end - BK, BK);
+  }
+  int first, total, seq_start = 0;
+  packed_extent(a, first, total);
+  const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
+  if (q_first >= q_end) {  // no row of this tile belongs to a sequence
+    if (threadIdx.x == 0) {
+      mbar_wait(qfull, 0, a.status, kTimeoutDrain);
+      mbar_wait(&kfull[0], 0, a.status, kTimeoutDrain);
+    }
+    return;
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, Sh::TMEM_COLS);
     tmem_relinquish();
   }
   if (warp == 2) {
-    if (q_first != q0) {  // the first sequence starts inside the tile
-      seq_start = first;
-    }
+    packed_seq_warp(a.cu, a.n_seqs, q0, lane, seq_start);
+    if (q_first != q0) seq_start = first;  // the first sequence starts inside the tile
     const int start = min(max(seq_start, 0), q_first);
     if (lane == 0) *s_begin = a.window > 0 ? max(start, q_first - a.window + 1) : start;
   }
@@ -186,30 +224,23 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // key tiles end with the query tile (with its last row in use): tile t holds
-  // keys k_org + t BK .., the first of them possibly below the buffer (read as zero)
-  const int k_hi = q0 + (q_end - q0 + BK - 1) / BK * BK;
-  const int n = (k_hi - *s_begin + BK - 1) / BK;
-  const int k_org = k_hi - n * BK;
+  const int n = (k_end - *s_begin + BK - 1) / BK;
 
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- TMA producer ----------------
       // K runs one tile ahead of V: a K stage frees when its QK^T is done,
       // a V stage only after the (later) P.V that reads it.
-      int nk = 0, nv = 0;  // tiles whose K / V load has been issued
+      int nk = 1, nv = 0;  // tiles whose K / V load has been issued
       for (int i = 0; i <= n && !*abort_flag; ++i) {
-        if (i < n) {
+        if (i > 0 && i < n) {
           const int s = i % KST;
           if (!mbar_wait(&kempty[s], ((i / KST) & 1) ^ 1, a.status, kTimeoutAttention)) {
             *abort_flag = 1;
             break;
           }
           mbar_arrive_expect_tx(&kfull[s], Sh::KV_BYTES);
-          for (int at = 0; at < ATOMS; ++at)
-            for (int bx = 0; bx < BK / 64; ++bx)
-              tma_load_3d(sK + s * Sh::KV_BYTES + at * (BK * 128) + bx * (64 * 128), &maps.k, &kfull[s], at * 64, hk,
-                          k_org + i * BK + bx * 64);
+          load_tile(sK + s * Sh::KV_BYTES, &maps.k, &kfull[s], hk, k_end - (i + 1) * BK, BK);
           nk = i + 1;
         }
         if (i >= 1) {
@@ -219,10 +250,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
             break;
           }
           mbar_arrive_expect_tx(&vfull[s], Sh::KV_BYTES);
-          for (int at = 0; at < ATOMS; ++at)
-            for (int bx = 0; bx < BK / 64; ++bx)
-              tma_load_3d(sV + s * Sh::KV_BYTES + at * (BK * 128) + bx * (64 * 128), &maps.v, &vfull[s], at * 64, hk,
-                          k_org + u * BK + bx * 64);
+          load_tile(sV + s * Sh::KV_BYTES, &maps.v, &vfull[s], hk, k_end - i * BK, BK);
           nv = u + 1;
         }
       }
@@ -235,9 +263,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           free_ = free_ && mbar_wait(&kempty[t % KST], (t / KST) & 1, a.status, kTimeoutAttention);
         if (free_) {
           mbar_arrive_expect_tx(gfull, Sh::Q_BYTES);
-          for (int at = 0; at < ATOMS; ++at)
-            for (int half = 0; half < 2; ++half)
-              tma_load_3d(sK + at * (BQ * 128) + half * (64 * 128), &maps.gate, gfull, at * 64, h, q0 + half * 64);
+          load_tile(sK, &maps.gate, gfull, h, q0, BQ);
           gate_issued = true;
         } else {
           *abort_flag = 1;
@@ -258,7 +284,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     auto issue_pv = [&](int u) -> bool {
       const int s = u & 1, vs = u % KST;  // S/P buffer, V stage
       if (!wait(&vfull[vs], (u / KST) & 1)) return false;
-      const int live = total - (k_org + u * BK);  // value rows of this tile that belong to a sequence
+      const int live = total - (k_end - (u + 1) * BK);  // value rows of this tile that belong to a sequence
       if (live < BK) {
         // rows behind the last sequence hold anything: zero times it is not zero
         for (int i = max(live, 0) * 8 + lane; i < BK * 8; i += 32)
@@ -271,20 +297,11 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       tc_fence_after();
       if (lane == 0) {
         const uint32_t v_addr = smem_u32(sV + vs * Sh::KV_BYTES);
-        if constexpr (Sh::P_TMEM) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)  // 16 keys of P = 8 TMEM columns
-            umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8,
-                         smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
-        } else {
-          const uint32_t p_addr = smem_u32(sP + s * Sh::P_BYTES);
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            umma_bf16(tmem + Sh::O_COL, smem_desc_k128(p_addr + kk * 32),
-                      smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < BK / 16; ++kk)  // 16 keys of P = 8 TMEM columns
+          umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8,
+                       smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&vempty[vs]);
-        umma_commit(&pempty[s]);
         umma_commit(ofull);
       }
       __syncwarp();
@@ -353,24 +370,17 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
     float m = -INFINITY, l = 0.f;  // running max (log2 units, possibly stale by < 8) and this part's sum
     bool ok = true;
-    // A failed wait sets `fail`.  With one part a warp leaves the loop at
-    // once; with several, never alone: the next tile's exchange barrier ORs
-    // the flags and every part leaves together.
+    // A failed wait sets `fail`; no warp leaves alone: the next tile's exchange
+    // barrier ORs the flags and every warp leaves together.
     bool fail = false;
     for (int t = 0; t < n; ++t) {
       const int s = t & 1;
       const uint32_t ph = (t >> 1) & 1;
-      const int k0 = k_org + t * BK + c0;  // first key of this part
+      const int k0 = k_end - (t + 1) * BK + c0;  // first key of this part
       if (!fail) {
         const bool ready = mbar_wait(&sfull[s], ph, a.status, kTimeoutAttention);
         __syncwarp();
         fail = !__all_sync(0xffffffffu, ready);
-      }
-      if constexpr (NP == 1) {
-        if (fail) {
-          ok = false;
-          break;
-        }
       }
       tc_fence_after();
       uint32_t sr[BKP];
@@ -406,125 +416,76 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         for (int c = 8; c < BKP; ++c) pm[c & 7] = fmaxf(pm[c & 7], __uint_as_float(sr[c]));
         mt = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
       }
-      if constexpr (NP > 1) {
-        // both parts of a row end with the same maximum, bit for bit
-        xbuf[(s * NP + part) * 128 + r] = mt;
-        if (bar_red_or(1, NT, fail)) {
-          ok = false;
-          break;
-        }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) mt = fmaxf(mt, xbuf[(s * NP + p) * 128 + r]);
+      // both parts of a row end with the same maximum, bit for bit
+      xbuf[(s * NP + part) * 128 + r] = mt;
+      if (bar_red_or(1, NT, fail)) {
+        ok = false;
+        break;
       }
+      mt = fmaxf(mt, xbuf[(s * NP + (part ^ 1)) * 128 + r]);
       const float mn = fmaxf(m, mt * scale_log2);
       if (m == -INFINITY) m = mn;  // the row's first keys: its O and l are zero
-      {
-        // the parts of a row see the same m and mn, so they decide alike
-        const bool need = mn > m + 8.f;
-        if (__any_sync(0xffffffffu, need)) {
-          // O must hold P_{t-1} V_{t-1} before it is rescaled.
-          const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
-          __syncwarp();
-          if (!__all_sync(0xffffffffu, done)) {
-            fail = true;
-            if constexpr (NP == 1) {
-              ok = false;
-              break;
-            } else {
-              continue;
-            }
-          }
-          tc_fence_after();
-          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
-          m = mn;
-          l *= corr;
-#pragma unroll 1
-          for (int c = part * DP; c < (part + 1) * DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st32(tmem + t_lane + Sh::O_COL + c, o);
-          }
-          tmem_wait_st();
-        }
-      }
-      // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
-      const bool pe = mbar_wait(&pempty[s], ph ^ 1, a.status, kTimeoutAttention);
-      __syncwarp();
-      if (!__all_sync(0xffffffffu, pe)) {
-        fail = true;
-        if constexpr (NP == 1) {
-          ok = false;
-          break;
-        } else {
+      // the parts of a row see the same m and mn, so they decide alike
+      if (__any_sync(0xffffffffu, mn > m + 8.f)) {
+        // O must hold P_{t-1} V_{t-1} before it is rescaled.
+        const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, done)) {
+          fail = true;
           continue;
         }
+        tc_fence_after();
+        const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+        m = mn;
+        l *= corr;
+#pragma unroll 1
+        for (int c = part * DP; c < (part + 1) * DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st32(tmem + t_lane + Sh::O_COL + c, o);
+        }
+        tmem_wait_st();
       }
+      // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
+      // (its S buffer is this tile's, so the P.V that read the buffer's last P is done)
       const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
       float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if constexpr (Sh::P_TMEM) {
-        // packed as bf16 pairs over the first BK/2 columns of its S buffer
-        // (key j in column j/2): this part's keys in columns [c0/2, (c0 + BKP)/2)
+      // packed as bf16 pairs over the first BK/2 columns of the buffer (key j
+      // in column j/2): this part's keys in columns [c0/2, (c0 + BKP)/2)
 #pragma unroll
-        for (int w = 0; w < NWP / 2; ++w) {
-          uint32_t pw[32];
-          if (none) {
+      for (int w = 0; w < NWP; ++w) {
+        uint32_t pw[16];
+        if (none) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) pw[e] = 0u;
-          } else {
+          for (int e = 0; e < 16; ++e) pw[e] = 0u;
+        } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int c = 64 * w + 2 * e;
+          for (int e = 0; e < 16; ++e) {
+            const int c = 32 * w + 2 * e;
             const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), scale_log2, neg_m));
             const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), scale_log2, neg_m));
             ps[c & 7] += p0;
             ps[(c + 1) & 7] += p1;
             pw[e] = pack_bf16x2(p0, p1);
           }
-          }
-          tmem_st32(tmem + t_lane + Sh::S_COL + s * BK + c0 / 2 + 32 * w, pw);
         }
-        tmem_wait_st();
-      } else {
-        // row r of the swizzled [128 x 64] P tile in shared memory (one part)
-        uint8_t* prow = sP + s * Sh::P_BYTES + r * 128;
-        if (none) {
-#pragma unroll
-          for (int ch = 0; ch < 8; ++ch) *reinterpret_cast<uint4*>(prow + (ch << 4)) = make_uint4(0u, 0u, 0u, 0u);
-        } else {
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[ch * 8 + 2 * e]), scale_log2, neg_m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[ch * 8 + 2 * e + 1]), scale_log2, neg_m));
-            ps[2 * e] += p0;
-            ps[2 * e + 1] += p1;
-            w[e] = pack_bf16x2(p0, p1);
-          }
-          *reinterpret_cast<uint4*>(prow + ((ch ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        }
-        fence_async_smem();
+        tmem_st16(tmem + t_lane + Sh::S_COL + s * BK + c0 / 2 + 16 * w, pw);
       }
+      tmem_wait_st();
       l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
       tc_fence_before();
       mbar_arrive(&pfull[s]);
     }
     ok = ok && !fail;
     if (!ok) *abort_flag = 1;
-    if constexpr (NP > 1) {
-      // the row sum: the parts' sums, added in part order
-      float* lbuf = xbuf + 2 * NP * 128;
-      lbuf[part * 128 + r] = l;
-      asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");
-      l = 0.f;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) l += lbuf[p * 128 + r];
-    }
+    // the row sum: the parts' sums, added in part order
+    float* lbuf = xbuf + 2 * NP * 128;
+    lbuf[part * 128 + r] = l;
+    asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");
+    l = lbuf[r] + lbuf[128 + r];
     // ---------------- epilogue ----------------
     // Phase 1: thread r forms its row (its part's columns) and writes it into
     // the Q buffer (free: every MMA has completed once ofinal fires) in the
@@ -533,62 +494,64 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     const bool fin = ok && mbar_wait(ofinal, 0, a.status, kTimeoutAttention);
     const bool have_gate = fin && a.gate && mbar_wait(gfull, 0, a.status, kTimeoutAttention);
     // Phase 2: a tile of sequence rows only leaves through TMA bulk stores, each
-    // 64-column atom as soon as its rows are staged; otherwise the rows leave
-    // through coalesced 16-byte stores at the end, and rows outside the
-    // sequences stay as they were.
+    // 64-column atom as soon as its rows are staged (D = 64: the parts share the
+    // atom); otherwise the rows leave through coalesced 16-byte stores at the
+    // end, and rows outside the sequences stay as they were.
     const bool whole = q_first == q0 && q_end == q0 + BQ;
     const bool out_ok = !bar_red_or(1, NT, !(fin && (have_gate || !a.gate)));  // every softmax warp agrees
     if (out_ok) {
       tc_fence_after();
+      auto store_atom = [&](int at) {
+        for (int half = 0; half < 2; ++half)
+          tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
+        tma_store_commit();
+      };
+      constexpr int EC = D == 256 ? 32 : 16;  // columns at a time (two CTAs an SM leave 96 registers a thread)
       const float inv = 1.f / l;
       bool bad = false;
 #pragma unroll 1
-      for (int at = part * (DP / 64); at < (part + 1) * (DP / 64); ++at) {
-#pragma unroll 1
-        for (int c = at * 64; c < at * 64 + 64; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
-          const uint32_t base = at * (BQ * 128) + r * 128;
-          auto place = [&](int v4) { return base + (((((c >> 3) + v4) & 7) ^ (r & 7)) << 4); };
-          float sg[32];
-          if (a.gate) {  // while O is on its way
-            uint4 gq[4];
+      for (int c = part * DP; c < (part + 1) * DP; c += EC) {
+        uint32_t o[EC];
 #pragma unroll
-            for (int v4 = 0; v4 < 4; ++v4) gq[v4] = *reinterpret_cast<const uint4*>(sK + place(v4));
-            sigmoid32(gq, sg);
-          }
-          tmem_wait_ld();
+        for (int w = 0; w < EC; w += 16) tmem_ld16(tmem + t_lane + Sh::O_COL + c + w, o + w);
+        const uint32_t base = (c >> 6) * (BQ * 128) + r * 128;
+        auto place = [&](int v4) { return base + (((((c >> 3) + v4) & 7) ^ (r & 7)) << 4); };
+        float sg[EC];
+        if (a.gate) {  // while O is on its way
+          uint4 gq[EC / 8];
 #pragma unroll
-          for (int v4 = 0; v4 < 4; ++v4) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
-              bad |= y[e] != y[e];
-              if (a.gate) y[e] *= sg[v4 * 8 + e];
-            }
-            *reinterpret_cast<uint4*>(sQ + place(v4)) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                                                                   pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
-          }
+          for (int v4 = 0; v4 < EC / 8; ++v4) gq[v4] = *reinterpret_cast<const uint4*>(sK + place(v4));
+          sigmoids(gq, sg);
         }
-        if (whole && at * 64 < a.d) {
+        tmem_wait_ld();
+#pragma unroll
+        for (int v4 = 0; v4 < EC / 8; ++v4) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
+            bad |= y[e] != y[e];
+            if (a.gate) y[e] *= sg[v4 * 8 + e];
+          }
+          *reinterpret_cast<uint4*>(sQ + place(v4)) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                                 pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+        }
+        if (D >= 128 && whole && (c + EC) % 64 == 0 && (c & ~63) < a.d) {
           fence_async_smem();  // generic-proxy writes -> visible to the TMA engine
           if (part == 0)  // the four warps of this part
             asm volatile("bar.sync 2, 128;" ::: "memory");
           else
             asm volatile("bar.sync 3, 128;" ::: "memory");
-          if (r == 0) {
-            for (int half = 0; half < 2; ++half)
-              tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
-            tma_store_commit();
-          }
+          if (r == 0) store_atom(c >> 6);
         }
       }
       const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
       if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
+      if (D == 64 && whole) fence_async_smem();
       asm volatile("bar.sync 1, %0;" ::"r"(NT) : "memory");  // every softmax warp
       if (whole) {
         if (r == 0) {
+          if (D == 64 && part == 0) store_atom(0);
           // the staging buffer must outlive the copy; a row that is computed again must find it done
           if (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3])
             tma_store_wait_all();
