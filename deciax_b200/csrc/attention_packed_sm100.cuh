@@ -106,6 +106,17 @@ __device__ __forceinline__ void sigmoids(const uint4 (&gq)[Q], float (&sg)[8 * Q
   }
 }
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -175,7 +186,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out NaN
   float* xbuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);  // softmax parts' exchange
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from a shuffle, so that the compiler knows the warp's index, and what follows from it, to be uniform
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
   const int hk = h / (a.H / a.Hk);
   // tile t holds keys k_end - (t + 1) BK .., possibly below the buffer (read as zero)
@@ -276,8 +288,10 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       for (int t = max(0, nv - KST); t < nv; ++t) mbar_wait(&vfull[t % KST], (t / KST) & 1, a.status, kTimeoutDrain);
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer (lane 0; the warp waits together) ----------------
-    const uint32_t q_addr = smem_u32(sQ);
+    // ---------------- MMA issuer (one lane; the warp waits together) ----------------
+    // descriptors of the first stages: others are a constant further
+    const uint64_t q_desc = smem_desc_k128(smem_u32(sQ)), k_desc = smem_desc_k128(smem_u32(sK));
+    const uint64_t v_desc = smem_desc_mn128(smem_u32(sV), BK * 128);
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.status, kTimeoutAttention));
     };
@@ -295,12 +309,12 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       }
       if (!wait(&pfull[s], (u >> 1) & 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t v_addr = smem_u32(sV + vs * Sh::KV_BYTES);
+      if (elect_one()) {
+        const uint64_t v = v_desc + vs * (Sh::KV_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk)  // 16 keys of P = 8 TMEM columns
-          umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8,
-                       smem_desc_mn128(v_addr + kk * 16 * 128, BK * 128), IDESC_PV, (u > 0 || kk > 0) ? 1u : 0u);
+          umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8, v + kk * (16 * 128 >> 4), IDESC_PV,
+                       (u > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&vempty[vs]);
         umma_commit(ofull);
       }
@@ -316,13 +330,13 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         break;
       }
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t k_addr = smem_u32(sK + ks * Sh::KV_BYTES);
+      if (elect_one()) {
+        const uint64_t k = k_desc + ks * (Sh::KV_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int at = kk >> 2, w = kk & 3;
-          umma_bf16(tmem + Sh::S_COL + s * BK, smem_desc_k128(q_addr + at * (BQ * 128) + w * 32),
-                    smem_desc_k128(k_addr + at * (BK * 128) + w * 32), IDESC_QK, kk > 0 ? 1u : 0u);
+          umma_bf16(tmem + Sh::S_COL + s * BK, q_desc + ((at * (BQ * 128) + w * 32) >> 4),
+                    k + ((at * (BK * 128) + w * 32) >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
         }
         umma_commit(&kempty[ks]);
         umma_commit(&sfull[s]);
@@ -334,7 +348,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       }
     }
     ok = ok && !stopped() && issue_pv(n - 1);
-    if (lane == 0) {
+    if (elect_one()) {
       if (!ok) *abort_flag = 1;
       umma_commit(ofinal);
       umma_commit(drain);
