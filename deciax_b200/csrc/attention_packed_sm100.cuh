@@ -2,12 +2,12 @@
 // cores: bf16 operands with 16-byte aligned rows, head size a multiple of 8 up
 // to 256 (computed as 64, 128 or 256: TMA reads zeros past the head's end).
 //
-// One CTA = 128 consecutive packed rows of one query head, 320 threads:
+// One CTA = 128 consecutive packed rows of one query head, 352 threads:
 //   warp 0      TMA producer: the Q tile, then K and V tiles through one ring
 //               each, then the gate tile into the K stages.
-//   warp 1      issues tcgen05.mma: S_t = Q K_t^T into one of two TMEM
-//               buffers, then O += P_{t-1} V_{t-1}.
-//   warps 2..9  softmax, two warps a row (part 0 and 1: half of every key tile
+//   warp 1      issues tcgen05.mma: S_t = Q K_t^T into one of two TMEM buffers.
+//   warp 2      issues O += P_t V_t.
+//   warps 3..10 softmax, two warps a row (part 0 and 1: half of every key tile
 //               and half of O's columns each): mask, running maximum and sum, P
 //               as bf16 back over its S buffer, the A operand of P.V; at the end
 //               O / l * sigmoid(gate).
@@ -19,7 +19,9 @@
 // A part of a tile that every row of a warp masks leaves P = 0 and nothing else.
 //
 // D = 256: 128-key tiles, one CTA an SM (Q, K and V stages fill shared memory,
-// two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs.
+// two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs
+// (128-key tiles leave room for one S buffer: the two CTAs then took turns, and
+// serving batches ran 10% slower).
 //
 // Differs from attention_sm100.cuh in what bounds a row's keys, and in the
 // rounding: the sigmoid gate multiplies in FP32 and the result is rounded once.
@@ -140,7 +142,8 @@ struct AttnPackedTcShape {
   static constexpr int KST = D == 256 ? 1 : 2;   // K and V stages each
   static constexpr int NP = 2;                   // softmax warps a row
   static constexpr int CTAS = D == 256 ? 1 : 2;  // per SM
-  static constexpr int THREADS = 64 + 128 * NP;
+  static constexpr int FIRST = 96;               // first softmax thread
+  static constexpr int THREADS = FIRST + 128 * NP;
   static constexpr uint32_t Q_BYTES = BQ * D * 2;   // ATOMS x [128 rows x 128 B]
   static constexpr uint32_t KV_BYTES = BK * D * 2;  // ATOMS x [BK rows x 128 B]
   static constexpr uint32_t TMEM_COLS = D + 2 * BK <= 256 ? 256 : 512;
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     attn_packed_tc_kernel(const __grid_constant__ AttnPackedMaps maps,
                           const __grid_constant__ AttnPackedArgs<__nv_bfloat16> a) {
   using Sh = AttnPackedTcShape<D>;
-  constexpr int BQ = Sh::BQ, BK = Sh::BK, ATOMS = Sh::ATOMS, KST = Sh::KST;
+  constexpr int BQ = Sh::BQ, BK = Sh::BK, ATOMS = Sh::ATOMS, KST = Sh::KST, BKP = BK / Sh::NP;
   constexpr uint32_t IDESC_QK = idesc_bf16_f32(BQ, BK);
   constexpr uint32_t IDESC_PV = idesc_bf16_f32(BQ, D) | (1u << 16);  // B (V) is MN-major
   constexpr float LOG2E = 1.4426950408889634f;
@@ -174,13 +177,13 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   uint64_t* vfull = bars + 5;
   uint64_t* vempty = bars + 7;
   uint64_t* sfull = bars + 9;
-  uint64_t* sfree = bars + 11;
-  uint64_t* pfull = bars + 13;
+  uint64_t* pfull = bars + 11;
+  uint64_t* pempty = bars + 13;
   uint64_t* ofull = bars + 15;
   uint64_t* ofinal = bars + 16;
-  uint64_t* drain = bars + 17;
-  uint64_t* gfull = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* drain = bars + 17;  // [2]
+  uint64_t* gfull = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_begin = abort_flag + 1;  // first key of the tile's first row
   uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out NaN
@@ -198,8 +201,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         tma_load_3d(dst + at * (rows * 128) + bx * 128, map, bar, at * 64, head, row + bx);
   };
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 19; ++i) {
-      const bool softmax_arrives = (i >= 11 && i < 15);  // sfree[2], pfull[2]: one arrive per softmax thread
+    for (int i = 0; i < 20; ++i) {
+      const bool softmax_arrives = (i >= 11 && i < 13);  // pfull[2]: one arrive per softmax thread
       mbar_init(&bars[i], softmax_arrives ? 128 * Sh::NP : 1);
     }
     *abort_flag = 0;
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     tmem_alloc(tmem_slot, Sh::TMEM_COLS);
     tmem_relinquish();
   }
-  if (warp == 2) {
+  if (warp == 3) {
     packed_seq_warp(a.cu, a.n_seqs, q0, lane, seq_start);
     if (q_first != q0) seq_start = first;  // the first sequence starts inside the tile
     const int start = min(max(seq_start, 0), q_first);
@@ -287,13 +290,34 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       for (int t = max(0, nk - KST); t < nk; ++t) mbar_wait(&kfull[t % KST], (t / KST) & 1, a.status, kTimeoutDrain);
       for (int t = max(0, nv - KST); t < nv; ++t) mbar_wait(&vfull[t % KST], (t / KST) & 1, a.status, kTimeoutDrain);
     }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer (one lane; the warp waits together) ----------------
-    // descriptors of the first stages: others are a constant further
+  } else if (warp < 3) {
+    // ---------------- MMA issuers (one lane; the warp waits together) ----------------
+    // Issue is serial work (8 or 16 instructions and four waits a tile cost 2000
+    // cycles in one warp): warp 1 issues S_t = Q K_t^T, warp 2 O += P_t V_t.
+    // Descriptors of the first stages; others are a constant further.
     const uint64_t q_desc = smem_desc_k128(smem_u32(sQ)), k_desc = smem_desc_k128(smem_u32(sK));
     const uint64_t v_desc = smem_desc_mn128(smem_u32(sV), BK * 128);
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.status, kTimeoutAttention));
+    };
+    auto issue_qk = [&](int t) -> bool {
+      const int s = t & 1, ks = t % KST;  // S buffer, K stage
+      // the buffer is free when the P.V that read the P in it is done
+      if (!wait(&kfull[ks], (t / KST) & 1) || !wait(&pempty[s], ((t >> 1) & 1) ^ 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t k = k_desc + ks * (Sh::KV_BYTES >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int at = kk >> 2, w = kk & 3;
+          umma_bf16(tmem + Sh::S_COL + s * BK, q_desc + ((at * (BQ * 128) + w * 32) >> 4),
+                    k + ((at * (BK * 128) + w * 32) >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&kempty[ks]);
+        umma_commit(&sfull[s]);
+      }
+      __syncwarp();
+      return true;
     };
     auto issue_pv = [&](int u) -> bool {
       const int s = u & 1, vs = u % KST;  // S/P buffer, V stage
@@ -312,47 +336,26 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       if (elect_one()) {
         const uint64_t v = v_desc + vs * (Sh::KV_BYTES >> 4);
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk)  // 16 keys of P = 8 TMEM columns
-          umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + kk * 8, v + kk * (16 * 128 >> 4), IDESC_PV,
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          // 16 keys of P = 8 TMEM columns, each part's from the start of its share of S
+          const int p_col = kk * 16 / BKP * BKP + kk * 16 % BKP / 2;
+          umma_bf16_ts(tmem + Sh::O_COL, tmem + Sh::S_COL + s * BK + p_col, v + kk * (16 * 128 >> 4), IDESC_PV,
                        (u > 0 || kk > 0) ? 1u : 0u);
+        }
         umma_commit(&vempty[vs]);
+        umma_commit(&pempty[s]);
         umma_commit(ofull);
       }
       __syncwarp();
       return true;
     };
-    bool ok = wait(qfull, 0);
-    auto stopped = [&] { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };  // the same answer in every lane
-    for (int t = 0; ok && t < n; ++t) {
-      const int s = t & 1, ks = t % KST;  // S buffer, K stage
-      if (stopped() || !wait(&kfull[ks], (t / KST) & 1) || !wait(&sfree[s], ((t >> 1) & 1) ^ 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t k = k_desc + ks * (Sh::KV_BYTES >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const int at = kk >> 2, w = kk & 3;
-          umma_bf16(tmem + Sh::S_COL + s * BK, q_desc + ((at * (BQ * 128) + w * 32) >> 4),
-                    k + ((at * (BK * 128) + w * 32) >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&kempty[ks]);
-        umma_commit(&sfull[s]);
-      }
-      __syncwarp();
-      if (t >= 1 && !issue_pv(t - 1)) {
-        ok = false;
-        break;
-      }
-    }
-    ok = ok && !stopped() && issue_pv(n - 1);
+    bool ok = warp == 2 || wait(qfull, 0);
+    for (int t = 0; ok && t < n; ++t) ok = warp == 1 ? issue_qk(t) : issue_pv(t);
     if (elect_one()) {
       if (!ok) *abort_flag = 1;
-      umma_commit(ofinal);
-      umma_commit(drain);
-      mbar_wait(drain, 0, a.status, kTimeoutDrain);
+      if (warp == 2) umma_commit(ofinal);
+      umma_commit(&drain[warp - 1]);
+      mbar_wait(&drain[warp - 1], 0, a.status, kTimeoutDrain);
     }
   } else {
     // ---------------- softmax / epilogue warps ----------------
@@ -360,9 +363,9 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // [p BKP, (p + 1) BKP) of every tile and O columns [p D/NP, (p + 1) D/NP).
     // The parts exchange their tile maxima through shared memory (one
     // barrier per tile); their row sums are added once, at the end.
-    constexpr int NP = Sh::NP, BKP = BK / NP, NWP = BKP / 32, NT = 128 * NP, DP = D / NP;
+    constexpr int NP = Sh::NP, NWP = BKP / 32, NT = 128 * NP, DP = D / NP;
     const int q4 = warp & 3;  // TMEM lane quarter
-    const int part = (warp - 2) >> 2;
+    const int part = (warp - 3) >> 2;
     const int c0 = part * BKP;  // this part's first key column within a tile
     const int r = q4 * 32 + lane;
     const int row = q0 + r;
@@ -379,6 +382,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     }
     // over the warp's rows: keys below lo_min or above its last row are masked for all of them
     const int lo_max = __reduce_max_sync(0xffffffffu, lo), lo_min = __reduce_min_sync(0xffffffffu, lo);
+    const int w_first = q0 + q4 * 32, w_last = w_first + 31;
     const uint32_t t_lane = static_cast<uint32_t>(q4 * 32) << 16;
     const float scale = rsqrtf(static_cast<float>(a.d));
     const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
@@ -389,54 +393,49 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     bool fail = false;
     for (int t = 0; t < n; ++t) {
       const int s = t & 1;
-      const uint32_t ph = (t >> 1) & 1;
       const int k0 = k_end - (t + 1) * BK + c0;  // first key of this part
       if (!fail) {
-        const bool ready = mbar_wait(&sfull[s], ph, a.status, kTimeoutAttention);
+        const bool ready = mbar_wait(&sfull[s], (t >> 1) & 1, a.status, kTimeoutAttention);
         __syncwarp();
         fail = !__all_sync(0xffffffffu, ready);
       }
       tc_fence_after();
-      uint32_t sr[BKP];
+      const uint32_t s_at = tmem + t_lane + Sh::S_COL + s * BK + c0;  // this part's scores, then its P
+      uint32_t sr[NWP][32];
+      // 32 keys that every row of the warp masks: short sequences, a window's edge
+      auto none = [&](int w) { return k0 + 32 * w > w_last || k0 + 32 * w + 31 < lo_min; };
+      float mt = -INFINITY;
       if (!fail) {
 #pragma unroll
-        for (int w = 0; w < NWP; ++w)
-          tmem_ld32(tmem + t_lane + Sh::S_COL + s * BK + c0 + 32 * w, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * w]));
+        for (int w = 0; w < NWP; ++w) tmem_ld32(s_at + 32 * w, sr[w]);
         tmem_wait_ld();
-        tc_fence_before();
-        mbar_arrive(&sfree[s]);
-      }
-      // every key of this part is masked for every row of the warp: short sequences, a window's edge
-      const bool none = k0 > q0 + q4 * 32 + 31 || k0 + BKP - 1 < lo_min;
-      if constexpr (CAP) {
-        if (!none) {
+        float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < BKP; ++c)
-            sr[c] = __float_as_uint(packed_score(__uint_as_float(sr[c]), scale, a.softcap));
+        for (int w = 0; w < NWP; ++w) {
+          if (none(w)) continue;
+          const int k = k0 + 32 * w;
+          if constexpr (CAP) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              sr[w][c] = __float_as_uint(packed_score(__uint_as_float(sr[w][c]), scale, a.softcap));
+          }
+          if (k + 31 > w_first || k < lo_max) {  // some key is masked for some row of the warp
+            const int top = row - k, low = lo - k;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) sr[w][c] = c >= low && c <= top ? sr[w][c] : 0xff800000u;  // -inf
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pm[c & 3] = fmaxf(pm[c & 3], __uint_as_float(sr[w][c]));
         }
-      }
-      float mt = -INFINITY;
-      if (!none) {
-        if (k0 + BKP - 1 > q0 + q4 * 32 || k0 < lo_max) {  // some key of this part is masked for some row of the warp
-          const int top = row - k0, low = lo - k0;
-#pragma unroll
-          for (int c = 0; c < BKP; ++c) sr[c] = c >= low && c <= top ? sr[c] : 0xff800000u;  // -inf
-        }
-        // Row max with 8 independent partial maxima (short dependency chains).
-        float pm[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sr[e]);
-#pragma unroll
-        for (int c = 8; c < BKP; ++c) pm[c & 7] = fmaxf(pm[c & 7], __uint_as_float(sr[c]));
-        mt = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
+        mt = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
       }
       // both parts of a row end with the same maximum, bit for bit
-      xbuf[(s * NP + part) * 128 + r] = mt;
+      xbuf[((t & 1) * NP + part) * 128 + r] = mt;
       if (bar_red_or(1, NT, fail)) {
         ok = false;
         break;
       }
-      mt = fmaxf(mt, xbuf[(s * NP + (part ^ 1)) * 128 + r]);
+      mt = fmaxf(mt, xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r]);
       const float mn = fmaxf(m, mt * scale_log2);
       if (m == -INFINITY) m = mn;  // the row's first keys: its O and l are zero
       // the parts of a row see the same m and mn, so they decide alike
@@ -464,32 +463,30 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         tmem_wait_st();
       }
       // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
-      // (its S buffer is this tile's, so the P.V that read the buffer's last P is done)
       const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
-      float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      // packed as bf16 pairs over the first BK/2 columns of the buffer (key j
-      // in column j/2): this part's keys in columns [c0/2, (c0 + BKP)/2)
+      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+      // packed as bf16 pairs from the start of this part's scores (key j in
+      // column j/2), which only this warp reads
 #pragma unroll
       for (int w = 0; w < NWP; ++w) {
         uint32_t pw[16];
-        if (none) {
+        if (none(w)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) pw[e] = 0u;
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int c = 32 * w + 2 * e;
-            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c]), scale_log2, neg_m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + 1]), scale_log2, neg_m));
-            ps[c & 7] += p0;
-            ps[(c + 1) & 7] += p1;
+            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[w][2 * e]), scale_log2, neg_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[w][2 * e + 1]), scale_log2, neg_m));
+            ps[2 * e & 3] += p0;
+            ps[(2 * e + 1) & 3] += p1;
             pw[e] = pack_bf16x2(p0, p1);
           }
         }
-        tmem_st16(tmem + t_lane + Sh::S_COL + s * BK + c0 / 2 + 16 * w, pw);
+        tmem_st16(s_at + 16 * w, pw);
       }
       tmem_wait_st();
-      l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
       tc_fence_before();
       mbar_arrive(&pfull[s]);
     }
@@ -574,7 +571,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         }
       } else {
         const int chunks = a.d / 8;
-        for (int idx = static_cast<int>(threadIdx.x) - 64; idx < BQ * chunks; idx += NT) {
+        for (int idx = static_cast<int>(threadIdx.x) - Sh::FIRST; idx < BQ * chunks; idx += NT) {
           const int rr = idx / chunks, ch = idx % chunks;
           if (q0 + rr < q_first || q0 + rr >= q_end) continue;
           *reinterpret_cast<uint4*>(a.out + (q0 + rr) * a.ldo + h * a.hso + ch * 8) =
