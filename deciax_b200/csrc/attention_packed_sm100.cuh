@@ -15,8 +15,13 @@
 // the query tile: it loads with the queries, before the tile knows where its
 // first row's sequence starts, and every row meets its own key at once.  Only
 // the diagonal and tiles that reach below some row's first key need a mask.
-// The maximum moves, and O is rescaled, only when it grows by more than 2^8.
-// A part of a tile that every row of a warp masks leaves P = 0 and nothing else.
+// P is taken against the maximum of the tiles before the last one: the row's
+// parts then exchange their maxima while P.V runs instead of before it (bf16
+// has FP32's exponents, so a P above 1 loses nothing).  The maximum moves, and O
+// is rescaled, only when it grows by more than 2^8.  A row whose scores jump by
+// more than 2^127 from one tile to the next comes out infinite, and is computed
+// again like one that came out NaN.  32 keys that every row of a warp masks
+// leave P = 0 and nothing else.
 //
 // D = 256: 128-key tiles, one CTA an SM (Q, K and V stages fill shared memory,
 // two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_begin = abort_flag + 1;  // first key of the tile's first row
-  uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out NaN
+  uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out infinite or NaN
   float* xbuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);  // softmax parts' exchange
 
   // from a shuffle, so that the compiler knows the warp's index, and what follows from it, to be uniform
@@ -386,10 +391,13 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     const uint32_t t_lane = static_cast<uint32_t>(q4 * 32) << 16;
     const float scale = rsqrtf(static_cast<float>(a.d));
     const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
-    float m = -INFINITY, l = 0.f;  // running max (log2 units, possibly stale by < 8) and this part's sum
+    // m: the maximum P is taken against (log2 units), at most 8 below that of the
+    // tiles before the last; l: this part's sum; last: this part's maximum of the last tile
+    float m = -INFINITY, l = 0.f, last = -INFINITY;
+    const int t_own = (k_end - 1 - w_last) / BK;  // the tile with the warp's own rows' keys: the first it sees
     bool ok = true;
-    // A failed wait sets `fail`; no warp leaves alone: the next tile's exchange
-    // barrier ORs the flags and every warp leaves together.
+    // A failed wait sets `fail`; the two warps of a row leave together, by their
+    // next exchange barrier, and the others by their own waits.
     bool fail = false;
     for (int t = 0; t < n; ++t) {
       const int s = t & 1;
@@ -404,12 +412,21 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       uint32_t sr[NWP][32];
       // 32 keys that every row of the warp masks: short sequences, a window's edge
       auto none = [&](int w) { return k0 + 32 * w > w_last || k0 + 32 * w + 31 < lo_min; };
-      float mt = -INFINITY;
+      float mt = -INFINITY;  // this part's row maximum (log2 units)
+      auto row_max = [&] {
+        float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int w = 0; w < NWP; ++w)
+          if (!none(w)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pm[c & 3] = fmaxf(pm[c & 3], __uint_as_float(sr[w][c]));
+          }
+        mt = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * scale_log2;
+      };
       if (!fail) {
 #pragma unroll
         for (int w = 0; w < NWP; ++w) tmem_ld32(s_at + 32 * w, sr[w]);
         tmem_wait_ld();
-        float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int w = 0; w < NWP; ++w) {
           if (none(w)) continue;
@@ -424,43 +441,48 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 #pragma unroll
             for (int c = 0; c < 32; ++c) sr[w][c] = c >= low && c <= top ? sr[w][c] : 0xff800000u;  // -inf
           }
-#pragma unroll
-          for (int c = 0; c < 32; ++c) pm[c & 3] = fmaxf(pm[c & 3], __uint_as_float(sr[w][c]));
         }
-        mt = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
       }
-      // both parts of a row end with the same maximum, bit for bit
-      xbuf[((t & 1) * NP + part) * 128 + r] = mt;
-      if (bar_red_or(1, NT, fail)) {
-        ok = false;
-        break;
-      }
-      mt = fmaxf(mt, xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r]);
-      const float mn = fmaxf(m, mt * scale_log2);
-      if (m == -INFINITY) m = mn;  // the row's first keys: its O and l are zero
-      // the parts of a row see the same m and mn, so they decide alike
-      if (__any_sync(0xffffffffu, mn > m + 8.f)) {
-        // O must hold P_{t-1} V_{t-1} before it is rescaled.
-        const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
-        __syncwarp();
-        if (!__all_sync(0xffffffffu, done)) {
-          fail = true;
-          continue;
+      if (t == t_own) {
+        // the rows' first keys: the parts agree on their maximum at once
+        row_max();
+        xbuf[((t & 1) * NP + part) * 128 + r] = mt;
+        if (bar_red_or(4 + q4, 32 * NP, fail)) {
+          ok = false;
+          break;
         }
-        tc_fence_after();
-        const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
-        m = mn;
-        l *= corr;
+        m = fmaxf(mt, xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r]);
+      } else if (t > t_own + 1) {
+        // later the maximum of the tile before: this one's P may be large
+        if (bar_red_or(4 + q4, 32 * NP, fail)) {
+          ok = false;
+          break;
+        }
+        const float mn = fmaxf(fmaxf(m, last), xbuf[(((t - 1) & 1) * NP + (part ^ 1)) * 128 + r]);
+        // the parts of a row see the same m and mn, so they decide alike
+        if (__any_sync(0xffffffffu, mn > m + 8.f)) {
+          // O must hold P_{t-1} V_{t-1} before it is rescaled.
+          const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, done)) {
+            fail = true;
+            continue;
+          }
+          tc_fence_after();
+          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+          m = mn;
+          l *= corr;
 #pragma unroll 1
-        for (int c = part * DP; c < (part + 1) * DP; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(tmem + t_lane + Sh::O_COL + c, o);
-          tmem_wait_ld();
+          for (int c = part * DP; c < (part + 1) * DP; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-          tmem_st32(tmem + t_lane + Sh::O_COL + c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
+          }
+          tmem_wait_st();
         }
-        tmem_wait_st();
       }
       // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
       const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
@@ -486,9 +508,14 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         tmem_st16(s_at + 16 * w, pw);
       }
       tmem_wait_st();
-      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
       tc_fence_before();
       mbar_arrive(&pfull[s]);
+      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      if (t > t_own) {  // for the next tile, while P.V runs
+        row_max();
+        last = mt;
+        xbuf[((t & 1) * NP + part) * 128 + r] = mt;
+      }
     }
     ok = ok && !fail;
     if (!ok) *abort_flag = 1;
@@ -519,7 +546,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       };
       constexpr int EC = D == 256 ? 32 : 16;  // columns at a time (two CTAs an SM leave 96 registers a thread)
       const float inv = 1.f / l;
-      bool bad = false;
+      bool bad = !(l < INFINITY);
 #pragma unroll 1
       for (int c = part * DP; c < (part + 1) * DP; c += EC) {
         uint32_t o[EC];
@@ -541,7 +568,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
-            bad |= y[e] != y[e];
+            bad |= !(fabsf(y[e]) < INFINITY);
             if (a.gate) y[e] *= sg[v4 * 8 + e];
           }
           *reinterpret_cast<uint4*>(sQ + place(v4)) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),

@@ -365,6 +365,12 @@ def test_attention_packed_long_rows_with_large_scores(d):
     check_attention([1500, 20, 600], 2, 1, d, qscale=6.0)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_packed_scores_that_jump(d):
+    """Scores of some +-2000: they grow by more than FP32's range from one key tile to the next."""
+    check_attention([400, 7, 300], 2, 1, d, qscale=500.0, pad=9)
+
+
 @pytest.mark.parametrize("dtype,tokens", [("bf16", 4500), ("fp32", 1100)])
 def test_attention_packed_benchmark_heads(dtype, tokens):
     check_attention([tokens], 16, 8, 256, dtype)
