@@ -51,6 +51,11 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {  // into L2
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 // Every store of this thread's bulk groups is complete, not only read.
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
@@ -77,39 +82,79 @@ __device__ __forceinline__ int packed_seq_warp(const int32_t* cu, int n, int row
   return lo;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Two FP32 operations in one instruction, on register pairs.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
   return r;
 }
-// Sigmoids of 8 Q gates (bf16).  Two share one reciprocal, 1/a = b / (ab): the
-// special-function unit, at 16 results a cycle and SM, bounds the epilogue.
+__device__ __forceinline__ float2 unpair2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Sigmoids of 8 Q gates (bf16).  Two share one reciprocal, 1/a = b / (ab), for
+// the special-function unit gives 16 results a cycle and SM (exponentials from
+// the FMA pipe instead, for a quarter or half of them, were no faster).
 // The product of two sums 1 + e^-g stays finite while -g log2 e <= 63; a row
 // with a gate below -43, or NaN, takes a reciprocal for each.
 template <int Q>
-__device__ __forceinline__ void sigmoids(const uint4 (&gq)[Q], float (&sg)[8 * Q]) {
+__device__ __forceinline__ void sigmoids(const uint4 (&gq)[Q], uint64_t (&sg)[4 * Q]) {
+  const uint64_t neg_log2e = pair2(-1.4426950408889634f, -1.4426950408889634f);
   float top = -INFINITY;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     const uint32_t gw[4] = {gq[q].x, gq[q].y, gq[q].z, gq[q].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sg[8 * q + 2 * e] = __uint_as_float(gw[e] << 16) * -1.4426950408889634f;
-      sg[8 * q + 2 * e + 1] = __uint_as_float(gw[e] & 0xffff0000u) * -1.4426950408889634f;
-      top = max_nan(top, max_nan(sg[8 * q + 2 * e], sg[8 * q + 2 * e + 1]));
+      sg[4 * q + e] = mul2(pair2(__uint_as_float(gw[e] << 16), __uint_as_float(gw[e] & 0xffff0000u)), neg_log2e);
+      const float2 t = unpair2(sg[4 * q + e]);
+      top = max3_nan(top, t.x, t.y);
     }
   }
+  const uint64_t one = pair2(1.f, 1.f);
   if (top <= 63.f) {
 #pragma unroll
-    for (int e = 0; e < 8 * Q; e += 2) {
-      const float a = 1.f + ex2_approx(sg[e]), b = 1.f + ex2_approx(sg[e + 1]);
-      const float r = rcp_approx(a * b);
-      sg[e] = r * b;
-      sg[e + 1] = r * a;
+    for (int e = 0; e < 4 * Q; ++e) {
+      const float2 t = unpair2(sg[e]);
+      const uint64_t ab = add2(one, pair2(ex2_approx(t.x), ex2_approx(t.y)));
+      const float2 d = unpair2(ab);
+      const float r = rcp_approx(d.x * d.y);
+      sg[e] = mul2(pair2(r, r), pair2(d.y, d.x));
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8 * Q; ++e) sg[e] = rcp_approx(1.f + ex2_approx(sg[e]));
+    for (int e = 0; e < 4 * Q; ++e) {
+      const float2 t = unpair2(sg[e]);
+      sg[e] = pair2(rcp_approx(1.f + ex2_approx(t.x)), rcp_approx(1.f + ex2_approx(t.y)));
+    }
   }
 }
 
@@ -196,7 +241,11 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 
   // from a shuffle, so that the compiler knows the warp's index, and what follows from it, to be uniform
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * BQ, h = blockIdx.y;
+  // heads_at_once heads after the others; of them every head's last tiles first (the longest, where sequences are long)
+  const int tiles = gridDim.x / a.H, round = blockIdx.x / (tiles * a.heads_at_once);
+  const int in_round = blockIdx.x % (tiles * a.heads_at_once);
+  const int h = round * a.heads_at_once + in_round % a.heads_at_once;
+  const int q0 = (tiles - 1 - in_round / a.heads_at_once) * BQ;
   const int hk = h / (a.H / a.Hk);
   // tile t holds keys k_end - (t + 1) BK .., possibly below the buffer (read as zero)
   const int k_end = q0 + BQ;
@@ -249,6 +298,10 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- TMA producer ----------------
+      // The gate tile's place frees late (below): it waits for it in L2.
+      if (a.gate)
+        for (int at = 0; at < ATOMS; ++at)
+          for (int half = 0; half < 2; ++half) tma_prefetch_3d(&maps.gate, at * 64, h, q0 + half * 64);
       // K runs one tile ahead of V: a K stage frees when its QK^T is done,
       // a V stage only after the (later) P.V that reads it.
       int nk = 1, nv = 0;  // tiles whose K / V load has been issued
@@ -419,7 +472,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         for (int w = 0; w < NWP; ++w)
           if (!none(w)) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) pm[c & 3] = fmaxf(pm[c & 3], __uint_as_float(sr[w][c]));
+            for (int c = 0; c < 32; c += 2)
+              pm[c / 2 & 3] = max3(pm[c / 2 & 3], __uint_as_float(sr[w][c]), __uint_as_float(sr[w][c + 1]));
           }
         mt = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * scale_log2;
       };
@@ -486,7 +540,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       }
       // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
       const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
-      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pair2(scale_log2, scale_log2), neg_m2 = pair2(neg_m, neg_m);
+      uint64_t ps[2] = {0ull, 0ull};  // sums of even and odd keys
       // packed as bf16 pairs from the start of this part's scores (key j in
       // column j/2), which only this warp reads
 #pragma unroll
@@ -498,10 +553,9 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[w][2 * e]), scale_log2, neg_m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[w][2 * e + 1]), scale_log2, neg_m));
-            ps[2 * e & 3] += p0;
-            ps[(2 * e + 1) & 3] += p1;
+            const float2 x = unpair2(fma2(pair2(__uint_as_float(sr[w][2 * e]), __uint_as_float(sr[w][2 * e + 1])), scale2, neg_m2));
+            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+            ps[e & 1] = add2(ps[e & 1], pair2(p0, p1));
             pw[e] = pack_bf16x2(p0, p1);
           }
         }
@@ -510,7 +564,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&pfull[s]);
-      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      const float2 sum = unpair2(add2(ps[0], ps[1]));
+      l += sum.x + sum.y;
       if (t > t_own) {  // for the next tile, while P.V runs
         row_max();
         last = mt;
@@ -529,8 +584,25 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // the Q buffer (free: every MMA has completed once ofinal fires) in the
     // TMA layout [atom][128 rows][128 B] with the 128-byte swizzle; the gate
     // rows come from the same layout in the K stages.
+    // The first PRE of a thread's chunks have their gates ready before the last
+    // P.V is done: half of the gates' time passes in that wait.
+    constexpr int EC = D == 256 ? 32 : 16, NC = DP / EC, PRE = D == 256 ? 3 : 2;  // columns a chunk, chunks
+    auto place = [&](int c, int v4) {  // 16 bytes of row r, columns c + 8 v4 ..
+      return (c >> 6) * (BQ * 128) + r * 128 + (((((c >> 3) + v4) & 7) ^ (r & 7)) << 4);
+    };
+    auto gates = [&](int c, uint64_t (&sg)[EC / 2]) {
+      uint4 gq[EC / 8];
+#pragma unroll
+      for (int v4 = 0; v4 < EC / 8; ++v4) gq[v4] = *reinterpret_cast<const uint4*>(sK + place(c, v4));
+      sigmoids(gq, sg);
+    };
+    uint64_t early[PRE][EC / 2];
+    const bool have_gate = ok && a.gate && mbar_wait(gfull, 0, a.status, kTimeoutAttention);
+    if (have_gate) {
+#pragma unroll
+      for (int i = 0; i < PRE; ++i) gates(part * DP + i * EC, early[i]);
+    }
     const bool fin = ok && mbar_wait(ofinal, 0, a.status, kTimeoutAttention);
-    const bool have_gate = fin && a.gate && mbar_wait(gfull, 0, a.status, kTimeoutAttention);
     // Phase 2: a tile of sequence rows only leaves through TMA bulk stores, each
     // 64-column atom as soon as its rows are staged (D = 64: the parts share the
     // atom); otherwise the rows leave through coalesced 16-byte stores at the
@@ -544,35 +616,38 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           tma_store_3d(&maps.out, sQ + at * (BQ * 128) + half * (64 * 128), at * 64, h, q0 + half * 64);
         tma_store_commit();
       };
-      constexpr int EC = D == 256 ? 32 : 16;  // columns at a time (two CTAs an SM leave 96 registers a thread)
       const float inv = 1.f / l;
-      bool bad = !(l < INFINITY);
-#pragma unroll 1
-      for (int c = part * DP; c < (part + 1) * DP; c += EC) {
+      const uint64_t inv2 = pair2(inv, inv);
+      uint64_t odd2 = 0ull;  // sum of 0 * y: NaN once a y is infinite or NaN
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = part * DP + i * EC;
         uint32_t o[EC];
 #pragma unroll
         for (int w = 0; w < EC; w += 16) tmem_ld16(tmem + t_lane + Sh::O_COL + c + w, o + w);
-        const uint32_t base = (c >> 6) * (BQ * 128) + r * 128;
-        auto place = [&](int v4) { return base + (((((c >> 3) + v4) & 7) ^ (r & 7)) << 4); };
-        float sg[EC];
-        if (a.gate) {  // while O is on its way
-          uint4 gq[EC / 8];
+        uint64_t sg[EC / 2];
+        if (a.gate) {
+          if (i < PRE) {
 #pragma unroll
-          for (int v4 = 0; v4 < EC / 8; ++v4) gq[v4] = *reinterpret_cast<const uint4*>(sK + place(v4));
-          sigmoids(gq, sg);
+            for (int e = 0; e < EC / 2; ++e) sg[e] = early[i < PRE ? i : 0][e];
+          } else {
+            gates(c, sg);  // while O is on its way
+          }
         }
         tmem_wait_ld();
 #pragma unroll
         for (int v4 = 0; v4 < EC / 8; ++v4) {
-          float y[8];
+          uint32_t yw[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            y[e] = __uint_as_float(o[v4 * 8 + e]) * inv;
-            bad |= !(fabsf(y[e]) < INFINITY);
-            if (a.gate) y[e] *= sg[v4 * 8 + e];
+          for (int e = 0; e < 4; ++e) {
+            const int at = v4 * 4 + e;
+            uint64_t y = mul2(pair2(__uint_as_float(o[2 * at]), __uint_as_float(o[2 * at + 1])), inv2);
+            odd2 = fma2(y, 0ull, odd2);
+            if (a.gate) y = mul2(y, sg[at]);
+            const float2 yy = unpair2(y);
+            yw[e] = pack_bf16x2(yy.x, yy.y);
           }
-          *reinterpret_cast<uint4*>(sQ + place(v4)) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                                                                 pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+          *reinterpret_cast<uint4*>(sQ + place(c, v4)) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
         }
         if (D >= 128 && whole && (c + EC) % 64 == 0 && (c & ~63) < a.d) {
           fence_async_smem();  // generic-proxy writes -> visible to the TMA engine
@@ -583,6 +658,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           if (r == 0) store_atom(c >> 6);
         }
       }
+      const float2 odd = unpair2(odd2);
+      const bool bad = !(l < INFINITY) || odd.x != 0.f || odd.y != 0.f;
       const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
       if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
       if (D == 64 && whole) fence_async_smem();

@@ -152,16 +152,28 @@ static void launch_packed_simt(const AttnPackedArgs<T>& a, cudaStream_t st) {
   CUDA_CHECK(cudaGetLastError());
 }
 
+// Heads whose tiles run side by side: all of them let the longest tiles of
+// every head start first (24 records of 16384 rows, 32 heads of 128: 300 us
+// against 320 us eight heads at a time), as long as the keys and values that
+// they read stay within three quarters of L2 (one sequence of 16384, 16 heads
+// of 256: all at once 1680 us, four or eight 1600 us).
+static int packed_heads_at_once(const AttnPackedArgs<bf16>& a) {
+  const long long kv_bytes = 4LL * a.tokens * a.d;
+  int kv = static_cast<int>(std::max(1LL, std::min<long long>(a.Hk, (96LL << 20) / std::max(1LL, kv_bytes))));
+  while (a.Hk % kv) --kv;
+  return kv * (a.H / a.Hk);
+}
+
 template <int D, bool CAP>
 static void launch_packed_tc(const AttnPackedMaps& maps, const AttnPackedArgs<bf16>& a, cudaStream_t st) {
   using Sh = AttnPackedTcShape<D>;
   allow_smem(attn_packed_tc_kernel<D, CAP>, Sh::SMEM);
-  attn_packed_tc_kernel<D, CAP><<<dim3((a.tokens + 127) / 128, a.H), Sh::THREADS, Sh::SMEM, st>>>(maps, a);
+  attn_packed_tc_kernel<D, CAP><<<(a.tokens + 127) / 128 * a.H, Sh::THREADS, Sh::SMEM, st>>>(maps, a);
   CUDA_CHECK(cudaGetLastError());
 }
 
 template <typename T>
-static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
+static void attention_packed(AttnPackedArgs<T> a, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     // TMA needs 16-byte aligned rows; everything else runs on the CUDA cores
     const auto rows = [](const void* p, long long ld, long long hs, int heads) {
@@ -175,6 +187,7 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
       maps.v = tmap_bf16_heads(a.v, a.tokens, a.Hk, a.d, a.ldv, a.hsv);
       maps.gate = a.gate ? tmap_bf16_heads(a.gate, a.tokens, a.H, a.d, a.ldg, a.hsg) : maps.q;
       maps.out = tmap_bf16_heads(a.out, a.tokens, a.H, a.d, a.ldo, a.hso);
+      a.heads_at_once = packed_heads_at_once(a);
       const bool cap = a.softcap > 0.f;
       if (a.d <= 64)
         cap ? launch_packed_tc<64, true>(maps, a, st) : launch_packed_tc<64, false>(maps, a, st);
@@ -393,6 +406,7 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
     REQUIRE(tokens <= 1 << 30, "at most 2^30 tokens");
     REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be a multiple of key/value heads");
     REQUIRE(hq <= 65535, "at most 65535 query heads");
+    REQUIRE((static_cast<long long>(tokens) + 127) / 128 * hq < 1LL << 31, "too many query tiles");
     REQUIRE(d > 0 && d <= 256, "attention head size must be in [1, 256]");
     REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must not be negative (0 = off)");
     REQUIRE(window >= 0, "window must not be negative (0 = off)");
