@@ -41,7 +41,6 @@ struct AttnPackedArgs {
   float softcap;
   int window;
   int* status;
-  int heads_at_once;  // tensor cores: query heads whose tiles run side by side
 };
 
 // The packed rows that belong to a sequence: [first, total).  Whatever cu

@@ -241,11 +241,9 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
 
   // from a shuffle, so that the compiler knows the warp's index, and what follows from it, to be uniform
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  // heads_at_once heads after the others; of them every head's last tiles first (the longest, where sequences are long)
-  const int tiles = gridDim.x / a.H, round = blockIdx.x / (tiles * a.heads_at_once);
-  const int in_round = blockIdx.x % (tiles * a.heads_at_once);
-  const int h = round * a.heads_at_once + in_round % a.heads_at_once;
-  const int q0 = (tiles - 1 - in_round / a.heads_at_once) * BQ;
+  // grid (heads side by side, tiles, rounds of heads): of a round's heads the
+  // last tiles come first, the longest where sequences are long
+  const int h = blockIdx.z * gridDim.x + blockIdx.x, q0 = (static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y)) * BQ;
   const int hk = h / (a.H / a.Hk);
   // tile t holds keys k_end - (t + 1) BK .., possibly below the buffer (read as zero)
   const int k_end = q0 + BQ;

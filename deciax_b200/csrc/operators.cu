@@ -168,12 +168,13 @@ template <int D, bool CAP>
 static void launch_packed_tc(const AttnPackedMaps& maps, const AttnPackedArgs<bf16>& a, cudaStream_t st) {
   using Sh = AttnPackedTcShape<D>;
   allow_smem(attn_packed_tc_kernel<D, CAP>, Sh::SMEM);
-  attn_packed_tc_kernel<D, CAP><<<(a.tokens + 127) / 128 * a.H, Sh::THREADS, Sh::SMEM, st>>>(maps, a);
+  const int heads = packed_heads_at_once(a);
+  attn_packed_tc_kernel<D, CAP><<<dim3(heads, (a.tokens + 127) / 128, a.H / heads), Sh::THREADS, Sh::SMEM, st>>>(maps, a);
   CUDA_CHECK(cudaGetLastError());
 }
 
 template <typename T>
-static void attention_packed(AttnPackedArgs<T> a, cudaStream_t st) {
+static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     // TMA needs 16-byte aligned rows; everything else runs on the CUDA cores
     const auto rows = [](const void* p, long long ld, long long hs, int heads) {
@@ -187,7 +188,6 @@ static void attention_packed(AttnPackedArgs<T> a, cudaStream_t st) {
       maps.v = tmap_bf16_heads(a.v, a.tokens, a.Hk, a.d, a.ldv, a.hsv);
       maps.gate = a.gate ? tmap_bf16_heads(a.gate, a.tokens, a.H, a.d, a.ldg, a.hsg) : maps.q;
       maps.out = tmap_bf16_heads(a.out, a.tokens, a.H, a.d, a.ldo, a.hso);
-      a.heads_at_once = packed_heads_at_once(a);
       const bool cap = a.softcap > 0.f;
       if (a.d <= 64)
         cap ? launch_packed_tc<64, true>(maps, a, st) : launch_packed_tc<64, false>(maps, a, st);
@@ -403,10 +403,9 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
   return op_guarded([&] {
     size_of(dtype);
     REQUIRE(n_seqs >= 0 && tokens >= 0, "sequences and tokens must not be negative");
-    REQUIRE(tokens <= 1 << 30, "at most 2^30 tokens");
+    REQUIRE(tokens <= 65535 * 128, "at most 8388480 tokens");
     REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be a multiple of key/value heads");
     REQUIRE(hq <= 65535, "at most 65535 query heads");
-    REQUIRE((static_cast<long long>(tokens) + 127) / 128 * hq < 1LL << 31, "too many query tiles");
     REQUIRE(d > 0 && d <= 256, "attention head size must be in [1, 256]");
     REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must not be negative (0 = off)");
     REQUIRE(window >= 0, "window must not be negative (0 = off)");

@@ -321,7 +321,7 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
  * outside [cu_seqlens[0], cu_seqlens[n_seqs]) belong to no sequence, are not
  * read as keys, may hold anything, and their out is left as it was.  Infinities
  * and NaN of one sequence never reach another.  out must not overlap the
- * inputs.  d <= 256; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
+ * inputs.  d <= 256, tokens <= 8388480; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
  * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; anything
  * else on the CUDA cores in FP32. */
 int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,

@@ -61,7 +61,7 @@ def attention(lib, **kw):
 
 
 ATTENTION_REFUSED = [
-    dict(dtype=-1), dict(n_seqs=-1), dict(tokens=-1), dict(tokens=(1 << 30) + 1), dict(hq=0), dict(hkv=0), dict(hkv=3), dict(hq=65536, hkv=1),
+    dict(dtype=-1), dict(n_seqs=-1), dict(tokens=-1), dict(tokens=65535 * 128 + 1), dict(hq=0), dict(hkv=0), dict(hkv=3), dict(hq=65536, hkv=1),
     dict(d=0), dict(d=264), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(window=-1), dict(q=None),
     dict(k=None), dict(v=None), dict(out=None), dict(cu=None), dict(hsq=64), dict(ldk=127), dict(ldv=-256), dict(hsg=0), dict(hso=8),
 ]
