@@ -264,8 +264,8 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   const int dev = current_device();
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = a.dim % kVec == 0 && a.ldh % kVec == 0 && a.ldw % kVec == 0 && aligned16(a.hidden) && aligned16(a.head);
-  const bool tc = sizeof(T) == 2 && vec;
-  const bool pair = tc && a.rows > 128;
+  const bool tc = vec;  // 16-byte aligned rows
+  const bool pair = tc && sizeof(T) == 2 && a.rows > 128;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   int workers = sm_count(dev);
@@ -288,14 +288,12 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   else if (pair)
     logprob_runs(a, 256, 32, false, workers);
   else
-    logprob_runs(a, 256, 8, true, workers);
+    logprob_runs(a, sizeof(T) == 2 ? 256 : 128, 8, true, workers);
   const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(a.num_m) * a.splits, workers));
   const size_t states = static_cast<size_t>(a.splits) * a.rows;
-  OpScratch scratch(states * (3 + 2 * static_cast<size_t>(a.top)) * 4, st);
-  a.part_m = static_cast<float*>(scratch.p);
-  a.part_s = a.part_m + states;
-  a.part_t = a.part_s + states;
-  a.list_x = a.part_t + states;
+  OpScratch scratch(states * (4 + 2 * static_cast<size_t>(a.top)) * 4, st);
+  a.part = static_cast<float4*>(scratch.p);
+  a.list_x = reinterpret_cast<float*>(a.part + states);
   a.list_id = reinterpret_cast<int32_t*>(a.list_x + states * a.top);
   if constexpr (sizeof(T) == 2) {
     if (tc) {
@@ -314,18 +312,17 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
       }
     }
   }
-  auto simt = [&](auto kern) {
-    allow_smem(kern, logprob_simt_smem(kTopMax));
-    kern<<<grid, 256, logprob_simt_smem(a.top), st>>>(a);
-    CUDA_CHECK(cudaGetLastError());
-  };
   if constexpr (sizeof(T) == 4) {
-    if (vec)
-      simt(token_logprobs_simt_kernel<T, true, CAP>);
-    else
-      simt(token_logprobs_simt_kernel<T, false, CAP>);
-  } else {
-    if (!tc) simt(token_logprobs_simt_kernel<T, false, CAP>);
+    if (tc) {
+      allow_smem(token_logprobs_f32_tc_kernel<CAP>, LogprobF32Shape::smem(kTopMax));
+      token_logprobs_f32_tc_kernel<CAP><<<grid, LogprobF32Shape::THREADS, LogprobF32Shape::smem(a.top), st>>>(a);
+      CUDA_CHECK(cudaGetLastError());
+    }
+  }
+  if (!tc) {
+    allow_smem(token_logprobs_simt_kernel<T, CAP>, logprob_simt_smem(kTopMax));
+    token_logprobs_simt_kernel<T, CAP><<<grid, 256, logprob_simt_smem(a.top), st>>>(a);
+    CUDA_CHECK(cudaGetLastError());
   }
   auto finish = [&](auto kern) {
     allow_smem(kern, static_cast<size_t>(kLogprobMaxSplits) * kTopMax * 8);

@@ -15,8 +15,8 @@
 //
 // With s and t joined at m = max m_i:  H = ln s - ln2 t / s.
 //
-// Here: the state, the joining kernel, and the CUDA-core form (FP32 operands, or
-// rows that are not 16-byte aligned).  token_logprobs_sm100.cuh has the tensor-core form.
+// Here: the state, the joining kernel, and the CUDA-core form (rows that are not
+// 16-byte aligned).  token_logprobs_sm100.cuh has the tensor-core form.
 #pragma once
 
 #include "common.cuh"
@@ -36,11 +36,9 @@ struct LogprobArgs {
   // units of work: num_m row tiles x `splits` runs of `run` columns, in tiles of `tile`
   int num_m, splits, run, tile;
   int copies;  // tensor cores, at most 32 (64) rows: the row tile holds them four times (twice)
-  // scratch: per (split, row) the state, then the list
-  float* part_m;
-  float* part_s;
-  float* part_t;
-  float* list_x;    // [splits][rows][top], largest first
+  // scratch, a row's splits side by side: states {m, s, t, 0} and lists
+  float4* part;     // [rows][splits]
+  float* list_x;    // [rows][splits][top], largest first
   int32_t* list_id;
   int* status;
 };
@@ -172,10 +170,8 @@ __device__ __forceinline__ void join_state(RowState& st, float m, float s, float
 // Leaves the state in scratch, and the list in order.
 __device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, int split, int row, float* lx,
                                             const int32_t* lid, int r) {
-  const size_t at = static_cast<size_t>(split) * a.rows + row;
-  a.part_m[at] = st.m;
-  a.part_s[at] = st.s;
-  a.part_t[at] = st.t;
+  const size_t at = static_cast<size_t>(row) * a.splits + split;
+  a.part[at] = make_float4(st.m, st.s, st.t, 0.f);
   unsigned taken = 0u;  // top <= 32
   for (int j = 0; j < a.top; ++j) {
     float x = -INFINITY;
@@ -226,7 +222,7 @@ __device__ __forceinline__ void load8(const T* p, int k, int dim, bool live, flo
   }
 }
 
-template <typename T, bool VEC, bool CAP>
+template <typename T, bool CAP>
 __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_constant__ LogprobArgs a) {
   extern __shared__ __align__(16) float lp_smem[];
   float(*sA)[132] = reinterpret_cast<float(*)[132]>(lp_smem);
@@ -247,8 +243,8 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
       const T* pb = static_cast<const T*>(a.head) + static_cast<long long>(n0 + lr) * a.ldw;
       const bool lb = n0 + lr < a.vocab;
       float va[8], vb[8], acc[8][8] = {};
-      load8<T, VEC>(pa, lk, a.dim, la, va);
-      load8<T, VEC>(pb, lk, a.dim, lb, vb);
+      load8<T, false>(pa, lk, a.dim, la, va);
+      load8<T, false>(pb, lk, a.dim, lb, vb);
       for (int k0 = 0; k0 < a.dim; k0 += 16) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -257,8 +253,8 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
         }
         __syncthreads();
         if (k0 + 16 < a.dim) {
-          load8<T, VEC>(pa, k0 + 16 + lk, a.dim, la, va);
-          load8<T, VEC>(pb, k0 + 16 + lk, a.dim, lb, vb);
+          load8<T, false>(pa, k0 + 16 + lk, a.dim, la, va);
+          load8<T, false>(pb, k0 + 16 + lk, a.dim, lb, vb);
         }
 #pragma unroll
         for (int kk = 0; kk < 16; ++kk) {
@@ -364,17 +360,14 @@ __global__ void __launch_bounds__(128) token_logprobs_finish_kernel(const __grid
 #pragma unroll
   for (int o = 0; o < kLogprobMaxSplits / 128; ++o) {
     const int i = tid + 128 * o;
-    const size_t at = static_cast<size_t>(i) * a.rows + row;
-    const bool in = i < a.splits;
-    pm[o] = in ? a.part_m[at] : -INFINITY;
-    ps[o] = in ? a.part_s[at] : 0.f;
-    pt[o] = in ? a.part_t[at] : 0.f;
-    m = fmaxf(m, pm[o]);
+    const float4 p = i < a.splits ? a.part[static_cast<size_t>(row) * a.splits + i] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    pm[o] = p.x, ps[o] = p.y, pt[o] = p.z;
+    m = fmaxf(m, p.x);
   }
-  for (int e = tid; e < a.splits * a.top; e += 128) {
-    const size_t at = (static_cast<size_t>(e / a.top) * a.rows + row) * a.top + e % a.top;
-    fin_x[e] = a.list_x[at];
-    fin_id[e] = a.list_id[at];
+  const int entries = a.splits * a.top;
+  for (int e = tid; e < entries; e += 128) {
+    fin_x[e] = a.list_x[static_cast<size_t>(row) * entries + e];
+    fin_id[e] = a.list_id[static_cast<size_t>(row) * entries + e];
   }
   m = warp_max(m);
   if (lane == 0) s_red[0][warp] = m;

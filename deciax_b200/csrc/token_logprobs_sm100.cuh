@@ -300,4 +300,262 @@ __global__ void __launch_bounds__(192, 1)
   }
 }
 
+// ---------------------------------------------------------------------------
+// FP32 operands: each value as three bf16 (24 bits of mantissa in 3 x 8), six products
+// ---------------------------------------------------------------------------
+//
+//   x = h + m + l,  h = bf16(x), m = bf16(x - h), l = bf16(x - h - m)   (exact)
+//   x y = hh' + hm' + mh' + hl' + lh' + mm'  + terms below 2^-24 of |x y|
+//
+// Six tensor-core products of 16 cycles a column replace the 64 FMA cycles that
+// the CUDA cores need: 128 rows x 128 columns x 64 deep take 1540 cycles of MMA
+// against 4096 of FMA.  The split costs 5.5 operations a value:
+//   warps 0..15  two groups take turns: load a 64-deep step into registers,
+//                write it as swizzled bf16 tiles, hidden and head, three of each
+//                (one group of eight warps could not hide its loads: 95 us for
+//                97 rows x 32003 x 1024)
+//   warp 16      issues the products
+//   warps 17..20 thread = row: scan
+// The accumulator cuts off below its last bit at every step, so the five small
+// products, 5 of 6 steps, have an accumulator of their own, 2^-8 as large.
+// Roofline at few rows: the head's bytes; else 6 x the bf16 products.
+struct LogprobF32Shape {
+  static constexpr int BM = 128, BN = 128, BK = 64, STAGES = 2, THREADS = 21 * 32;
+  static constexpr uint32_t TILE = 128 * BK * 2;  // one bf16 tile of 128 rows
+  static constexpr uint32_t TMEM_COLS = 512;  // two tiles of 128 columns: h h', and the small products
+  static constexpr size_t smem(int top) { return 1024 + STAGES * 6 * TILE + 256 + 128 * 8 * static_cast<size_t>(top); }
+};
+
+// A pair's three bf16 parts, packed (of an infinity: one infinity and two NaN).
+__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const uint64_t minus = pair2(-1.f, -1.f);
+  auto rest = [&](uint64_t v, uint32_t part) {
+    return fma2(pair2(__uint_as_float(part << 16), __uint_as_float(part & 0xffff0000u)), minus, v);
+  };
+  h = pack_bf16x2(x, y);
+  const uint64_t r = rest(pair2(x, y), h);
+  const float2 rf = unpair2(r);
+  m = pack_bf16x2(rf.x, rf.y);
+  const float2 lf = unpair2(rest(r, m));
+  l = pack_bf16x2(lf.x, lf.y);
+}
+
+template <bool CAP>
+__global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
+    token_logprobs_f32_tc_kernel(const __grid_constant__ LogprobArgs args) {
+  using S = LogprobF32Shape;
+  constexpr int BM = S::BM, BN = S::BN, BK = S::BK, STAGES = S::STAGES;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * 6 * S::TILE);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* lx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);
+  int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * args.top);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int units = args.num_m * args.splits;
+  const int num_kb = (args.dim + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 256);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);  // one arrive per epilogue warp
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 16) {
+    tmem_alloc(tmem_slot, S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp < 16) {
+    // thread: elements 4 j .. 4 j + 3 and 32 + 4 j .. of rows r0, r0 + 32, .. of both operands, of every other step
+    const int stage = warp >> 3, r0 = (threadIdx.x & 255) >> 3, j = threadIdx.x & 7;
+    float4 next[16];
+    int unit = blockIdx.x, c = 0, c_end = 0, kb = 0;  // the step: unit, its tile's first column, 64 of dim
+    const float *pa = nullptr, *pb = nullptr;  // this thread's first element of the tile's operands
+    uint32_t there = 0;                        // bit i: its i-th row exists (four of hidden, four of head)
+    auto tile = [&] {
+      const int m = unit % args.num_m * BM + r0;
+      pa = static_cast<const float*>(args.hidden) + m * args.ldh + 4 * j;
+      pb = static_cast<const float*>(args.head) + (c + r0) * args.ldw + 4 * j;
+      there = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        there |= (m + 32 * i < args.rows ? 1u : 0u) << i;
+        there |= (r0 + 32 * i < args.tile && c + r0 + 32 * i < args.vocab ? 16u : 0u) << i;
+      }
+    };
+    auto begin = [&] {
+      if (unit < units) {
+        c = run_begin(args, unit / args.num_m);
+        c_end = run_begin(args, unit / args.num_m + 1);
+        tile();
+      }
+    };
+    auto advance = [&] {
+      if (++kb < num_kb) return;
+      kb = 0;
+      c += args.tile;
+      if (c < c_end) {
+        tile();
+      } else {
+        unit += gridDim.x;
+        begin();
+      }
+    };
+    const long long step_a = 32 * args.ldh, step_b = 32 * args.ldw;
+    auto load = [&] {
+      if (unit >= units) return;
+      const int k = kb * BK + 4 * j;
+      const uint32_t low = k < args.dim ? there : 0u, high = k + 32 < args.dim ? there : 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* p = (i < 4 ? pa + i * step_a : pb + (i - 4) * step_b) + kb * BK;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        next[2 * i] = (low >> i) & 1u ? *reinterpret_cast<const float4*>(p) : zero;
+        next[2 * i + 1] = (high >> i) & 1u ? *reinterpret_cast<const float4*>(p + 32) : zero;
+      }
+    };
+    begin();
+    if (stage == 1 && unit < units) advance();
+    load();
+    uint32_t phase = 0;
+    bool ok = true;
+    while (unit < units) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, args.status, kTimeoutProducer));
+      if (!ok) break;
+      uint8_t* dst = smem + stage * 6 * S::TILE;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = r0 + 32 * (i / 2 & 3), chunk = (i & 1) * 4 + j / 2;
+        uint2 h, m, l;
+        split3(next[i].x, next[i].y, h.x, m.x, l.x);
+        split3(next[i].z, next[i].w, h.y, m.y, l.y);
+        uint8_t* p = dst + (i < 8 ? 0 : 3 * S::TILE) + r * 128 + ((chunk ^ (r & 7)) << 4) + (j & 1) * 8;
+        *reinterpret_cast<uint2*>(p) = h;
+        *reinterpret_cast<uint2*>(p + S::TILE) = m;
+        *reinterpret_cast<uint2*>(p + 2 * S::TILE) = l;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&full[stage]);
+      phase ^= 1;
+      advance();
+      if (unit < units) advance();
+      load();
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp == 16) {
+    const uint32_t idesc = idesc_bf16_f32(BM, (args.tile + 15) / 16 * 16);
+    const uint64_t desc = smem_desc_k128(smem_u32(smem));
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, args.status, kTimeoutMma));
+    };
+    int stage = 0, local = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+      const int split = unit / args.num_m;
+      const int c_end = run_begin(args, split + 1);
+      for (int c = run_begin(args, split); ok && c < c_end; c += args.tile, ++local) {
+        const int acc = local & 1;
+        ok = wait(&tempty[acc], ((local >> 1) & 1) ^ 1);
+        tc_fence_after();
+        for (int kb = 0; ok && kb < num_kb; ++kb) {
+          ok = wait(&full[stage], phase);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t a = desc + stage * (6 * S::TILE >> 4), b = a + (3 * S::TILE >> 4);
+            constexpr int A[6] = {0, 2, 0, 1, 1, 0}, B[6] = {0, 0, 2, 1, 0, 1};  // h h', then l h', h l', m m', m h', h m'
+            const uint32_t d = tmem_base + acc * 2 * BN;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+#pragma unroll
+              for (int p = 0; p < 6; ++p)
+                umma_bf16(p == 0 ? d : d + BN, a + ((A[p] * S::TILE + k * 32) >> 4), b + ((B[p] * S::TILE + k * 32) >> 4),
+                          idesc, (kb > 0 || k > 0 || p > 1) ? 1u : 0u);
+            umma_commit(&empty[stage]);
+          }
+          __syncwarp();
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+        if (ok && elect_one()) umma_commit(&tfull[acc]);
+        __syncwarp();
+      }
+    }
+    if (elect_one()) {
+      if (!ok) *abort_flag = 1;
+      umma_commit(drain);
+      mbar_wait(drain, 0, args.status, kTimeoutDrain);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter; row of the tile
+    int local = 0;
+    bool ok = true;
+    for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+      const int split = unit / args.num_m, row = unit % args.num_m * BM + r;
+      const int c_end = run_begin(args, split + 1);
+      const bool any = row - lane < args.rows;  // some row of this warp exists
+      RowState st;
+      list_clear(lx, lid, args.top, r);
+      for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
+        const int acc = local & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue));
+        if (!ok) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + acc * 2 * BN + (static_cast<uint32_t>(q * 32) << 16);
+        if (any) {
+          const int cols = min(args.tile, c_end - c0);
+#pragma unroll 1
+          for (int c = 0; c < cols; c += 32) {
+            float x[32];
+#pragma unroll
+            for (int half = 0; half < 32; half += 16) {
+              uint32_t v[16], w[16];
+              tmem_ld16(taddr + c + half, v);
+              tmem_ld16(taddr + BN + c + half, w);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[half + e] = __uint_as_float(v[e]) + __uint_as_float(w[e]);
+            }
+            if (row < args.rows) scan32<CAP>(st, x, c0 + c, cols - c, args.softcap, lx, lid, args.top, r);
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+      }
+      if (ok && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+    }
+  }
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 16) tmem_dealloc(tmem_base, S::TMEM_COLS);
+}
+
 }  // namespace clef

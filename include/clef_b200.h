@@ -342,8 +342,9 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
  * x, largest first, equal ones by the lowest id (top <= 32).  Products and sums
  * are FP32 and x is not rounded.  n_targets = 0, entropy = NULL and top = 0 leave
  * an output out; rows = 0 does nothing.  A row with a NaN logit has NaN logprobs
- * and entropy.  bf16 with 16-byte aligned rows (pointers, ldh, ldw, dim % 8 == 0)
- * runs on the tensor cores.  Scratch comes from the library's stream-ordered
+ * and entropy.  16-byte aligned rows (pointers, ldh and ldw, whole 16 bytes of
+ * dim) run on the tensor cores, FP32 values as three bf16 parts each (what is left
+ * out of a product is below 2^-24 of it).  Scratch comes from the library's stream-ordered
  * pool: make one call on each device before capturing one into a graph. */
 int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const void* lm_head, int64_t ldw, int rows, int vocab,
                            int dim, float softcap, const int32_t* targets, int n_targets, float* logprobs, float* entropy,

@@ -545,6 +545,29 @@ def test_token_logprobs_of_a_sharp_distribution(dtype):
     check_logprobs(140, 3000, 1024, dtype, std=0.1)
 
 
+@pytest.mark.parametrize("n,dim,dtype", [(5, 1024, "fp32"), (150, 516, "fp32"), (60, 1022, "fp32"), (5, 1024, "bf16"), (300, 2048, "bf16")])
+def test_token_logprobs_of_full_mantissas(n, dim, dtype):
+    """Values off the grid: every product and sum rounds.  The alternatives' scores have to be the largest up to the tolerance."""
+    import torch
+
+    g = generator(n)
+    hidden, head = normal(g, n, dim, dtype=dtype), normal(g, 5000, dim, dtype=dtype, std=0.05)
+    targets = torch.randint(0, 5000, (n, 3), generator=g, device="cuda", dtype=torch.int32)
+    logp, ent, ids, best = run_logprobs(hidden, head, targets, 6)
+    z = hidden.double() @ head.double().T
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    want = z - lse
+    e = 2 * (dim + 8) * U32 * (hidden.double().abs() @ head.double().abs().T).amax(1, keepdim=True)
+    tol = 2 * e + (5000 / 32 + 64) * U32 + 2.0**-20 + 2 * U32 * (z.abs() + lse.abs())
+    assert ((logp.double() - want.gather(1, targets.long())).abs() <= tol.gather(1, targets.long())).all()
+    assert ((best.double() - want.gather(1, ids.long())).abs() <= tol.gather(1, ids.long())).all()
+    assert ((best.double() - torch.topk(want, 6, 1).values).abs() <= 2 * tol.amax(1, keepdim=True)).all()
+    assert (ids.sort(1).values.diff(dim=1) > 0).all()
+    p = want.exp()
+    assert ((ent.double() + (p * want).sum(1)).abs() <= (4 * e[:, 0] + 2 * (5000 / 32 + 64) * U32 + 2.0**-19) * ((p * (z - z.amax(1, keepdim=True)).abs()).sum(1) + 1)).all()
+    print("mean error in units of 2^-24", ((logp.double() - want.gather(1, targets.long())).abs().mean() / U32).item())
+
+
 def test_token_logprobs_every_token_is_an_alternative():
     check_logprobs(130, 32, 64, "bf16", top=32)
     check_logprobs(3, 5, 64, "fp32", top=5)
