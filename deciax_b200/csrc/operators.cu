@@ -291,7 +291,11 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
     logprob_runs(a, sizeof(T) == 2 ? 256 : 128, 8, true, workers);
   const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(a.num_m) * a.splits, workers));
   const size_t states = static_cast<size_t>(a.splits) * a.rows;
-  OpScratch scratch(states * (4 + 2 * static_cast<size_t>(a.top)) * 4, st);
+  // FP32 on the tensor cores: the hidden states' three parts behind the states and lists
+  const int dim_split = (a.dim + 7) / 8 * 8;
+  const size_t state_bytes = (states * (4 + 2 * static_cast<size_t>(a.top)) * 4 + 255) / 256 * 256;
+  const size_t split_bytes = tc && sizeof(T) == 4 ? 3 * static_cast<size_t>(a.rows) * dim_split * 2 : 0;
+  OpScratch scratch(state_bytes + split_bytes, st);
   a.part = static_cast<float4*>(scratch.p);
   a.list_x = reinterpret_cast<float*>(a.part + states);
   a.list_id = reinterpret_cast<int32_t*>(a.list_x + states * a.top);
@@ -315,7 +319,13 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
     if (tc) {
       allow_smem(token_logprobs_f32_tc_kernel<CAP>, LogprobF32Shape::smem(kTopMax));
-      token_logprobs_f32_tc_kernel<CAP><<<grid, LogprobF32Shape::THREADS, LogprobF32Shape::smem(a.top), st>>>(a);
+      bf16* parts = reinterpret_cast<bf16*>(static_cast<uint8_t*>(scratch.p) + state_bytes);
+      const long long runs8 = static_cast<long long>(a.rows) * (dim_split / 8);
+      split_rows_kernel<<<static_cast<int>((runs8 + 255) / 256), 256, 0, st>>>(static_cast<const float*>(a.hidden), a.ldh,
+                                                                               a.rows, a.dim, dim_split, parts);
+      CUDA_CHECK(cudaGetLastError());
+      const CUtensorMap ta = tmap_bf16(parts, 3ULL * a.rows, dim_split, dim_split, hidden_box(a.rows));
+      token_logprobs_f32_tc_kernel<CAP><<<grid, LogprobF32Shape::THREADS, LogprobF32Shape::smem(a.top), st>>>(ta, a);
       CUDA_CHECK(cudaGetLastError());
     }
   }

@@ -309,18 +309,19 @@ __global__ void __launch_bounds__(192, 1)
 //
 // Six tensor-core products of 16 cycles a column replace the 64 FMA cycles that
 // the CUDA cores need: 128 rows x 128 columns x 64 deep take 1540 cycles of MMA
-// against 4096 of FMA.  The split costs 5.5 operations a value:
-//   warps 0..15  two groups take turns: load a 64-deep step into registers,
-//                write it as swizzled bf16 tiles, hidden and head, three of each
-//                (one group of eight warps could not hide its loads: 95 us for
-//                97 rows x 32003 x 1024)
+// against 4096 of FMA.  The hidden states are split once, into scratch; the head
+// is split on its way into shared memory, 5.5 operations a value:
+//   warps 0..15  two groups take turns: load a 64-deep step of head rows into
+//                registers, write it as three swizzled bf16 tiles
 //   warp 16      issues the products
 //   warps 17..20 thread = row: scan
+//   warp 21      loads the hidden states' three tiles by TMA
+// Bound by shared memory at 128 columns: the products read 192 KB a step, the
+// tiles' writes are 96 KB (2300 cycles at 128 bytes a cycle).
 // The accumulator cuts off below its last bit at every step, so the five small
 // products, 5 of 6 steps, have an accumulator of their own, 2^-8 as large.
-// Roofline at few rows: the head's bytes; else 6 x the bf16 products.
 struct LogprobF32Shape {
-  static constexpr int BM = 128, BN = 128, BK = 64, STAGES = 2, THREADS = 21 * 32;
+  static constexpr int BM = 128, BN = 128, BK = 64, STAGES = 2, THREADS = 22 * 32;
   static constexpr uint32_t TILE = 128 * BK * 2;  // one bf16 tile of 128 rows
   static constexpr uint32_t TMEM_COLS = 512;  // two tiles of 128 columns: h h', and the small products
   static constexpr size_t smem(int top) { return 1024 + STAGES * 6 * TILE + 256 + 128 * 8 * static_cast<size_t>(top); }
@@ -340,9 +341,29 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& 
   l = pack_bf16x2(lf.x, lf.y);
 }
 
+// out[p][row][dim_out]: part p of the rows' values, eight a thread; dim_out = dim rounded up to 8.
+__global__ void __launch_bounds__(256)
+    split_rows_kernel(const float* __restrict__ x, long long ldx, int rows, int dim, int dim_out, __nv_bfloat16* out) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = dim_out / 8;
+  if (i >= static_cast<long long>(rows) * per_row) return;
+  const int row = static_cast<int>(i / per_row), k = static_cast<int>(i % per_row) * 8;
+  float v[8];
+  load8<float, true>(x + row * ldx, k, dim, true, v);
+  uint4 h, m, l;
+  split3(v[0], v[1], h.x, m.x, l.x);
+  split3(v[2], v[3], h.y, m.y, l.y);
+  split3(v[4], v[5], h.z, m.z, l.z);
+  split3(v[6], v[7], h.w, m.w, l.w);
+  const long long plane = static_cast<long long>(rows) * dim_out, at = static_cast<long long>(row) * dim_out + k;
+  *reinterpret_cast<uint4*>(out + at) = h;
+  *reinterpret_cast<uint4*>(out + plane + at) = m;
+  *reinterpret_cast<uint4*>(out + 2 * plane + at) = l;
+}
+
 template <bool CAP>
 __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
-    token_logprobs_f32_tc_kernel(const __grid_constant__ LogprobArgs args) {
+    token_logprobs_f32_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ LogprobArgs args) {
   using S = LogprobF32Shape;
   constexpr int BM = S::BM, BN = S::BN, BK = S::BK, STAGES = S::STAGES;
 
@@ -364,7 +385,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 256);
+      mbar_init(&full[s], 257);  // a group of splitting threads, and the TMA warp
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -385,22 +406,19 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp < 16) {
-    // thread: elements 4 j .. 4 j + 3 and 32 + 4 j .. of rows r0, r0 + 32, .. of both operands, of every other step
-    const int stage = warp >> 3, r0 = (threadIdx.x & 255) >> 3, j = threadIdx.x & 7;
-    float4 next[16];
+    // thread: elements 4 j .. 4 j + 3 of both halves of head rows r0, r0 + 32, ..,
+    // of every other step; odd rows take their halves in the other order, so that a
+    // warp's stores meet every bank
+    const int stage = warp >> 3, r0 = (threadIdx.x & 255) >> 3, j = threadIdx.x & 7, half0 = (r0 & 1) * 32;
+    float4 next[8];
     int unit = blockIdx.x, c = 0, c_end = 0, kb = 0;  // the step: unit, its tile's first column, 64 of dim
-    const float *pa = nullptr, *pb = nullptr;  // this thread's first element of the tile's operands
-    uint32_t there = 0;                        // bit i: its i-th row exists (four of hidden, four of head)
+    const float* head = nullptr;                      // this thread's first element of the tile
+    uint32_t there = 0;                               // bit i: its i-th row exists
     auto tile = [&] {
-      const int m = unit % args.num_m * BM + r0;
-      pa = static_cast<const float*>(args.hidden) + m * args.ldh + 4 * j;
-      pb = static_cast<const float*>(args.head) + (c + r0) * args.ldw + 4 * j;
+      head = static_cast<const float*>(args.head) + (c + r0) * args.ldw + 4 * j;
       there = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        there |= (m + 32 * i < args.rows ? 1u : 0u) << i;
-        there |= (r0 + 32 * i < args.tile && c + r0 + 32 * i < args.vocab ? 16u : 0u) << i;
-      }
+      for (int i = 0; i < 4; ++i) there |= (r0 + 32 * i < args.tile && c + r0 + 32 * i < args.vocab ? 1u : 0u) << i;
     };
     auto begin = [&] {
       if (unit < units) {
@@ -420,17 +438,16 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
         begin();
       }
     };
-    const long long step_a = 32 * args.ldh, step_b = 32 * args.ldw;
+    const long long step = 32 * args.ldw;
     auto load = [&] {
       if (unit >= units) return;
       const int k = kb * BK + 4 * j;
-      const uint32_t low = k < args.dim ? there : 0u, high = k + 32 < args.dim ? there : 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float* p = (i < 4 ? pa + i * step_a : pb + (i - 4) * step_b) + kb * BK;
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        next[2 * i] = (low >> i) & 1u ? *reinterpret_cast<const float4*>(p) : zero;
-        next[2 * i + 1] = (high >> i) & 1u ? *reinterpret_cast<const float4*>(p + 32) : zero;
+        const int half = (i & 1) ? 32 - half0 : half0;
+        next[i] = (there >> (i / 2) & 1u) && k + half < args.dim
+                      ? *reinterpret_cast<const float4*>(head + (i / 2) * step + kb * BK + half)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     };
     begin();
@@ -443,12 +460,12 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
       if (!ok) break;
       uint8_t* dst = smem + stage * 6 * S::TILE;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = r0 + 32 * (i / 2 & 3), chunk = (i & 1) * 4 + j / 2;
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 32 * (i / 2), chunk = ((i & 1) ? 32 - half0 : half0) / 8 + j / 2;
         uint2 h, m, l;
         split3(next[i].x, next[i].y, h.x, m.x, l.x);
         split3(next[i].z, next[i].w, h.y, m.y, l.y);
-        uint8_t* p = dst + (i < 8 ? 0 : 3 * S::TILE) + r * 128 + ((chunk ^ (r & 7)) << 4) + (j & 1) * 8;
+        uint8_t* p = dst + 3 * S::TILE + r * 128 + ((chunk ^ (r & 7)) << 4) + (j & 1) * 8;
         *reinterpret_cast<uint2*>(p) = h;
         *reinterpret_cast<uint2*>(p + S::TILE) = m;
         *reinterpret_cast<uint2*>(p + 2 * S::TILE) = l;
@@ -506,6 +523,27 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
       mbar_wait(drain, 0, args.status, kTimeoutDrain);
     }
     __syncwarp();
+  } else if (warp == 21) {
+    const int a_box = hidden_box(args.rows);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+      const int m = unit % args.num_m, split = unit / args.num_m;
+      const int c_end = run_begin(args, split + 1);
+      for (int c = run_begin(args, split); ok && c < c_end; c += args.tile)
+        for (int kb = 0; ok && kb < num_kb; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, args.status, kTimeoutProducer));
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&full[stage], 3 * a_box * BK * 2);
+            for (int p = 0; p < 3; ++p)  // rows behind the last hold the next part's: their scores are not read
+              tma_load_2d(smem + (stage * 6 + p) * S::TILE, &tma_a, &full[stage], kb * BK, p * args.rows + m * BM);
+          }
+          __syncwarp();
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+    }
+    if (!ok) *abort_flag = 1;
   } else {
     const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter; row of the tile
     int local = 0;
