@@ -128,19 +128,52 @@ __device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h,
 template <int DP>
 struct AttnPackedSimtShape {
   static constexpr int BQ = 64, BK = 64, LD = DP + 4, LDP = BK + 4;
-  static constexpr size_t SMEM = (2 * 64 * LD + 64 * DP + BQ * LDP) * sizeof(float);
+  static constexpr int CTAS = DP <= 128 ? 2 : 1;  // per SM
+  static constexpr size_t SMEM = (2 * 64 * LD + BQ * LDP) * sizeof(float);
+};
+
+// A 64-row tile in registers on its way to shared memory: float4 i of a thread is
+// float4 tid + 256 i of the tile.  Rows past `end` and elements past d read zero.
+template <typename T, int DP>
+struct TileOnTheWay {
+  float4 v[DP / 16];
+  __device__ __forceinline__ void load(const T* base, long long ld, int row0, int end, int d, bool vec) {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / (DP / 4), c = at % (DP / 4) * 4;
+      const T* p = base + (row0 + r) * ld + c;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row0 + r < end) {
+        if (sizeof(T) == 4 && vec) {
+          if (c < d) v[i] = *reinterpret_cast<const float4*>(p);
+        } else {
+          if (c < d) v[i].x = to_f32(p[0]);
+          if (c + 1 < d) v[i].y = to_f32(p[1]);
+          if (c + 2 < d) v[i].z = to_f32(p[2]);
+          if (c + 3 < d) v[i].w = to_f32(p[3]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* tile, int ld) const {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int at = static_cast<int>(threadIdx.x) + 256 * i;
+      *reinterpret_cast<float4*>(tile + at / (DP / 4) * ld + at % (DP / 4) * 4) = v[i];
+    }
+  }
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel(const __grid_constant__ AttnPackedArgs<T> a) {
+__global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
+    attn_packed_simt_kernel(const __grid_constant__ AttnPackedArgs<T> a, bool vec) {
   using Sh = AttnPackedSimtShape<DP>;
   constexpr int BQ = Sh::BQ, BK = Sh::BK, LD = Sh::LD, LDP = Sh::LDP, NC = DP / 64;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(16) float simt_smem[];
   float* sQ = simt_smem;
-  float* sK = sQ + BQ * LD;
-  float* sV = sK + BK * LD;
-  float* sP = sV + BK * DP;
+  float* sKV = sQ + BQ * LD;  // the key tile, then the value tile
+  float* sP = sKV + BK * LD;
   __shared__ int s_lo[BQ];
   __shared__ unsigned long long s_nan;
 
@@ -156,10 +189,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
     s_lo[tid] = row >= q_first && row < q_end ? packed_first_key(a, row, 0, a.n_seqs - 1) : row + 1;
   }
   if (tid == 0) s_nan = 0;
-  for (int i = tid; i < BQ * DP; i += 256) {
-    const int r = i / DP, c = i % DP;
-    sQ[r * LD + c] = q0 + r < q_end && c < a.d ? to_f32(a.q[(q0 + r) * a.ldq + h * a.hsq + c]) : 0.f;
-  }
+  TileOnTheWay<T, DP> way;
+  way.load(a.q + h * a.hsq, a.ldq, q0, q_end, a.d, vec);
+  way.store(sQ, LD);
   __syncthreads();
   int lo[4];
 #pragma unroll
@@ -174,15 +206,16 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
 #pragma unroll
     for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
   }
+  // rows of this warp: tiles above the last or below the first one's keys cost it nothing
+  const int w_last = q0 + (tid / 32) * 8 + 7, w_lo = s_lo[(tid / 32) * 8];
+  way.load(a.k + hk * a.hsk, a.ldk, k_begin, q_end, a.d, vec);
   for (int k0 = k_begin; k0 < q_end; k0 += BK) {
-    __syncthreads();  // the last tile has been read
-    for (int i = tid; i < BK * DP; i += 256) {
-      const int r = i / DP, c = i % DP;
-      const bool in = k0 + r < q_end && c < a.d;
-      sK[r * LD + c] = in ? to_f32(a.k[(k0 + r) * a.ldk + hk * a.hsk + c]) : 0.f;
-      sV[r * DP + c] = in ? to_f32(a.v[(k0 + r) * a.ldv + hk * a.hsv + c]) : 0.f;
-    }
+    const bool any = k0 <= w_last && k0 + BK > w_lo;
+    __syncthreads();  // the last value tile has been read
+    way.store(sKV, LD);
     __syncthreads();
+    way.load(a.v + hk * a.hsv, a.ldv, k0, q_end, a.d, vec);
+    if (any) {
     float s[4][4] = {};
 #pragma unroll 4
     for (int c = 0; c < DP; c += 4) {
@@ -190,7 +223,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
 #pragma unroll
       for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * LD + c]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sK[(tx + 16 * j) * LD + c]);
+      for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sKV[(tx + 16 * j) * LD + c]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -230,7 +263,12 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
 #pragma unroll
       for (int c = 0; c < 4 * NC; ++c) o[i][c] = corr == 0.f ? 0.f : o[i][c] * corr;
     }
-    __syncwarp();  // a row's P is written and read by one half-warp
+    }
+    __syncthreads();  // the key tile has been read
+    way.store(sKV, LD);
+    __syncthreads();
+    if (k0 + BK < q_end) way.load(a.k + hk * a.hsk, a.ldk, k0 + BK, q_end, a.d, vec);
+    if (any) {
 #pragma unroll 2
     for (int j = 0; j < BK; j += 4) {
       float4 pf[4];
@@ -240,7 +278,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
       for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const float4 vf = *reinterpret_cast<const float4*>(&sV[(j + jj) * DP + 64 * c + tx * 4]);
+          const float4 vf = *reinterpret_cast<const float4*>(&sKV[(j + jj) * LD + 64 * c + tx * 4]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
@@ -251,7 +289,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attn_packed_simt_kernel
           }
         }
     }
-    __syncwarp();
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -147,8 +147,12 @@ static CUtensorMap tmap_bf16_heads(const void* ptr, int tokens, int heads, int d
 template <typename T, int DP>
 static void launch_packed_simt(const AttnPackedArgs<T>& a, cudaStream_t st) {
   constexpr size_t smem = AttnPackedSimtShape<DP>::SMEM;
+  const auto rows = [](const void* p, long long ld, long long hs, int heads) {
+    return aligned16(p) && ld % 4 == 0 && (heads == 1 || hs % 4 == 0);
+  };
+  const bool vec = a.d % 4 == 0 && rows(a.q, a.ldq, a.hsq, a.H) && rows(a.k, a.ldk, a.hsk, a.Hk) && rows(a.v, a.ldv, a.hsv, a.Hk);
   allow_smem(attn_packed_simt_kernel<T, DP>, smem);
-  attn_packed_simt_kernel<T, DP><<<dim3((a.tokens + 63) / 64, a.H), 256, smem, st>>>(a);
+  attn_packed_simt_kernel<T, DP><<<dim3((a.tokens + 63) / 64, a.H), 256, smem, st>>>(a, vec);
   CUDA_CHECK(cudaGetLastError());
 }
 
