@@ -246,7 +246,7 @@ struct OpScratch {
 };
 
 // Clusters of two CTAs of the pair kernel that fit the device at once.
-template <bool CAP>
+template <bool CAP, int K>
 static int logprob_pairs(int dev, cudaLaunchConfig_t cfg) {
   static std::mutex mu;
   static std::map<int, int> fits;
@@ -256,13 +256,13 @@ static int logprob_pairs(int dev, cudaLaunchConfig_t cfg) {
   cfg.gridDim = dim3(sm_count(dev) / 2 * 2);
   cfg.dynamicSmemBytes = LogprobShape<true>::smem(kTopMax);
   int n = 0;
-  CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, token_logprobs_tc_kernel<true, CAP>, &cfg));
+  CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, token_logprobs_tc_kernel<true, CAP, K>, &cfg));
   REQUIRE(n > 0, "no CTA-pair cluster fits on this device");
   fits[dev] = n;
   return n;
 }
 
-template <typename T, bool CAP>
+template <typename T, bool CAP, int K>
 static void token_logprobs(FinishArgs f, cudaStream_t st) {
   LogprobArgs& a = f.l;
   const int dev = current_device();
@@ -274,7 +274,7 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   int workers = sm_count(dev);
   if (pair) {
-    allow_smem(token_logprobs_tc_kernel<true, CAP>, LogprobShape<true>::smem(kTopMax));
+    allow_smem(token_logprobs_tc_kernel<true, CAP, K>, LogprobShape<true>::smem(kTopMax));
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
@@ -283,7 +283,7 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    workers = logprob_pairs<CAP>(dev, cfg);
+    workers = logprob_pairs<CAP, K>(dev, cfg);
   }
   const int bm = pair ? 256 : 128;
   a.num_m = (a.rows + bm - 1) / bm;
@@ -312,30 +312,30 @@ static void token_logprobs(FinishArgs f, cudaStream_t st) {
       if (pair) {
         cfg.gridDim = dim3(2 * grid);
         cfg.dynamicSmemBytes = LogprobShape<true>::smem(a.top);
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprobs_tc_kernel<true, CAP>, ta, tb, tb16, a));
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprobs_tc_kernel<true, CAP, K>, ta, tb, tb16, a));
       } else {
-        allow_smem(token_logprobs_tc_kernel<false, CAP>, LogprobShape<false>::smem(kTopMax));
-        token_logprobs_tc_kernel<false, CAP><<<grid, 192, LogprobShape<false>::smem(a.top), st>>>(ta, tb, tb16, a);
+        allow_smem(token_logprobs_tc_kernel<false, CAP, K>, LogprobShape<false>::smem(kTopMax));
+        token_logprobs_tc_kernel<false, CAP, K><<<grid, 192, LogprobShape<false>::smem(a.top), st>>>(ta, tb, tb16, a);
         CUDA_CHECK(cudaGetLastError());
       }
     }
   }
   if constexpr (sizeof(T) == 4) {
     if (tc) {
-      allow_smem(token_logprobs_f32_tc_kernel<CAP>, LogprobF32Shape::smem(kTopMax));
+      allow_smem(token_logprobs_f32_tc_kernel<CAP, K>, LogprobF32Shape::smem(kTopMax));
       bf16* parts = reinterpret_cast<bf16*>(static_cast<uint8_t*>(scratch.p) + state_bytes);
       const long long runs8 = static_cast<long long>(a.rows) * (dim_split / 8);
       split_rows_kernel<<<static_cast<int>((runs8 + 255) / 256), 256, 0, st>>>(static_cast<const float*>(a.hidden), a.ldh,
                                                                                a.rows, a.dim, dim_split, parts);
       CUDA_CHECK(cudaGetLastError());
       const CUtensorMap ta = tmap_bf16(parts, 3ULL * a.rows, dim_split, dim_split, hidden_box(a.rows));
-      token_logprobs_f32_tc_kernel<CAP><<<grid, LogprobF32Shape::THREADS, LogprobF32Shape::smem(a.top), st>>>(ta, a);
+      token_logprobs_f32_tc_kernel<CAP, K><<<grid, LogprobF32Shape::THREADS, LogprobF32Shape::smem(a.top), st>>>(ta, a);
       CUDA_CHECK(cudaGetLastError());
     }
   }
   if (!tc) {
-    allow_smem(token_logprobs_simt_kernel<T, CAP>, logprob_simt_smem(kTopMax));
-    token_logprobs_simt_kernel<T, CAP><<<grid, 256, logprob_simt_smem(a.top), st>>>(a);
+    allow_smem(token_logprobs_simt_kernel<T, CAP, K>, logprob_simt_smem(kTopMax));
+    token_logprobs_simt_kernel<T, CAP, K><<<grid, 256, logprob_simt_smem(a.top), st>>>(a);
     CUDA_CHECK(cudaGetLastError());
   }
   auto finish = [&](auto kern) {
@@ -399,10 +399,17 @@ int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const voi
     f.top_ids = top_ids;
     f.top_logprobs = top_logprobs;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto run = [&](auto* type, auto cap) {
+      using T = std::remove_pointer_t<decltype(type)>;
+      if (top <= 8)
+        token_logprobs<T, decltype(cap)::value, 8>(f, st);
+      else
+        token_logprobs<T, decltype(cap)::value, kTopMax>(f, st);
+    };
     if (dtype == CLEF_DTYPE_BF16)
-      softcap > 0.f ? token_logprobs<bf16, true>(f, st) : token_logprobs<bf16, false>(f, st);
+      softcap > 0.f ? run(static_cast<bf16*>(nullptr), std::true_type{}) : run(static_cast<bf16*>(nullptr), std::false_type{});
     else
-      softcap > 0.f ? token_logprobs<float, true>(f, st) : token_logprobs<float, false>(f, st);
+      softcap > 0.f ? run(static_cast<float*>(nullptr), std::true_type{}) : run(static_cast<float*>(nullptr), std::false_type{});
   });
 }
 

@@ -53,37 +53,91 @@ __device__ __forceinline__ float capped(float x, float softcap) {
   return CAP ? softcap * tanhf(x / softcap) : x;
 }
 
-// A row's running state.  m, s, t are in log2 units of z.  The list of the
-// largest x lies in shared memory, entry j of row r at [j * 128 + r], in no
-// order; its smallest entry (the highest id among equals) is x = thr at `worst`.
+// A row's running sums, in log2 units of z.
 struct RowState {
-  float m = -INFINITY, s = 0.f, t = 0.f, thr = -INFINITY;
-  int worst = 0;
+  float m = -INFINITY, s = 0.f, t = 0.f;
 };
 
-__device__ __forceinline__ void list_clear(float* lx, int32_t* lid, int top, int r) {
-  for (int j = 0; j < top; ++j) {
-    lx[j * 128 + r] = -INFINITY;
-    lid[j * 128 + r] = -1;
-  }
-}
+// The `top` largest scores of a row, entered by a chunk of 32 columns at a time.
+// Ids rise from chunk to chunk, so a score that equals the smallest entry stays
+// out.  Both forms use `area` (shared memory, list_bytes(top) a CTA); r is the
+// thread's place in it (0..127).
+//
+// Up to 8: in registers, largest first.  An insertion is 8 independent
+// comparisons and the moves they choose; a chunk with a candidate is laid down in
+// `area` so that a bit mask can walk the candidates.  (Lists in shared memory, and
+// the chunk's maximum searched for again for every insertion, took 1100 cycles an
+// insertion of a warp: 227 us instead of 104 without a list at 2000 rows x 32000 x 1024.)
+template <int K>
+struct TopList {
+  static_assert(K == 8);
+  float v[K];
+  int32_t id[K];
+  float thr;
 
-// x > thr takes the place of the smallest entry.  One pass finds the next one:
-// its loads do not depend on each other, unlike the shifts of a sorted list.
-__device__ __forceinline__ void list_replace(RowState& st, float x, int id, float* lx, int32_t* lid, int top, int r) {
-  lx[st.worst * 128 + r] = x;
-  lid[st.worst * 128 + r] = id;
-  float low = x;
-  int low_id = id, at = st.worst;
-#pragma unroll 4
-  for (int j = 0; j < top; ++j) {
-    const float v = lx[j * 128 + r];
-    const int i = lid[j * 128 + r];
-    if (v < low || (v == low && i > low_id)) low = v, low_id = i, at = j;
+  __device__ __forceinline__ void clear(int top, float*, int) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      v[j] = -INFINITY;
+      id[j] = -1;
+    }
+    thr = top > 0 ? -INFINITY : INFINITY;
   }
-  st.thr = low;
-  st.worst = at;
-}
+  template <bool ANY_ORDER = false>
+  __device__ __forceinline__ void insert(float x, int32_t i, int top) {
+    bool before[K];  // x goes before entry j
+#pragma unroll
+    for (int j = 0; j < K; ++j) before[j] = x > v[j] || (ANY_ORDER && x == v[j] && i < id[j]);
+#pragma unroll
+    for (int j = K - 1; j > 0; --j) {
+      v[j] = before[j - 1] ? v[j - 1] : before[j] ? x : v[j];
+      id[j] = before[j - 1] ? id[j - 1] : before[j] ? i : id[j];
+    }
+    v[0] = before[0] ? x : v[0];
+    id[0] = before[0] ? i : id[0];
+    thr = v[0];
+#pragma unroll
+    for (int j = 1; j < K; ++j) thr = j < top ? fminf(thr, v[j]) : thr;  // entry top - 1
+  }
+  // best = the largest of x; entries that do not count are -inf
+  __device__ __forceinline__ void take(float (&x)[32], float best, int col, int top, float* area, int r) {
+    if (!(best > thr)) return;
+    uint32_t mask[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      if (x[c] > thr) mask[c & 3] |= 1u << c;
+      area[c * 128 + r] = x[c];
+    }
+    for (uint32_t left = (mask[0] | mask[1]) | (mask[2] | mask[3]); left; left &= left - 1) {
+      const int c = __ffs(static_cast<int>(left)) - 1;
+      const float y = area[c * 128 + r];
+      if (y > thr) insert(y, col + c, top);
+    }
+  }
+  __device__ __forceinline__ void publish(int, float* area, int r) const {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      area[j * 128 + r] = v[j];
+      reinterpret_cast<int32_t*>(area)[(K + j) * 128 + r] = id[j];
+    }
+  }
+  __device__ __forceinline__ void join(int top, float* area, int r, int r2) {
+    for (int j = 0; j < top; ++j) {
+      const float x = area[j * 128 + r2];
+      const int32_t i = reinterpret_cast<const int32_t*>(area)[(K + j) * 128 + r2];
+      if (i < 0 || x < thr) break;  // it is sorted
+      insert<true>(x, i, top);
+    }
+  }
+  __device__ __forceinline__ void store(int top, float*, int, float* lx, int32_t* lid) const {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j < top) {
+        lx[j] = v[j];
+        lid[j] = id[j];
+      }
+  }
+};
 
 __device__ __forceinline__ float max32(const float (&x)[32]) {
   float p[4] = {x[0], x[1], x[2], x[3]};
@@ -92,21 +146,95 @@ __device__ __forceinline__ float max32(const float (&x)[32]) {
   return fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
 }
 
+// Up to kTopMax: in shared memory, entry j of row r at [j * 128 + r], in no
+// order; the smallest entry (the highest id among equals) is thr, at `worst`.
+// Candidates of a chunk are taken largest first, at most `top` rounds of a warp.
+template <>
+struct TopList<kTopMax> {
+  float thr;
+  int worst;
+
+  static __device__ __forceinline__ int32_t* ids(float* area, int top) { return reinterpret_cast<int32_t*>(area) + 128 * top; }
+  __device__ __forceinline__ void clear(int top, float* area, int r) {
+    thr = top > 0 ? -INFINITY : INFINITY;
+    worst = 0;
+    for (int j = 0; j < top; ++j) {
+      area[j * 128 + r] = -INFINITY;
+      ids(area, top)[j * 128 + r] = -1;
+    }
+  }
+  // One pass finds the next smallest entry: its loads do not depend on each other.
+  __device__ __forceinline__ void replace(float x, int32_t i, int top, float* area, int r) {
+    int32_t* lid = ids(area, top);
+    area[worst * 128 + r] = x;
+    lid[worst * 128 + r] = i;
+    float low = x;
+    int low_id = i, at = worst;
+#pragma unroll 4
+    for (int j = 0; j < top; ++j) {
+      const float y = area[j * 128 + r];
+      const int k = lid[j * 128 + r];
+      if (y < low || (y == low && k > low_id)) low = y, low_id = k, at = j;
+    }
+    thr = low;
+    worst = at;
+  }
+  __device__ __forceinline__ void take(float (&x)[32], float best, int col, int top, float* area, int r) {
+    while (best > thr) {
+      int at = 0;
+#pragma unroll
+      for (int c = 31; c >= 0; --c)
+        if (x[c] == best) at = c;
+      replace(best, col + at, top, area, r);
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c == at) x[c] = -INFINITY;
+      best = max32(x);
+    }
+  }
+  __device__ __forceinline__ void publish(int, float*, int) const {}
+  __device__ __forceinline__ void join(int top, float* area, int r, int r2) {
+    const int32_t* lid = ids(area, top);
+    for (int j = 0; j < top; ++j) {
+      const float x = area[j * 128 + r2];
+      const int32_t i = lid[j * 128 + r2];
+      if (i >= 0 && (x > thr || (x == thr && i < lid[worst * 128 + r]))) replace(x, i, top, area, r);
+    }
+  }
+  __device__ __forceinline__ void store(int top, float* area, int r, float* lx, int32_t* lid) const {
+    unsigned taken = 0u;
+    for (int j = 0; j < top; ++j) {
+      float x = -INFINITY;
+      int id = INT32_MAX, from = -1;
+#pragma unroll 4
+      for (int i = 0; i < top; ++i) {
+        const float v = area[i * 128 + r];
+        const int vi = ids(area, top)[i * 128 + r];
+        if (!((taken >> i) & 1u) && vi >= 0 && (v > x || (v == x && vi < id))) x = v, id = vi, from = i;
+      }
+      if (from >= 0) taken |= 1u << from;
+      lx[j] = x;
+      lid[j] = from >= 0 ? id : -1;
+    }
+  }
+};
+
+// Shared memory of a CTA's 128 lists.
+__host__ __device__ constexpr size_t list_bytes(int top) {
+  return top == 0 ? 0 : top <= 8 ? 128 * 32 * sizeof(float) : 128 * 8 * static_cast<size_t>(top);
+}
+
 // Scores x of columns col .. col + 31, the first `valid` of which exist.
-// Candidates for the list are taken largest first, so that a chunk costs a
-// warp at most `top` rounds (and about one when the list has settled), not one
-// for every lane's every candidate.  Ids rise from chunk to chunk and equal
-// scores of a chunk go by the lowest column: an equal score never displaces.
-template <bool CAP>
-__device__ __forceinline__ void scan32(RowState& st, float (&x)[32], int col, int valid, float softcap, float* lx,
-                                       int32_t* lid, int top, int r) {
+template <bool CAP, int K>
+__device__ __forceinline__ void scan32(RowState& st, TopList<K>& list, float (&x)[32], int col, int valid, float softcap,
+                                       int top, float* area, int r) {
   constexpr float LOG2E = 1.4426950408889634f;
   if (valid < 32) {
 #pragma unroll
     for (int c = 0; c < 32; ++c)
       if (c >= valid) x[c] = -INFINITY;
   }
-  float best = max32(x);
+  const float best = max32(x);
   const float zmax = capped<CAP>(best, softcap) * LOG2E;
   if (zmax > st.m) {  // the sums move to the new maximum
     const float step = st.m - zmax, f = exp2f(step);
@@ -136,56 +264,25 @@ __device__ __forceinline__ void scan32(RowState& st, float (&x)[32], int col, in
   }
   st.s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   st.t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
-  if (top > 0) {
-    while (best > st.thr) {
-      int at = 0;
-#pragma unroll
-      for (int c = 31; c >= 0; --c)
-        if (x[c] == best) at = c;
-      list_replace(st, best, col + at, lx, lid, top, r);
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (c == at) x[c] = -INFINITY;
-      best = max32(x);
-    }
-  }
+  list.take(x, best, col, top, area, r);
 }
 
-// Joins thread r2's state and list (in shared memory) into thread r's.
-__device__ __forceinline__ void join_state(RowState& st, float m, float s, float t, int r2, float* lx, int32_t* lid,
-                                           int top, int r) {
+// Joins another state into this one.  A side without columns has m = -inf, s = t = 0: it weighs nothing.
+__device__ __forceinline__ void join_state(RowState& st, float m, float s, float t) {
   const float mx = fmaxf(st.m, m);
   const float d0 = st.m - mx, d1 = m - mx, w0 = exp2f(d0), w1 = exp2f(d1);
-  // a side without columns has m = -inf, s = t = 0: it weighs nothing
   st.t = (w0 == 0.f ? 0.f : w0 * fmaf(d0, st.s, st.t)) + (w1 == 0.f ? 0.f : w1 * fmaf(d1, s, t));
   st.s = w0 * st.s + w1 * s;
   st.m = mx;
-  for (int j = 0; j < top; ++j) {
-    const float x = lx[j * 128 + r2];
-    const int id = lid[j * 128 + r2];
-    if (id >= 0 && (x > st.thr || (x == st.thr && id < lid[st.worst * 128 + r]))) list_replace(st, x, id, lx, lid, top, r);
-  }
 }
 
-// Leaves the state in scratch, and the list in order.
-__device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, int split, int row, float* lx,
-                                            const int32_t* lid, int r) {
+// Leaves the state, and the list in order, in scratch.
+template <int K>
+__device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, const TopList<K>& list, int split,
+                                            int row, float* area, int r) {
   const size_t at = static_cast<size_t>(row) * a.splits + split;
   a.part[at] = make_float4(st.m, st.s, st.t, 0.f);
-  unsigned taken = 0u;  // top <= 32
-  for (int j = 0; j < a.top; ++j) {
-    float x = -INFINITY;
-    int id = INT32_MAX, from = -1;
-#pragma unroll 4
-    for (int i = 0; i < a.top; ++i) {
-      const float v = lx[i * 128 + r];
-      const int vi = lid[i * 128 + r];
-      if (!((taken >> i) & 1u) && vi >= 0 && (v > x || (v == x && vi < id))) x = v, id = vi, from = i;
-    }
-    if (from >= 0) taken |= 1u << from;
-    a.list_x[at * a.top + j] = x;
-    a.list_id[at * a.top + j] = from >= 0 ? id : -1;
-  }
+  list.store(a.top, area, r, a.list_x + at * a.top, a.list_id + at * a.top);
 }
 
 // ---------------------------------------------------------------------------
@@ -197,7 +294,7 @@ __device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState
 
 constexpr int kLogprobSimtLdc = 132;
 constexpr size_t logprob_simt_smem(int top) {
-  return (2 * 16 * 132 + 128 * kLogprobSimtLdc + 2 * 128 * top) * sizeof(float);
+  return (2 * 16 * 132 + 128 * kLogprobSimtLdc) * sizeof(float) + list_bytes(top);
 }
 
 // Elements k .. k + 7 of a row (zeros past its end); VEC: by 16-byte loads.
@@ -222,21 +319,21 @@ __device__ __forceinline__ void load8(const T* p, int k, int dim, bool live, flo
   }
 }
 
-template <typename T, bool CAP>
+template <typename T, bool CAP, int K>
 __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_constant__ LogprobArgs a) {
   extern __shared__ __align__(16) float lp_smem[];
   float(*sA)[132] = reinterpret_cast<float(*)[132]>(lp_smem);
   float(*sB)[132] = reinterpret_cast<float(*)[132]>(lp_smem + 16 * 132);
   float* sC = lp_smem + 2 * 16 * 132;
-  float* lx = sC + 128 * kLogprobSimtLdc;
-  int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * a.top);
+  float* area = sC + 128 * kLogprobSimtLdc;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int lr = tid >> 1, lk = (tid & 1) * 8;  // row and first k this thread loads
   for (int unit = blockIdx.x; unit < a.num_m * a.splits; unit += gridDim.x) {
     const int m0 = unit % a.num_m * 128, split = unit / a.num_m;
     const int n_end = run_begin(a, split + 1);
     RowState st;
-    if (tid < 128) list_clear(lx, lid, a.top, tid);
+    TopList<K> list;
+    if (tid < 128) list.clear(a.top, area, tid);
     const T* pa = static_cast<const T*>(a.hidden) + (m0 + lr) * a.ldh;
     const bool la = m0 + lr < a.rows;
     for (int n0 = run_begin(a, split); n0 < n_end; n0 += 128) {
@@ -284,12 +381,12 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             *reinterpret_cast<float4*>(x + 4 * j) = *reinterpret_cast<const float4*>(sC + tid * kLogprobSimtLdc + c + 4 * j);
-          scan32<CAP>(st, x, n0 + c, a.vocab - n0 - c, a.softcap, lx, lid, a.top, tid);
+          scan32<CAP>(st, list, x, n0 + c, a.vocab - n0 - c, a.softcap, a.top, area, tid);
         }
       }
       // the next tile writes sC only after its own barriers
     }
-    if (tid < 128 && m0 + tid < a.rows) store_state(a, st, split, m0 + tid, lx, lid, tid);
+    if (tid < 128 && m0 + tid < a.rows) store_state(a, st, list, split, m0 + tid, area, tid);
   }
 }
 

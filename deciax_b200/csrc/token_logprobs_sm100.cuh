@@ -32,7 +32,7 @@ struct LogprobShape {
   static constexpr uint32_t A_BYTES = 128 * BK * 2;                 // rows a CTA holds
   static constexpr uint32_t B_BYTES = (PAIR ? 128 : 256) * BK * 2;  // head rows a CTA holds
   static constexpr uint32_t TMEM_COLS = 512;
-  static constexpr size_t smem(int top) { return 1024 + STAGES * (A_BYTES + B_BYTES) + 256 + 128 * 8 * static_cast<size_t>(top); }
+  static constexpr size_t smem(int top) { return 1024 + STAGES * (A_BYTES + B_BYTES) + 256 + list_bytes(top); }
 };
 
 // Columns the MMA of the tile at c computes, in the instruction's steps of 32
@@ -48,7 +48,7 @@ __device__ __forceinline__ int tile_width(const LogprobArgs& a, int c, int c_end
 // whatever shared memory held; their scores are never read.
 __host__ __device__ inline int hidden_box(int rows) { return rows > 64 ? 128 : rows > 32 ? 64 : rows > 8 ? 32 : 8; }
 
-template <bool PAIR, bool CAP>
+template <bool PAIR, bool CAP, int K>
 __global__ void __launch_bounds__(192, 1)
     token_logprobs_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                              const __grid_constant__ CUtensorMap tma_b16, const __grid_constant__ LogprobArgs args) {
@@ -66,8 +66,7 @@ __global__ void __launch_bounds__(192, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* lx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);
-  int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * args.top);
+  float* area = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // of the lists
   __shared__ float3 state[PAIR ? 1 : 128];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -234,7 +233,8 @@ __global__ void __launch_bounds__(192, 1)
       const int row = m * BM + static_cast<int>(rank) * 128 + r - share * rows_seen;
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
-      list_clear(lx, lid, args.top, r);
+      TopList<K> list;
+      list.clear(args.top, area, r);
       for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
         const int acc = local & 1;
         ok = mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue);
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(192, 1)
             float x[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
-            if (row < args.rows) scan32<CAP>(st, x, c0 + c, cols - c, args.softcap, lx, lid, args.top, r);
+            if (row < args.rows) scan32<CAP>(st, list, x, c0 + c, cols - c, args.softcap, args.top, area, r);
             __syncwarp();
           }
         }
@@ -273,16 +273,18 @@ __global__ void __launch_bounds__(192, 1)
         if (copies > 1) {
           // the shares of a row meet in the first one's thread
           state[r] = make_float3(st.m, st.s, st.t);
+          if (args.top > 0) list.publish(args.top, area, r);
           ok = !bar_red_or(1, 128, !ok);  // a failed wait ends every warp's loop together
           if (ok && share == 0 && row < args.rows)
             for (int i = 1; i < copies; ++i) {
               const int r2 = r + i * rows_seen;
               const float3 o = state[r2];
-              join_state(st, o.x, o.y, o.z, r2, lx, lid, args.top, r);
+              join_state(st, o.x, o.y, o.z);
+              list.join(args.top, area, r, r2);
             }
         }
       }
-      if (ok && share == 0 && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+      if (ok && share == 0 && row < args.rows) store_state(args, st, list, split, row, area, r);
       if (!PAIR && copies > 1) asm volatile("bar.sync 1, 128;" ::: "memory");  // the lists may be cleared
     }
   }
@@ -324,7 +326,7 @@ struct LogprobF32Shape {
   static constexpr int BM = 128, BN = 128, BK = 64, STAGES = 2, THREADS = 22 * 32;
   static constexpr uint32_t TILE = 128 * BK * 2;  // one bf16 tile of 128 rows
   static constexpr uint32_t TMEM_COLS = 512;  // two tiles of 128 columns: h h', and the small products
-  static constexpr size_t smem(int top) { return 1024 + STAGES * 6 * TILE + 256 + 128 * 8 * static_cast<size_t>(top); }
+  static constexpr size_t smem(int top) { return 1024 + STAGES * 6 * TILE + 256 + list_bytes(top); }
 };
 
 // A pair's three bf16 parts, packed (of an infinity: one infinity and two NaN).
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(256)
   *reinterpret_cast<uint4*>(out + 2 * plane + at) = l;
 }
 
-template <bool CAP>
+template <bool CAP, int K>
 __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
     token_logprobs_f32_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ LogprobArgs args) {
   using S = LogprobF32Shape;
@@ -376,8 +378,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* lx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);
-  int32_t* lid = reinterpret_cast<int32_t*>(lx + 128 * args.top);
+  float* area = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // of the lists
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int units = args.num_m * args.splits;
@@ -553,7 +554,8 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
       const int c_end = run_begin(args, split + 1);
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
-      list_clear(lx, lid, args.top, r);
+      TopList<K> list;
+      list.clear(args.top, area, r);
       for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
         const int acc = local & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue));
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 16; ++e) x[half + e] = __uint_as_float(v[e]) + __uint_as_float(w[e]);
             }
-            if (row < args.rows) scan32<CAP>(st, x, c0 + c, cols - c, args.softcap, lx, lid, args.top, r);
+            if (row < args.rows) scan32<CAP>(st, list, x, c0 + c, cols - c, args.softcap, args.top, area, r);
             __syncwarp();
           }
         }
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&tempty[acc]);
       }
-      if (ok && row < args.rows) store_state(args, st, split, row, lx, lid, r);
+      if (ok && row < args.rows) store_state(args, st, list, split, row, area, r);
     }
   }
 
