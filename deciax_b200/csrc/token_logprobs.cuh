@@ -63,19 +63,18 @@ struct RowState {
 // out.  Both forms use `area` (shared memory, list_bytes(top) a CTA); r is the
 // thread's place in it (0..127).
 //
-// Up to 8: in registers, largest first.  An insertion is 8 independent
-// comparisons and the moves they choose; a chunk with a candidate is laid down in
-// `area` so that a bit mask can walk the candidates.  (Lists in shared memory, and
+// The list lies in registers, largest first, K = 8 or 32 places.  An insertion is
+// K independent comparisons and the moves they choose; a chunk with a candidate is
+// laid down in `area` so that a bit mask can walk the candidates.  (Lists in shared memory, and
 // the chunk's maximum searched for again for every insertion, took 1100 cycles an
 // insertion of a warp: 227 us instead of 104 without a list at 2000 rows x 32000 x 1024.)
 template <int K>
 struct TopList {
-  static_assert(K == 8);
   float v[K];
   int32_t id[K];
   float thr;
 
-  __device__ __forceinline__ void clear(int top, float*, int) {
+  __device__ __forceinline__ void clear(int top) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       v[j] = -INFINITY;
@@ -114,7 +113,7 @@ struct TopList {
       if (y > thr) insert(y, col + c, top);
     }
   }
-  __device__ __forceinline__ void publish(int, float* area, int r) const {
+  __device__ __forceinline__ void publish(float* area, int r) const {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       area[j * 128 + r] = v[j];
@@ -129,7 +128,7 @@ struct TopList {
       insert<true>(x, i, top);
     }
   }
-  __device__ __forceinline__ void store(int top, float*, int, float* lx, int32_t* lid) const {
+  __device__ __forceinline__ void store(int top, float* lx, int32_t* lid) const {
 #pragma unroll
     for (int j = 0; j < K; ++j)
       if (j < top) {
@@ -146,82 +145,9 @@ __device__ __forceinline__ float max32(const float (&x)[32]) {
   return fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
 }
 
-// Up to kTopMax: in shared memory, entry j of row r at [j * 128 + r], in no
-// order; the smallest entry (the highest id among equals) is thr, at `worst`.
-// Candidates of a chunk are taken largest first, at most `top` rounds of a warp.
-template <>
-struct TopList<kTopMax> {
-  float thr;
-  int worst;
-
-  static __device__ __forceinline__ int32_t* ids(float* area, int top) { return reinterpret_cast<int32_t*>(area) + 128 * top; }
-  __device__ __forceinline__ void clear(int top, float* area, int r) {
-    thr = top > 0 ? -INFINITY : INFINITY;
-    worst = 0;
-    for (int j = 0; j < top; ++j) {
-      area[j * 128 + r] = -INFINITY;
-      ids(area, top)[j * 128 + r] = -1;
-    }
-  }
-  // One pass finds the next smallest entry: its loads do not depend on each other.
-  __device__ __forceinline__ void replace(float x, int32_t i, int top, float* area, int r) {
-    int32_t* lid = ids(area, top);
-    area[worst * 128 + r] = x;
-    lid[worst * 128 + r] = i;
-    float low = x;
-    int low_id = i, at = worst;
-#pragma unroll 4
-    for (int j = 0; j < top; ++j) {
-      const float y = area[j * 128 + r];
-      const int k = lid[j * 128 + r];
-      if (y < low || (y == low && k > low_id)) low = y, low_id = k, at = j;
-    }
-    thr = low;
-    worst = at;
-  }
-  __device__ __forceinline__ void take(float (&x)[32], float best, int col, int top, float* area, int r) {
-    while (best > thr) {
-      int at = 0;
-#pragma unroll
-      for (int c = 31; c >= 0; --c)
-        if (x[c] == best) at = c;
-      replace(best, col + at, top, area, r);
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (c == at) x[c] = -INFINITY;
-      best = max32(x);
-    }
-  }
-  __device__ __forceinline__ void publish(int, float*, int) const {}
-  __device__ __forceinline__ void join(int top, float* area, int r, int r2) {
-    const int32_t* lid = ids(area, top);
-    for (int j = 0; j < top; ++j) {
-      const float x = area[j * 128 + r2];
-      const int32_t i = lid[j * 128 + r2];
-      if (i >= 0 && (x > thr || (x == thr && i < lid[worst * 128 + r]))) replace(x, i, top, area, r);
-    }
-  }
-  __device__ __forceinline__ void store(int top, float* area, int r, float* lx, int32_t* lid) const {
-    unsigned taken = 0u;
-    for (int j = 0; j < top; ++j) {
-      float x = -INFINITY;
-      int id = INT32_MAX, from = -1;
-#pragma unroll 4
-      for (int i = 0; i < top; ++i) {
-        const float v = area[i * 128 + r];
-        const int vi = ids(area, top)[i * 128 + r];
-        if (!((taken >> i) & 1u) && vi >= 0 && (v > x || (v == x && vi < id))) x = v, id = vi, from = i;
-      }
-      if (from >= 0) taken |= 1u << from;
-      lx[j] = x;
-      lid[j] = from >= 0 ? id : -1;
-    }
-  }
-};
-
 // Shared memory of a CTA's 128 lists.
 __host__ __device__ constexpr size_t list_bytes(int top) {
-  return top == 0 ? 0 : top <= 8 ? 128 * 32 * sizeof(float) : 128 * 8 * static_cast<size_t>(top);
+  return top == 0 ? 0 : 128 * (top <= 8 ? 32 : 2 * kTopMax) * sizeof(float);
 }
 
 // Scores x of columns col .. col + 31, the first `valid` of which exist.
@@ -279,10 +205,10 @@ __device__ __forceinline__ void join_state(RowState& st, float m, float s, float
 // Leaves the state, and the list in order, in scratch.
 template <int K>
 __device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState& st, const TopList<K>& list, int split,
-                                            int row, float* area, int r) {
+                                            int row) {
   const size_t at = static_cast<size_t>(row) * a.splits + split;
   a.part[at] = make_float4(st.m, st.s, st.t, 0.f);
-  list.store(a.top, area, r, a.list_x + at * a.top, a.list_id + at * a.top);
+  list.store(a.top, a.list_x + at * a.top, a.list_id + at * a.top);
 }
 
 // ---------------------------------------------------------------------------
@@ -333,7 +259,7 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
     const int n_end = run_begin(a, split + 1);
     RowState st;
     TopList<K> list;
-    if (tid < 128) list.clear(a.top, area, tid);
+    list.clear(a.top);
     const T* pa = static_cast<const T*>(a.hidden) + (m0 + lr) * a.ldh;
     const bool la = m0 + lr < a.rows;
     for (int n0 = run_begin(a, split); n0 < n_end; n0 += 128) {
@@ -386,7 +312,7 @@ __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_c
       }
       // the next tile writes sC only after its own barriers
     }
-    if (tid < 128 && m0 + tid < a.rows) store_state(a, st, list, split, m0 + tid, area, tid);
+    if (tid < 128 && m0 + tid < a.rows) store_state(a, st, list, split, m0 + tid);
   }
 }
 

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(192, 1)
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
       TopList<K> list;
-      list.clear(args.top, area, r);
+      list.clear(args.top);
       for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
         const int acc = local & 1;
         ok = mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue);
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(192, 1)
         if (copies > 1) {
           // the shares of a row meet in the first one's thread
           state[r] = make_float3(st.m, st.s, st.t);
-          if (args.top > 0) list.publish(args.top, area, r);
+          if (args.top > 0) list.publish(area, r);
           ok = !bar_red_or(1, 128, !ok);  // a failed wait ends every warp's loop together
           if (ok && share == 0 && row < args.rows)
             for (int i = 1; i < copies; ++i) {
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(192, 1)
             }
         }
       }
-      if (ok && share == 0 && row < args.rows) store_state(args, st, list, split, row, area, r);
+      if (ok && share == 0 && row < args.rows) store_state(args, st, list, split, row);
       if (!PAIR && copies > 1) asm volatile("bar.sync 1, 128;" ::: "memory");  // the lists may be cleared
     }
   }
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
       const bool any = row - lane < args.rows;  // some row of this warp exists
       RowState st;
       TopList<K> list;
-      list.clear(args.top, area, r);
+      list.clear(args.top);
       for (int c0 = run_begin(args, split); c0 < c_end; c0 += args.tile, ++local) {
         const int acc = local & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, args.status, kTimeoutEpilogue));
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&tempty[acc]);
       }
-      if (ok && row < args.rows) store_state(args, st, list, split, row, area, r);
+      if (ok && row < args.rows) store_state(args, st, list, split, row);
     }
   }
 
