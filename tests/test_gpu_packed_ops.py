@@ -640,3 +640,103 @@ def test_token_logprobs_of_two_streams_at_once():
     torch.cuda.synchronize()
     for x in got:
         assert all(torch.equal(a, b) for a, b in zip(x, want))
+
+
+# --------------------------------------------------------------------------- together, as a prompt runs through them
+
+
+def test_a_packed_prompt_from_projection_to_token_scores():
+    """Three prompts end to end, one with image tokens: rotary positions in place on
+    the packed projection, attention, output projection with the residual, norm and
+    token scores, on one stream.  Each stage is held against 64 bits from what the
+    stage before left; each prompt alone gives the same scores within its roundings,
+    and so do the padded operators for the text prompts."""
+    import torch
+
+    hq, hkv, d, dim, vocab, rot = 4, 2, 128, 512, 3000, 64
+    lens = [150, 0, 37, 200]
+    n, bounds = sum(lens), [0, 150, 150, 187, 387]
+    g = generator(21)
+    width = 2 * hq * d + 2 * hkv * d
+    proj, res = normal(g, n, width), normal(g, n, dim)
+    qw, kw, nw = normal(g, d, std=0.1), normal(g, d, std=0.1), normal(g, dim, std=0.1)
+    w_o, head = normal(g, dim, hq * d, std=0.05), normal(g, vocab, dim, std=0.05)
+    targets = torch.randint(0, vocab, (n, 1), generator=g, device="cuda", dtype=torch.int32)
+    sections = (12, 10, 10)
+    pos = torch.cat([torch.arange(m, device="cuda") for m in lens]).int().repeat(3, 1)
+    patch = torch.arange(64, device="cuda").int()  # rows 200..263 of the last prompt: a frame of 8 x 8 patches
+    pos[0, 200:264], pos[1, 200:264], pos[2, 200:264] = 13, 13 + patch // 8, 13 + patch % 8
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+
+    def views(p):
+        t = p.shape[0]
+        heads = p[:, : 2 * hq * d].unflatten(1, (hq, 2 * d))
+        k0 = 2 * hq * d
+        return heads[..., :d], heads[..., d:], p[:, k0 : k0 + hkv * d].view(t, hkv, d), p[:, k0 + hkv * d :].view(t, hkv, d)
+
+    def through(p, r, positions, lengths, tgt):
+        t = p.shape[0]
+        q, gate, k, v = views(p)
+        run_rope(q, k, q, k, positions, sections, True, rot, 1e4, qw, kw)
+        att = torch.empty(t, hq, d, dtype=torch.bfloat16, device="cuda")
+        run_attention(q, k, v, gate, att, lengths)
+        x, y = torch.empty(t, dim, dtype=torch.bfloat16, device="cuda"), torch.empty(t, dim, dtype=torch.bfloat16, device="cuda")
+        _lib.check(lib().clef_op_gemm(_lib.DTYPE_BF16, 2, t, dim, hq * d, att.data_ptr(), w_o.data_ptr(), x.data_ptr(), dim, None,
+                                      r.data_ptr(), dim, stream()))
+        _lib.check(lib().clef_op_rmsnorm(_lib.DTYPE_BF16, x.data_ptr(), nw.data_ptr(), y.data_ptr(), t, dim, 1e-6, stream()))
+        return att, x, y, run_logprobs(y, head, tgt, 3)
+
+    before = proj.clone()
+    att, x, y, (logp, ent, ids, best) = through(proj, res, pos, cu, targets)
+    for view, old, w in zip(views(proj)[::2], views(before)[::2], (qw, kw)):
+        assert_rope(view, *rope_64(old, w, pos, sections, True, rot, 1e4), "bf16")
+    q, gate, k, v = views(proj)
+    for (a, b), (o, tol) in attention_64(q, k, v, gate, bounds, 0.0, 0, True).items():
+        assert ((att[a:b].double() - o).abs() <= tol + U["bf16"] * o.abs()).all()
+    z = y.double() @ head.double().T
+    want = torch.log_softmax(z, 1)
+    e = 2 * (dim + 8) * U32 * (y.double().abs() @ head.double().abs().T).amax()
+    assert ((logp.double() - want.gather(1, targets.long())).abs() <= 2 * e + 2.0**-16).all()
+    assert ((best.double() - torch.topk(want, 3, 1).values).abs() <= 4 * e + 2.0**-16).all()
+
+    # Each prompt alone: the same rotations, then attention sums in another order.  Its
+    # rounding moves att by 2^-7 of sum p |v| at most, that moves x by 2^-7 sum |att||w| and a step.
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        if a == b:
+            continue
+        one = torch.tensor([0, b - a], dtype=torch.int32, device="cuda")
+        part = before[a:b].clone()
+        att1, _, _, (logp1, ent1, _, _) = through(part, res[a:b].contiguous(), pos[:, a:b].contiguous(), one, targets[a:b].contiguous())
+        assert torch.equal(part, proj[a:b])
+        tol = attention_64(q[a:b], k[a:b], v[a:b], gate[a:b], [0, b - a], 0.0, 0, True)[0, b - a][1]
+        assert ((att1.double() - att[a:b].double()).abs() <= 2 * tol + 2 * U["bf16"] * att1.double().abs()).all()
+        # scores: the norm and the head see vectors that differ by bf16 steps
+        assert (logp1 - logp[a:b]).abs().max() <= 0.1 and (ent1 - ent[a:b]).abs().max() <= 0.1
+
+
+def test_packed_operators_agree_with_the_padded_ones():
+    """One text prompt through clef_op_qk_norm_rope + clef_op_attention and through the
+    packed operators: the former round the norm, cos, sin and both products (four more
+    bf16 half-steps of |y_lo| + |y_hi|), and the attention output before its gate."""
+    import torch
+
+    hq, hkv, d, n, rot = 4, 2, 128, 300, 64
+    g = generator(22)
+    a = normal(g, n, 2 * hq * d + 2 * hkv * d)
+    qw, kw = normal(g, d, std=0.1), normal(g, d, std=0.1)
+    b = a.clone()
+    _lib.check(lib().clef_op_qk_norm_rope(_lib.DTYPE_BF16, a.data_ptr(), 1, n, hq, hkv, d, rot / d, 1e4, qw.data_ptr(), kw.data_ptr(), 1e-6,
+                                          stream()))
+    q, k = b[:, : 2 * hq * d].view(n, hq, 2 * d)[..., :d], b[:, 2 * hq * d : 2 * hq * d + hkv * d].view(n, hkv, d)
+    _, scale = rope_64(q, qw, torch.arange(n, device="cuda")[None], None, False, rot, 1e4)
+    run_rope(q, k, q, k, torch.arange(n, device="cuda", dtype=torch.int32)[None], None, False, rot, 1e4, qw, kw)
+    off = (a[:, : 2 * hq * d].view(n, hq, 2 * d)[..., :d].double() - q.double()).abs().cpu().numpy()
+    assert (off <= 6 * U["bf16"] * scale + 1e-30).all()
+    out1, out2 = torch.empty(n, hq * d, dtype=torch.bfloat16, device="cuda"), torch.empty(n, hq, d, dtype=torch.bfloat16, device="cuda")
+    _lib.check(lib().clef_op_attention(_lib.DTYPE_BF16, b.data_ptr(), None, out1.data_ptr(), 1, n, hq, hkv, d, 0.0, 0, stream()))
+    v, gate = b[:, 2 * hq * d + hkv * d :].view(n, hkv, d), b[:, : 2 * hq * d].view(n, hq, 2 * d)[..., d:]
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    run_attention(q, k, v, gate, out2, cu)
+    tol = attention_64(q, k, v, gate, [0, n], 0.0, 0, True)[0, n][1]
+    y = out2.double()
+    assert ((out1.view(n, hq, d).double() - y).abs() <= 2 * tol + 4 * U["bf16"] * y.abs() + 1e-30).all()
