@@ -13,9 +13,12 @@
 //
 // Masked entries are excluded by selection, so scores of foreign keys may hold
 // anything.  Their values enter P.V times zero, which is not zero where a value
-// is infinite or NaN; a row whose result holds a NaN is therefore computed once
-// more from its own keys alone (attn_packed_redo), so that what a sequence
-// holds never reaches another.
+// is infinite or NaN; a row whose result holds a NaN (on the tensor cores, where
+// a tile's exponentials use the maximum of the tiles before, or an infinity) is
+// therefore computed once more from its own keys alone (attn_packed_redo), so
+// that what a sequence holds never reaches another.  A row whose own scores
+// hold a NaN is NaN whatever else it sees and is left as it came out: a prompt
+// gone NaN costs no second pass.
 //
 // attn_packed_simt_kernel (here): FP32 products on the CUDA cores, any head
 // size to 256, any strides and alignment.  64 x 64 score tiles, 4 x 4 a
@@ -74,7 +77,7 @@ __device__ __forceinline__ float packed_score(float x, float scale, float softca
 // One row again from its own keys [lo, row] alone, by the whole block (NT
 // threads, d <= NT): chunks of NT keys, a key a thread for the scores, an
 // element a thread for P.V.  smem: 256 + 2 * NT floats.  For rows that came
-// out NaN; every thread of the block must call it.
+// out infinite or NaN; every thread of the block must call it.
 template <typename T, int NT>
 __device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int row, int lo, float* smem) {
   float* sq = smem;            // [d]
@@ -108,7 +111,7 @@ __device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h,
     const float mn = fmaxf(m, red[0]);
     const float corr = m == mn ? 1.f : expf(m - mn);
     m = mn;
-    sp[tid] = tid < n ? expf(x - mn) : 0.f;
+    sp[tid] = x == -INFINITY ? 0.f : expf(x - mn);  // also where no score so far is above -inf
     __syncthreads();
     l *= corr;
     o *= corr;
@@ -216,53 +219,53 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     __syncthreads();
     way.load(a.v + hk * a.hsv, a.ldv, k0, q_end, a.d, vec);
     if (any) {
-    float s[4][4] = {};
+      float s[4][4] = {};
 #pragma unroll 4
-    for (int c = 0; c < DP; c += 4) {
-      float4 qf[4], kf[4];
+      for (int c = 0; c < DP; c += 4) {
+        float4 qf[4], kf[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * LD + c]);
+        for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * LD + c]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sKV[(tx + 16 * j) * LD + c]);
+        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sKV[(tx + 16 * j) * LD + c]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][j] = fmaf(qf[i].x, kf[j].x, s[i][j]);
+            s[i][j] = fmaf(qf[i].y, kf[j].y, s[i][j]);
+            s[i][j] = fmaf(qf[i].z, kf[j].z, s[i][j]);
+            s[i][j] = fmaf(qf[i].w, kf[j].w, s[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = q0 + ty * 4 + i;
+        float mt = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(qf[i].x, kf[j].x, s[i][j]);
-          s[i][j] = fmaf(qf[i].y, kf[j].y, s[i][j]);
-          s[i][j] = fmaf(qf[i].z, kf[j].z, s[i][j]);
-          s[i][j] = fmaf(qf[i].w, kf[j].w, s[i][j]);
+          const int key = k0 + tx + 16 * j;
+          s[i][j] = key >= lo[i] && key <= row ? packed_score(s[i][j], scale, a.softcap) * LOG2E : -INFINITY;
+          mt = fmaxf(mt, s[i][j]);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = q0 + ty * 4 + i;
-      float mt = -INFINITY;
+        for (int w = 8; w > 0; w >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, w));
+        const float mn = fmaxf(m[i], mt);
+        const float base = mn == -INFINITY ? 0.f : mn;  // no key of this row yet: every p is exp2(-inf) = 0
+        const float corr = exp2f(m[i] - base);
+        m[i] = mn;
+        float ps = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = k0 + tx + 16 * j;
-        s[i][j] = key >= lo[i] && key <= row ? packed_score(s[i][j], scale, a.softcap) * LOG2E : -INFINITY;
-        mt = fmaxf(mt, s[i][j]);
+        for (int j = 0; j < 4; ++j) {
+          const float p = exp2f(s[i][j] - base);
+          sP[(ty * 4 + i) * LDP + tx + 16 * j] = p;
+          ps += p;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
+        l[i] = l[i] * corr + ps;
+#pragma unroll
+        for (int c = 0; c < 4 * NC; ++c) o[i][c] = corr == 0.f ? 0.f : o[i][c] * corr;
       }
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, w));
-      const float mn = fmaxf(m[i], mt);
-      const float base = mn == -INFINITY ? 0.f : mn;  // no key of this row yet: every p is exp2(-inf) = 0
-      const float corr = exp2f(m[i] - base);
-      m[i] = mn;
-      float ps = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(s[i][j] - base);
-        sP[(ty * 4 + i) * LDP + tx + 16 * j] = p;
-        ps += p;
-      }
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
-      l[i] = l[i] * corr + ps;
-#pragma unroll
-      for (int c = 0; c < 4 * NC; ++c) o[i][c] = corr == 0.f ? 0.f : o[i][c] * corr;
-    }
     }
     __syncthreads();  // the key tile has been read
     way.store(sKV, LD);
@@ -270,25 +273,25 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     if (k0 + BK < q_end) way.load(a.k + hk * a.hsk, a.ldk, k0 + BK, q_end, a.d, vec);
     if (any) {
 #pragma unroll 2
-    for (int j = 0; j < BK; j += 4) {
-      float4 pf[4];
+      for (int j = 0; j < BK; j += 4) {
+        float4 pf[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pf[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * LDP + j]);
+        for (int i = 0; i < 4; ++i) pf[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * LDP + j]);
 #pragma unroll
-      for (int jj = 0; jj < 4; ++jj)
+        for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float4 vf = *reinterpret_cast<const float4*>(&sKV[(j + jj) * LD + 64 * c + tx * 4]);
+          for (int c = 0; c < NC; ++c) {
+            const float4 vf = *reinterpret_cast<const float4*>(&sKV[(j + jj) * LD + 64 * c + tx * 4]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
-            o[i][4 * c] = fmaf(p, vf.x, o[i][4 * c]);
-            o[i][4 * c + 1] = fmaf(p, vf.y, o[i][4 * c + 1]);
-            o[i][4 * c + 2] = fmaf(p, vf.z, o[i][4 * c + 2]);
-            o[i][4 * c + 3] = fmaf(p, vf.w, o[i][4 * c + 3]);
+            for (int i = 0; i < 4; ++i) {
+              const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
+              o[i][4 * c] = fmaf(p, vf.x, o[i][4 * c]);
+              o[i][4 * c + 1] = fmaf(p, vf.y, o[i][4 * c + 1]);
+              o[i][4 * c + 2] = fmaf(p, vf.z, o[i][4 * c + 2]);
+              o[i][4 * c + 3] = fmaf(p, vf.w, o[i][4 * c + 3]);
+            }
           }
-        }
-    }
+      }
     }
   }
 #pragma unroll
@@ -305,7 +308,8 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
       if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + col]));
       a.out[row * a.ldo + h * a.hso + col] = from_f32<T>(y);
     }
-    if (bad) atomicOr(&s_nan, 1ULL << (ty * 4 + i));
+    // a NaN sum has a NaN (or infinite) score of the row's own: the row is NaN, and stays so
+    if (bad && l[i] == l[i]) atomicOr(&s_nan, 1ULL << (ty * 4 + i));
   }
   __syncthreads();
   for (unsigned long long rows = s_nan; rows; rows &= rows - 1) {

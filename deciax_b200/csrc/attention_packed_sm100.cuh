@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           tc_fence_after();
           const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
           m = mn;
-          l *= corr;
+          l = corr == 0.f ? 0.f : l * corr;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
 #pragma unroll 1
           for (int c = part * DP; c < (part + 1) * DP; c += 16) {
             uint32_t o[16];
@@ -603,7 +603,9 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         }
       }
       const float2 odd = unpair2(odd2);
-      const bool bad = !(l < INFINITY) || odd.x != 0.f || odd.y != 0.f;
+      // a NaN sum has a NaN (or infinite) score of the row's own: the row is NaN, and stays so.
+      // One that overflowed and was rescaled to 0 left NaN in O.
+      const bool bad = l == l && (l == INFINITY || odd.x != 0.f || odd.y != 0.f);
       const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
       if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
       if (D == 64 && whole) fence_async_smem();

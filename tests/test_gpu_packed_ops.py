@@ -395,6 +395,42 @@ def test_attention_packed_infinities_stay_in_their_sequence(dtype, d):
     assert out[a + 20 : a + 25, 2:].isfinite().all() and out[a + 25 : bounds[2]].isnan().any(-1).all()
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
+def test_attention_packed_scores_of_minus_infinity(dtype, d):
+    """A key whose score is -inf has weight 0; a row that sees no other key is NaN."""
+    import torch
+
+    g = generator(21)
+    q, k, v, out = (normal(g, 560, h, d, dtype=dtype) for h in (2, 1, 1, 2))
+    q[40:500, :, 0] = q[40:500, :, 0].abs() + 0.5
+    k[40:240, 0, 0] = float("-inf")
+    v[500:] = float("nan")  # the next sequence, in the same tiles
+    run_attention(q, k, v, None, out, torch.tensor([0, 40, 500, 560], dtype=torch.int32, device="cuda"))
+    assert out[40:240].isnan().all() and out[500:].isnan().all()
+    # a row after those keys is that of a sequence without them
+    for a, b in ((0, 40), (240, 500)):
+        y, tol = attention_64(q, k, v, None, [a, b], 0.0, 0, dtype == "bf16")[a, b]
+        assert ((out[a:b].double() - y).abs() <= tol + U[dtype] * y.abs()).all()
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
+def test_attention_packed_a_prompt_gone_nan(dtype, d):
+    """All of the middle sequence is NaN; its neighbours keep their values."""
+    import torch
+
+    g = generator(22)
+    cu = torch.tensor([0, 70, 400, 470], dtype=torch.int32, device="cuda")
+    q, k, v, gt = (normal(g, 470, h, d, dtype=dtype) for h in (4, 2, 2, 4))
+    out = torch.empty_like(q)
+    for x in (q, k, v, gt):
+        x[70:400] = float("nan")
+    run_attention(q, k, v, gt, out, cu)
+    assert out[70:400].isnan().all()
+    for a, b in ((0, 70), (400, 470)):
+        y, tol = attention_64(q, k, v, gt, [a, b], 0.0, 0, dtype == "bf16")[a, b]
+        assert ((out[a:b].double() - y).abs() <= tol + U[dtype] * y.abs()).all()
+
+
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("bf16", 30), ("fp32", 64)])
 def test_attention_packed_offsets_past_32_bits(dtype, d):
     """The last rows of buffers of more than 2^31 elements."""
