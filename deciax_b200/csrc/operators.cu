@@ -29,6 +29,7 @@ static int op_guarded(F&& f) {
     return CLEF_OK;
   } catch (const Error& e) {
     set_global_error(e.what());
+    if (e.code == CLEF_ECUDA) (void)cudaGetLastError();  // a failed allocation is not the next launch's error
     return e.code;
   } catch (const std::exception& e) {
     set_global_error(e.what());

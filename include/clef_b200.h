@@ -342,7 +342,8 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
  * x, largest first, equal ones by the lowest id (top <= 32).  Products and sums
  * are FP32 and x is not rounded.  n_targets = 0, entropy = NULL and top = 0 leave
  * an output out; rows = 0 does nothing.  A row with a NaN logit has NaN logprobs
- * and entropy.  16-byte aligned rows (pointers, ldh and ldw, whole 16 bytes of
+ * and entropy; one with an infinite logit has NaN entropy, and its logprobs may be
+ * NaN.  16-byte aligned rows (pointers, ldh and ldw, whole 16 bytes of
  * dim) run on the tensor cores, FP32 values as three bf16 parts each (what is left
  * out of a product is below 2^-24 of it).  Scratch comes from the library's stream-ordered
  * pool: make one call on each device before capturing one into a graph. */
