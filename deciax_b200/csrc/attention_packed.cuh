@@ -201,13 +201,14 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
   for (int i = 0; i < 4; ++i) lo[i] = s_lo[ty * 4 + i];
   const int k_begin = s_lo[q_first - q0];
   const float scale = rsqrtf(static_cast<float>(a.d));
-  float m[4], l[4], o[4][4 * NC];
+  float m[4], l[4];
+  uint64_t o[4][2 * NC];  // pairs of columns
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
+    for (int c = 0; c < 2 * NC; ++c) o[i][c] = 0ull;
   }
   // rows of this warp: tiles above the last or below the first one's keys cost it nothing
   const int w_last = q0 + (tid / 32) * 8 + 7, w_lo = s_lo[(tid / 32) * 8];
@@ -219,24 +220,30 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     __syncthreads();
     way.load(a.v + hk * a.hsv, a.ldv, k0, q_end, a.d, vec);
     if (any) {
-      float s[4][4] = {};
+      uint64_t s2[4][4] = {};  // sums of even and odd elements
 #pragma unroll 4
       for (int c = 0; c < DP; c += 4) {
-        float4 qf[4], kf[4];
+        ulonglong2 qf[4], kf[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * LD + c]);
+        for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const ulonglong2*>(&sQ[(ty * 4 + i) * LD + c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(&sKV[(tx + 16 * j) * LD + c]);
+        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const ulonglong2*>(&sKV[(tx + 16 * j) * LD + c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[i][j] = fmaf(qf[i].x, kf[j].x, s[i][j]);
-            s[i][j] = fmaf(qf[i].y, kf[j].y, s[i][j]);
-            s[i][j] = fmaf(qf[i].z, kf[j].z, s[i][j]);
-            s[i][j] = fmaf(qf[i].w, kf[j].w, s[i][j]);
+            s2[i][j] = fma2(qf[i].x, kf[j].x, s2[i][j]);
+            s2[i][j] = fma2(qf[i].y, kf[j].y, s2[i][j]);
           }
       }
+      float s[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = unpair2(s2[i][j]);
+          s[i][j] = x.x + x.y;
+        }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = q0 + ty * 4 + i;
@@ -264,7 +271,7 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
         for (int w = 8; w > 0; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
         l[i] = l[i] * corr + ps;
 #pragma unroll
-        for (int c = 0; c < 4 * NC; ++c) o[i][c] = corr == 0.f ? 0.f : o[i][c] * corr;
+        for (int c = 0; c < 2 * NC; ++c) o[i][c] = corr == 0.f ? 0ull : mul2(o[i][c], pair2(corr, corr));
       }
     }
     __syncthreads();  // the key tile has been read
@@ -278,19 +285,23 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
 #pragma unroll
         for (int i = 0; i < 4; ++i) pf[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * LDP + j]);
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
+        for (int jj = 0; jj < 4; ++jj) {
+          uint64_t p2[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
+            p2[i] = pair2(p, p);
+          }
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const float4 vf = *reinterpret_cast<const float4*>(&sKV[(j + jj) * LD + 64 * c + tx * 4]);
+            const ulonglong2 vf = *reinterpret_cast<const ulonglong2*>(&sKV[(j + jj) * LD + 64 * c + tx * 4]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float p = jj == 0 ? pf[i].x : jj == 1 ? pf[i].y : jj == 2 ? pf[i].z : pf[i].w;
-              o[i][4 * c] = fmaf(p, vf.x, o[i][4 * c]);
-              o[i][4 * c + 1] = fmaf(p, vf.y, o[i][4 * c + 1]);
-              o[i][4 * c + 2] = fmaf(p, vf.z, o[i][4 * c + 2]);
-              o[i][4 * c + 3] = fmaf(p, vf.w, o[i][4 * c + 3]);
+              o[i][2 * c] = fma2(p2[i], vf.x, o[i][2 * c]);
+              o[i][2 * c + 1] = fma2(p2[i], vf.y, o[i][2 * c + 1]);
             }
           }
+        }
       }
     }
   }
@@ -303,7 +314,8 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     for (int c = 0; c < 4 * NC; ++c) {
       const int col = 64 * (c / 4) + tx * 4 + (c & 3);
       if (col >= a.d) continue;
-      float y = o[i][c] / l[i];
+      const float2 oo = unpair2(o[i][c / 2]);
+      float y = (c & 1 ? oo.y : oo.x) / l[i];
       bad |= y != y;
       if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + col]));
       a.out[row * a.ldo + h * a.hso + col] = from_f32<T>(y);
