@@ -101,7 +101,10 @@ __device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h,
       x = packed_score(s, scale, a.softcap);
     }
     red[tid] = x;
-    __syncthreads();
+    if (__syncthreads_or(x != x)) {  // a NaN score: the row is NaN
+      if (tid < a.d) a.out[row * a.ldo + h * a.hso + tid] = from_f32<T>(__int_as_float(0x7fffffff));
+      return;
+    }
     for (int w = NT; w > 1;) {  // NT need not be a power of two
       const int half = (w + 1) / 2;
       if (tid + half < w) red[tid] = fmaxf(red[tid], red[tid + half]);

@@ -129,6 +129,20 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// A pair's three bf16 parts, packed (of an infinity: one infinity and two NaN).
+__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const uint64_t minus = pair2(-1.f, -1.f);
+  auto rest = [&](uint64_t v, uint32_t part) {
+    return fma2(pair2(__uint_as_float(part << 16), __uint_as_float(part & 0xffff0000u)), minus, v);
+  };
+  h = pack_bf16x2(x, y);
+  const uint64_t r = rest(pair2(x, y), h);
+  const float2 rf = unpair2(r);
+  m = pack_bf16x2(rf.x, rf.y);
+  const float2 lf = unpair2(rest(r, m));
+  l = pack_bf16x2(lf.x, lf.y);
+}
+
 __device__ __forceinline__ void record_status(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }

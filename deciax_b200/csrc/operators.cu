@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "attention_packed.cuh"
+#include "attention_packed_f32_sm100.cuh"
 #include "attention_packed_sm100.cuh"
 #include "common.cuh"
 #include "host.cuh"
@@ -69,6 +70,18 @@ static int size_of(int dtype) {
   REQUIRE(dtype == CLEF_DTYPE_BF16 || dtype == CLEF_DTYPE_F32, "dtype must be CLEF_DTYPE_BF16 or CLEF_DTYPE_F32");
   return dtype == CLEF_DTYPE_BF16 ? 2 : 4;
 }
+
+// Stream-ordered scratch of one call, freed on the stream when the call's kernels are enqueued.
+struct OpScratch {
+  cudaStream_t st;
+  void* p = nullptr;
+  OpScratch(size_t bytes, cudaStream_t s) : st(s) {
+    CUDA_CHECK(cudaMallocFromPoolAsync(&p, bytes, op_scratch_pool(current_device()), st));
+  }
+  ~OpScratch() {
+    if (p) cudaFreeAsync(p, st);
+  }
+};
 
 static void rope_frequencies(RopeAxesArgs& a, int rot, double theta, int axes, const int32_t* sections,
                              int interleaved) {
@@ -178,6 +191,40 @@ static void launch_packed_tc(const AttnPackedMaps& maps, const AttnPackedArgs<bf
   CUDA_CHECK(cudaGetLastError());
 }
 
+template <int D, bool CAP>
+static void launch_packed_f32_tc(const AttnPackedArgs<float>& a, cudaStream_t st) {
+  using Sh = AttnPackedF32Shape<D>;
+  const auto rows = [](const void* p, long long ld, long long hs, int heads) {
+    return !p || (aligned16(p) && ld % 4 == 0 && (heads == 1 || hs % 4 == 0));
+  };
+  SplitHeadsArgs sp{};
+  sp.x[0] = a.q, sp.x[1] = a.k, sp.x[2] = a.v;
+  sp.ld[0] = a.ldq, sp.ld[1] = a.ldk, sp.ld[2] = a.ldv;
+  sp.hs[0] = a.hsq, sp.hs[1] = a.hsk, sp.hs[2] = a.hsv;
+  sp.heads[0] = a.H, sp.heads[1] = sp.heads[2] = a.Hk;
+  sp.tokens = a.tokens;
+  sp.d = a.d;
+  sp.d8 = (a.d + 7) / 8 * 8;
+  sp.vec = a.d % 4 == 0 && rows(a.q, a.ldq, a.hsq, a.H) && rows(a.k, a.ldk, a.hsk, a.Hk) && rows(a.v, a.ldv, a.hsv, a.Hk);
+  const size_t row = static_cast<size_t>(a.tokens) * sp.d8;  // elements of a head of one part
+  OpScratch scratch(3 * row * (a.H + 2 * a.Hk) * sizeof(bf16), st);
+  sp.out[0] = static_cast<bf16*>(scratch.p);
+  sp.out[1] = sp.out[0] + 3 * row * a.H;
+  sp.out[2] = sp.out[1] + 3 * row * a.Hk;
+  const long long groups = static_cast<long long>(row / 8) * (a.H + 2 * a.Hk);
+  REQUIRE(groups < (1LL << 38), "too many rows for one call");
+  AttnPackedF32Maps maps;
+  maps.q = tmap_bf16_heads(sp.out[0], 3 * a.tokens, a.H, sp.d8, static_cast<long long>(a.H) * sp.d8, sp.d8);
+  maps.k = tmap_bf16_heads(sp.out[1], 3 * a.tokens, a.Hk, sp.d8, static_cast<long long>(a.Hk) * sp.d8, sp.d8);
+  maps.v = tmap_bf16_heads(sp.out[2], 3 * a.tokens, a.Hk, sp.d8, static_cast<long long>(a.Hk) * sp.d8, sp.d8);
+  split_heads_kernel<<<static_cast<int>((groups + 255) / 256), 256, 0, st>>>(sp);
+  CUDA_CHECK(cudaGetLastError());
+  const bool vec = a.d % 4 == 0 && rows(a.gate, a.ldg, a.hsg, a.H) && rows(a.out, a.ldo, a.hso, a.H);
+  allow_smem(attn_packed_f32_tc_kernel<D, CAP>, Sh::SMEM);
+  attn_packed_f32_tc_kernel<D, CAP><<<dim3(a.H, (a.tokens + 127) / 128), Sh::THREADS, Sh::SMEM, st>>>(maps, a, vec);
+  CUDA_CHECK(cudaGetLastError());
+}
+
 template <typename T>
 static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
@@ -200,6 +247,16 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
         cap ? launch_packed_tc<128, true>(maps, a, st) : launch_packed_tc<128, false>(maps, a, st);
       else
         cap ? launch_packed_tc<256, true>(maps, a, st) : launch_packed_tc<256, false>(maps, a, st);
+      return;
+    }
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (a.d <= 128) {
+      const bool cap = a.softcap > 0.f;
+      if (a.d <= 64)
+        cap ? launch_packed_f32_tc<64, true>(a, st) : launch_packed_f32_tc<64, false>(a, st);
+      else
+        cap ? launch_packed_f32_tc<128, true>(a, st) : launch_packed_f32_tc<128, false>(a, st);
       return;
     }
   }
@@ -233,18 +290,6 @@ static void logprob_runs(LogprobArgs& a, int tile, int step, bool equal_tiles, i
     if (share <= step) break;
   }
 }
-
-// Stream-ordered scratch of one call, freed on the stream when the call's kernels are enqueued.
-struct OpScratch {
-  cudaStream_t st;
-  void* p = nullptr;
-  OpScratch(size_t bytes, cudaStream_t s) : st(s) {
-    CUDA_CHECK(cudaMallocFromPoolAsync(&p, bytes, op_scratch_pool(current_device()), st));
-  }
-  ~OpScratch() {
-    if (p) cudaFreeAsync(p, st);
-  }
-};
 
 // Clusters of two CTAs of the pair kernel that fit the device at once.
 template <bool CAP, int K>

@@ -329,20 +329,6 @@ struct LogprobF32Shape {
   static constexpr size_t smem(int top) { return 1024 + STAGES * 6 * TILE + 256 + list_bytes(top); }
 };
 
-// A pair's three bf16 parts, packed (of an infinity: one infinity and two NaN).
-__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
-  const uint64_t minus = pair2(-1.f, -1.f);
-  auto rest = [&](uint64_t v, uint32_t part) {
-    return fma2(pair2(__uint_as_float(part << 16), __uint_as_float(part & 0xffff0000u)), minus, v);
-  };
-  h = pack_bf16x2(x, y);
-  const uint64_t r = rest(pair2(x, y), h);
-  const float2 rf = unpair2(r);
-  m = pack_bf16x2(rf.x, rf.y);
-  const float2 lf = unpair2(rest(r, m));
-  l = pack_bf16x2(lf.x, lf.y);
-}
-
 // out[p][row][dim_out]: part p of the rows' values, eight a thread; dim_out = dim rounded up to 8.
 __global__ void __launch_bounds__(256)
     split_rows_kernel(const float* __restrict__ x, long long ldx, int rows, int dim, int dim_out, __nv_bfloat16* out) {
