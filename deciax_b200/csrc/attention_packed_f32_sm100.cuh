@@ -265,9 +265,11 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
         if (live) lo = packed_first_key(a, row, s0, s1);
       }
     }
-    const int lo_min = __reduce_min_sync(0xffffffffu, lo), w_last = q0 + q4 * 32 + 31;
+    const int lo_max = __reduce_max_sync(0xffffffffu, lo), lo_min = __reduce_min_sync(0xffffffffu, lo);
+    const int w_first = q0 + q4 * 32, w_last = w_first + 31;
     const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
-    const float scale = rsqrtf(static_cast<float>(a.d));
+    const float scale = rsqrtf(static_cast<float>(a.d)), scale_cap = scale * inverse_cap(a.softcap);
+    const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
     float m = -INFINITY, l = 0.f;  // the maximum P is taken against (log2 units); this part's sum
     bool fail = false;  // a failed wait: the two warps of a row leave together, by their exchange
     bool ok = true;
@@ -281,19 +283,26 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
       tc_fence_after();
       const uint32_t at = tmem + lanes + s * Sh::S_BUF + c0;  // this part's scores, then its P
       const bool none = k0 > w_last || k0 + 31 < lo_min;     // keys that every row of the warp masks
-      float x[32], mt = -INFINITY;
+      uint32_t z[32];
+      float mt = -INFINITY;
       if (!fail && !none) {
-        uint32_t big[32], small[32];
-        tmem_ld32(at, big);
+        uint32_t small[32];
+        tmem_ld32(at, z);
         tmem_ld32(at + BK, small);
         tmem_wait_ld();
-        const int top = row - k0, low = lo - k0;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float z = __uint_as_float(big[c]) + __uint_as_float(small[c]);
-          x[c] = c >= low && c <= top ? (CAP ? packed_score(z, scale, a.softcap) : z * scale) * LOG2E : -INFINITY;
-          mt = fmaxf(mt, x[c]);
+        for (int c = 0; c < 32; ++c) z[c] = __float_as_uint(__uint_as_float(z[c]) + __uint_as_float(small[c]));
+        if constexpr (CAP) cap_scores(z, scale_cap, a.softcap);
+        if (k0 + 31 > w_first || k0 < lo_max) {  // some key is masked for some row of the warp
+          const int top = row - k0, low = lo - k0;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) z[c] = c >= low && c <= top ? z[c] : 0xff800000u;  // -inf
         }
+        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+          best[c / 2 & 3] = max3(best[c / 2 & 3], __uint_as_float(z[c]), __uint_as_float(z[c + 1]));
+        mt = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * scale_log2;
       }
       float* mine = xbuf + (t & 1) * 256;
       mine[part * 128 + r] = mt;
@@ -327,18 +336,19 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
         m = mn;
         l *= corr;
       }
-      // P = exp2(x - m) in three parts: P_h over the sums of h h' with P_m behind it, P_l over the others
-      const float base = m == -INFINITY ? 0.f : m;  // no key yet: every p is exp2(-inf) = 0
-      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+      // P = exp2(z scale_log2 - m) in three parts: P_h over the sums of h h' with P_m behind it, P_l over the others
+      const float neg_m = m == -INFINITY ? 0.f : -m;  // no key yet: every p is exp2(-inf) = 0
+      const uint64_t scale2 = pair2(scale_log2, scale_log2), neg_m2 = pair2(neg_m, neg_m);
+      uint64_t ps[2] = {0ull, 0ull};  // sums of even and odd keys
       uint32_t ph[16], pm[16], pl[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         if (none) {
           ph[e] = pm[e] = pl[e] = 0u;
         } else {
-          const float p0 = ex2_approx(x[2 * e] - base), p1 = ex2_approx(x[2 * e + 1] - base);
-          ps[2 * (e & 1)] += p0;
-          ps[2 * (e & 1) + 1] += p1;
+          const float2 x = unpair2(fma2(pair2(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), scale2, neg_m2));
+          const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+          ps[e & 1] = add2(ps[e & 1], pair2(p0, p1));
           split3(p0, p1, ph[e], pm[e], pl[e]);
         }
       }
@@ -350,7 +360,8 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
       }
       tc_fence_before();
       mbar_arrive(&pfull[s]);
-      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      const float2 sum = unpair2(add2(ps[0], ps[1]));
+      l += sum.x + sum.y;
     }
     ok = ok && !fail;
     if (!ok) *abort_flag = 1;

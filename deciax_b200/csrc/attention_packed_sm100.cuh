@@ -94,6 +94,40 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
   return r;
 }
 
+// Scores x = softcap tanh(scale_cap x), 32 of a row.  While none of the warp's
+// lies beyond the series of tanh_flat (0.45: scores below 0.42 softcap), the
+// series alone, two scores at a time; else tanh_flat for each.
+__device__ __forceinline__ void cap_scores(uint32_t (&x)[32], float scale_cap, float softcap) {
+  const uint64_t sc2 = pair2(scale_cap, scale_cap), cap2 = pair2(softcap, softcap);
+  uint64_t y[16];
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    y[e] = mul2(pair2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), sc2);
+    const float2 u = unpair2(y[e]);
+    top = max3(top, fabsf(u.x), fabsf(u.y));
+  }
+  if (__any_sync(0xffffffffu, top >= kTanhSeries)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float2 u = unpair2(y[e]);
+      x[2 * e] = __float_as_uint(softcap * tanh_flat(u.x));
+      x[2 * e + 1] = __float_as_uint(softcap * tanh_flat(u.y));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t y2 = mul2(y[e], y[e]);
+      uint64_t p = pair2(kTanh[5], kTanh[5]);
+#pragma unroll
+      for (int i = 4; i >= 0; --i) p = fma2(p, y2, pair2(kTanh[i], kTanh[i]));
+      const float2 t = unpair2(mul2(fma2(mul2(y[e], y2), p, y[e]), cap2));
+      x[2 * e] = __float_as_uint(t.x);
+      x[2 * e + 1] = __float_as_uint(t.y);
+    }
+  }
+}
+
 // Sigmoids of 8 Q gates (bf16).  Two share one reciprocal, 1/a = b / (ab), for
 // the special-function unit gives 16 results a cycle and SM (exponentials from
 // the FMA pipe instead, for a quarter or half of them, were no faster).
@@ -386,7 +420,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     const int lo_max = __reduce_max_sync(0xffffffffu, lo), lo_min = __reduce_min_sync(0xffffffffu, lo);
     const int w_first = q0 + q4 * 32, w_last = w_first + 31;
     const uint32_t t_lane = static_cast<uint32_t>(q4 * 32) << 16;
-    const float scale = rsqrtf(static_cast<float>(a.d));
+    const float scale = rsqrtf(static_cast<float>(a.d)), scale_cap = scale * inverse_cap(a.softcap);
     const float scale_log2 = CAP ? LOG2E : scale * LOG2E;  // a capped score is scaled already
     // m: the maximum P is taken against (log2 units), at most 8 below that of the
     // tiles before the last; l: this part's sum; last: this part's maximum of the last tile
@@ -429,11 +463,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
         for (int w = 0; w < NWP; ++w) {
           if (none(w)) continue;
           const int k = k0 + 32 * w;
-          if constexpr (CAP) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              sr[w][c] = __float_as_uint(packed_score(__uint_as_float(sr[w][c]), scale, a.softcap));
-          }
+          if constexpr (CAP) cap_scores(sr[w], scale_cap, a.softcap);
           if (k + 31 > w_first || k < lo_max) {  // some key is masked for some row of the warp
             const int top = row - k, low = lo - k;
 #pragma unroll
