@@ -69,22 +69,6 @@ __device__ __forceinline__ int packed_first_key(const A& a, int row, int lo_seq,
   return a.window > 0 ? max(start, row - a.window + 1) : start;
 }
 
-// tanh without a branch (tanhf's, taken by some lanes and not by others, and the
-// division by softcap cost the FP32 tiles a quarter of their time): below 0.45
-// the Taylor series to y^13, whose next term is 2e-8 of y; above it
-// 1 - 2 / (1 + e^2|y|), off by at most 0.41 (2^-22 + 2^-23) there.
-constexpr float kTanhSeries = 0.45f;
-static __device__ constexpr float kTanh[6] = {-1.f / 3.f,  2.f / 15.f,          -17.f / 315.f,
-                                              62.f / 2835.f, -1382.f / 155925.f, 21844.f / 6081075.f};  // y^3 .. y^13
-__device__ __forceinline__ float tanh_flat(float y) {
-  const float u = fabsf(y), y2 = y * y;
-  const float big = fmaf(-2.f, rcp_approx(1.f + ex2_approx(u * 2.885390081777927f)), 1.f);  // 2 log2 e
-  float p = kTanh[5];
-#pragma unroll
-  for (int i = 4; i >= 0; --i) p = fmaf(p, y2, kTanh[i]);
-  return u < kTanhSeries ? fmaf(y * y2, p, y) : copysignf(big, y);
-}
-
 // 1 / softcap, 0 without one; finite, so that a score of 0 stays 0 under any cap.
 __device__ __forceinline__ float inverse_cap(float softcap) { return softcap > 0.f ? fminf(1.f / softcap, 3e38f) : 0.f; }
 

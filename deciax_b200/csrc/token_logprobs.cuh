@@ -168,28 +168,57 @@ __device__ __forceinline__ void scan32(RowState& st, TopList<K>& list, float (&x
     st.s *= f;
     st.m = zmax;
   }
-  float ps[4] = {0.f, 0.f, 0.f, 0.f}, pt[4] = {0.f, 0.f, 0.f, 0.f};
   const float neg_m = -st.m;
-  if (valid >= 32) {
+  if (valid >= 32) {  // two columns at a time
+    const uint64_t log2e2 = pair2(LOG2E, LOG2E), neg_m2 = pair2(neg_m, neg_m);
+    uint64_t ps[2] = {0ull, 0ull}, pt[2] = {0ull, 0ull};
+    auto add = [&](int e, uint64_t z2) {
+      const uint64_t d2 = fma2(z2, log2e2, neg_m2);
+      const float2 d = unpair2(d2);
+      const uint64_t e2 = pair2(ex2_approx(d.x), ex2_approx(d.y));
+      ps[e & 1] = add2(ps[e & 1], e2);
+      pt[e & 1] = fma2(d2, e2, pt[e & 1]);
+    };
+    if constexpr (CAP) {
+      // tanh by its series where all 32 columns allow it (2e-8 off), else by tanhf
+      const float inv = fminf(1.f / softcap, 3e38f);
+      const uint64_t inv2 = pair2(inv, inv), cap2 = pair2(softcap, softcap);
+      float far = 0.f;
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-      const float d = fmaf(capped<CAP>(x[c], softcap), LOG2E, neg_m);
-      const float e = ex2_approx(d);
-      ps[c & 3] += e;
-      pt[c & 3] = fmaf(d, e, pt[c & 3]);
+      for (int c = 0; c < 32; ++c) far = fmaxf(far, fabsf(x[c]));
+      if (far * inv < kTanhSeries) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint64_t y = mul2(pair2(x[2 * e], x[2 * e + 1]), inv2), y2 = mul2(y, y);
+          uint64_t p = pair2(kTanh[5], kTanh[5]);
+#pragma unroll
+          for (int i = 4; i >= 0; --i) p = fma2(p, y2, pair2(kTanh[i], kTanh[i]));
+          add(e, mul2(fma2(mul2(y, y2), p, y), cap2));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) add(e, pair2(capped<CAP>(x[2 * e], softcap), capped<CAP>(x[2 * e + 1], softcap)));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) add(e, pair2(x[2 * e], x[2 * e + 1]));
     }
+    const float2 s2 = unpair2(add2(ps[0], ps[1])), t2 = unpair2(add2(pt[0], pt[1]));
+    st.s += s2.x + s2.y;
+    st.t += t2.x + t2.y;
   } else {
+    float ps = 0.f, pt = 0.f;
 #pragma unroll
     for (int c = 0; c < 32; ++c)
       if (c < valid) {
         const float d = fmaf(capped<CAP>(x[c], softcap), LOG2E, neg_m);
         const float e = ex2_approx(d);
-        ps[c & 3] += e;
-        pt[c & 3] = fmaf(d, e, pt[c & 3]);
+        ps += e;
+        pt = fmaf(d, e, pt);
       }
+    st.s += ps;
+    st.t += pt;
   }
-  st.s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-  st.t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
   list.take(x, best, col, top, area, r);
 }
 
