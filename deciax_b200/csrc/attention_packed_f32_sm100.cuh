@@ -138,6 +138,8 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
     s_nan[0] = s_nan[1] = s_nan[2] = s_nan[3] = 0u;
     fence_barrier_init();
     fence_async_smem();
+    // launched while the parts are still being written: only these loads wait for them
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     load_parts(sQ, &maps.q, qfull, h, q0, BQ);
     load_parts(sK, &maps.k, kfull, hk, k_end - BK, BK);
   }

@@ -221,8 +221,17 @@ static void launch_packed_f32_tc(const AttnPackedArgs<float>& a, cudaStream_t st
   CUDA_CHECK(cudaGetLastError());
   const bool vec = a.d % 4 == 0 && rows(a.gate, a.ldg, a.hsg, a.H) && rows(a.out, a.ldo, a.hso, a.H);
   allow_smem(attn_packed_f32_tc_kernel<D, CAP>, Sh::SMEM);
-  attn_packed_f32_tc_kernel<D, CAP><<<dim3(a.H, (a.tokens + 127) / 128), Sh::THREADS, Sh::SMEM, st>>>(maps, a, vec);
-  CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(a.H, (a.tokens + 127) / 128);
+  cfg.blockDim = dim3(Sh::THREADS);
+  cfg.dynamicSmemBytes = Sh::SMEM;
+  cfg.stream = st;
+  cfg.attrs = early;
+  cfg.numAttrs = 1;
+  CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_packed_f32_tc_kernel<D, CAP>, maps, a, vec));
 }
 
 template <typename T>
@@ -251,7 +260,10 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
     }
   }
   if constexpr (sizeof(T) == 4) {
-    if (a.d <= 128) {
+    // Splitting costs a launch: from a few rows on at heads above 64 (16 heads of 128,
+    // 16 rows: 25 us against 31 on the CUDA cores), from two tiles on below
+    // (4 heads of 64, 128 rows: 27 against 25, 192 rows: 27 against 31).
+    if (a.d <= 128 && a.tokens > (a.d <= 64 ? 128 : 8)) {
       const bool cap = a.softcap > 0.f;
       if (a.d <= 64)
         cap ? launch_packed_f32_tc<64, true>(a, st) : launch_packed_f32_tc<64, false>(a, st);

@@ -322,8 +322,11 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
  * read as keys, may hold anything, and their out is left as it was.  Infinities
  * and NaN of one sequence never reach another.  out must not overlap the
  * inputs.  d <= 256, tokens <= 8388480; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
- * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; anything
- * else on the CUDA cores in FP32. */
+ * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; FP32 with d <= 128
+ * and more than a few tokens also, every value as three bf16 parts (what is left out of a
+ * product is below 2^-24 of it; values below 2^-110 keep fewer bits); anything
+ * else on the CUDA cores in FP32.  FP32 takes scratch, 6 bytes an element of q, k and v, from the
+ * library's stream-ordered pool: make one such call on each device before capturing one into a graph. */
 int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
                              const void* v, int64_t ldv, int64_t hsv, const void* gate, int64_t ldg, int64_t hsg, void* out,
                              int64_t ldo, int64_t hso, const int32_t* cu_seqlens, int n_seqs, int tokens, int hq, int hkv,

@@ -467,6 +467,43 @@ def test_attention_packed_captured_and_replayed_with_other_lengths():
         assert (out[: bounds[0]] == 7).all() and (out[bounds[-1] :] == 7).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_packed_fp32_graphs_and_streams_have_their_own_scratch(d):
+    """Two captured calls replayed side by side, and eager calls on two streams."""
+    import torch
+
+    g = generator(23)
+    cu = torch.tensor([0, 150, 400], dtype=torch.int32, device="cuda")
+    inputs = [[normal(g, 400, h, d, dtype="fp32") for h in (4, 2, 2)] for _ in range(2)]
+    want = [torch.empty_like(x[0]) for x in inputs]
+    for x, o in zip(inputs, want):
+        run_attention(*x, None, o, cu)
+    torch.cuda.synchronize()
+    graphs, outs = [], [torch.empty_like(x[0]) for x in inputs]
+    for x, o in zip(inputs, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            run_attention(*x, None, o, cu)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for run in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, graph, x, o in zip(streams, graphs, inputs, outs):
+            with torch.cuda.stream(s):
+                graph.replay() if run % 2 else run_attention(*x, None, o, cu)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (70, 20.0)])
+@pytest.mark.parametrize("d", [64, 72, 128])
+@pytest.mark.parametrize("layout", ["packed", "odd", "heads"])
+def test_attention_packed_fp32_layouts(layout, d, window, softcap):
+    """Scores on both sides of the cap's bend, rows before the first sequence and behind the last."""
+    check_attention([129, 0, 200, 1, 66], 6, 3, d, "fp32", window=window, softcap=softcap, qscale=6.0, layout=layout, lead=3, pad=70)
+
+
 def test_attention_packed_rows_do_not_depend_on_their_neighbours():
     """Twice the same call gives the same bits, and so do two streams at once."""
     import torch
