@@ -122,6 +122,8 @@ struct RopeShape {
 // the block's tokens are computed once, while the first rows load.  HBM bound:
 // rows come by asynchronous copies, DEPTH on the way, into slots of shared
 // memory that only their lane reads, so nothing waits at a barrier.
+// 131072 tokens x 48 heads of 128, bf16: 556 us, 5.8 TB/s; 4097 x 24 heads of 256, FP32:
+// 36.8 us, 5.5 TB/s.
 // grid (token spans, head groups of blockDim / LANES).
 template <typename T, int LANES>
 __global__ void __launch_bounds__(512) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int span) {

@@ -16,6 +16,10 @@
 // last one (head rows by 16: their MMAs are the bound); one CTA, bound by the
 // head's bytes, cuts it into equal tiles of any multiple of 8 columns, one box
 // each (a last tile in boxes of 16 rows made one row 30 us slower).
+//
+// Vocabulary 256000, dim 3584: 1 row 317 us and 32 rows 333 us, HBM bound (1.835 GB
+// at 5.8 and 5.5 TB/s; a stream of the head with nothing else takes 270 us); 2048
+// rows 2.86 ms, 1316 TFLOP/s, the tensor pipe under the power cap.
 #pragma once
 
 #include "attention_sm100.cuh"
