@@ -26,7 +26,7 @@
 // queries, keys, values and P in shared memory as FP32, pairs of elements (of
 // columns) a multiplication.  Latency bound: 16 warps an SM issue in 42% of the
 // cycles between the tile's barriers (2047 rows, 16 heads of 128, window 200,
-// capped: 182 us; the tensor cores take 70).
+// capped: 182 us; the tensor cores take 63).
 #pragma once
 
 #include "common.cuh"

@@ -18,7 +18,7 @@
 // (two accumulators each) the tensor memory's 512 columns.  Heads above 128 do
 // not fit and run on the CUDA cores.
 //
-// 2047 rows in records of 512, 16 heads of 128, window 200, capped: 70 us, 12 of
+// 2047 rows in records of 512, 16 heads of 128, window 200, capped: 63 us, 12 of
 // them the split (84 MB, HBM bound); one sequence of 2048, no window: 118 us.
 // Q from shared memory bounds the scores' MMAs (64 keys a tile: 6 KB read for 16
 // cycles of products) and the single stages a tile's loads.
