@@ -17,7 +17,9 @@
 // the diagonal and tiles that reach below some row's first key need a mask.
 // P is taken against the maximum of the tiles before the last one: the row's
 // parts then exchange their maxima while P.V runs instead of before it (bf16
-// has FP32's exponents, so a P above 1 loses nothing).  The maximum moves, and O
+// has FP32's exponents, so a P above 1 loses nothing).  The first tile's maximum
+// is exchanged before its P, and so are the next ones' while some row has met no
+// score above -inf.  The maximum moves, and O
 // is rescaled, only when it grows by more than 2^8.  A row whose scores jump by
 // more than 2^127 from one tile to the next comes out infinite, and is computed
 // again like one that came out NaN.  32 keys that every row of a warp masks
@@ -432,6 +434,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // tiles before the last; l: this part's sum; last: this part's maximum of the last tile
     float m = -INFINITY, l = 0.f, last = -INFINITY;
     const int t_own = (k_end - 1 - w_last) / BK;  // the tile with the warp's own rows' keys: the first it sees
+    int t_exact = n;  // the last tile whose maximum was exchanged before its P (none yet)
     bool ok = true;
     // A failed wait sets `fail`; the two warps of a row leave together, by their
     // next exchange barrier, and the others by their own waits.
@@ -477,45 +480,50 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           }
         }
       }
-      if (t == t_own) {
-        // the rows' first keys: the parts agree on their maximum at once
-        row_max();
-        xbuf[((t & 1) * NP + part) * 128 + r] = mt;
-        if (bar_red_or(4 + q4, 32 * NP, fail)) {
-          ok = false;
-          break;
-        }
-        m = fmaxf(mt, xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r]);
-      } else if (t > t_own + 1) {
-        // later the maximum of the tile before: this one's P may be large
-        if (bar_red_or(4 + q4, 32 * NP, fail)) {
-          ok = false;
-          break;
-        }
-        const float mn = fmaxf(fmaxf(m, last), xbuf[(((t - 1) & 1) * NP + (part ^ 1)) * 128 + r]);
-        // the parts of a row see the same m and mn, so they decide alike
-        if (__any_sync(0xffffffffu, mn > m + 8.f)) {
-          // O must hold P_{t-1} V_{t-1} before it is rescaled.
-          const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
-          __syncwarp();
-          if (!__all_sync(0xffffffffu, done)) {
-            fail = true;
-            continue;
-          }
-          tc_fence_after();
-          const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
-          m = mn;
-          l = corr == 0.f ? 0.f : l * corr;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
+      // O and l against a new maximum; false: a wait failed
+      auto rescale = [&](float mn) -> bool {
+        const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+        m = mn;  // also where the wait fails: the parts of a row go on deciding alike
+        // O must hold P_{t-1} V_{t-1} before it is rescaled.
+        const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, done)) return false;
+        tc_fence_after();
+        l = corr == 0.f ? 0.f : l * corr;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
 #pragma unroll 1
-          for (int c = part * DP; c < (part + 1) * DP; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
-            tmem_wait_ld();
+        for (int c = part * DP; c < (part + 1) * DP; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
-          }
-          tmem_wait_st();
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
+        }
+        tmem_wait_st();
+        return true;
+      };
+      // t_exact + 1 follows tiles whose maxima m holds.  A row that has met no score
+      // above -inf has no m to take this tile's P against: its warp exchanges again.
+      const bool exact = t == t_own || (t == t_exact + 1 && __any_sync(0xffffffffu, live && m == -INFINITY));
+      if (exact || t > t_exact + 1) {
+        if (exact) {
+          row_max();
+          xbuf[((t & 1) * NP + part) * 128 + r] = mt;
+        }
+        if (bar_red_or(4 + q4, 32 * NP, fail)) {
+          ok = false;
+          break;
+        }
+        // otherwise the maximum of the tile before: this one's P may be large
+        const float mn = exact ? fmaxf(fmaxf(m, mt), xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r])
+                               : fmaxf(fmaxf(m, last), xbuf[(((t - 1) & 1) * NP + (part ^ 1)) * 128 + r]);
+        if (exact) t_exact = t;
+        // the parts of a row see the same m and mn, so they decide alike
+        if (t == t_own) {
+          m = mn;  // the rows' first keys: O holds nothing yet
+        } else if (__any_sync(0xffffffffu, mn > m + 8.f) && !rescale(mn)) {
+          fail = true;
+          continue;
         }
       }
       // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
@@ -546,7 +554,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       mbar_arrive(&pfull[s]);
       const float2 sum = unpair2(add2(ps[0], ps[1]));
       l += sum.x + sum.y;
-      if (t > t_own) {  // for the next tile, while P.V runs
+      if (t > t_exact) {  // for the next tile, while P.V runs
         row_max();
         last = mt;
         xbuf[((t & 1) * NP + part) * 128 + r] = mt;

@@ -413,6 +413,44 @@ def test_attention_packed_scores_of_minus_infinity(dtype, d):
         assert ((out[a:b].double() - y).abs() <= tol + U[dtype] * y.abs()).all()
 
 
+def attention_of_seen_keys(q, k, v, seen, rounded_p):
+    """(expected [rows, heads, d], tolerance before the store) of one sequence whose row i sees the keys seen[i], in 64 bits."""
+    import torch
+
+    hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
+    qs, ks, vs = q.double().transpose(0, 1), *(x.double().transpose(0, 1).repeat_interleave(hq // hkv, 0) for x in (k, v))
+    p = torch.softmax((qs @ ks.transpose(1, 2) / d**0.5).masked_fill(~seen, float("-inf")), -1)
+    e = (d + 8) * U32 * (qs.abs() @ ks.abs().transpose(1, 2)) / d**0.5
+    e = torch.where(seen, e, 0).amax(-1, keepdim=True)
+    tol = (4 * e + (2.0**-8 if rounded_p else 0) + (q.shape[0] + 16) * U32 + 2.0**-21) * (p @ vs.abs())
+    return (p @ vs).transpose(0, 1), tol.transpose(0, 1)
+
+
+@pytest.mark.parametrize("low", [False, True])
+@pytest.mark.parametrize("n,blocked", [(560, slice(300, None)), (560, slice(128, None, 128)), (560, slice(64, None, 64)), (128, slice(64, None)),
+                                       (256, slice(128, None))])
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 128), ("fp32", 256)])
+def test_attention_packed_own_keys_of_minus_infinity(dtype, d, n, blocked, low):
+    """Rows whose nearest keys (their own among them) score -inf answer from the keys before those.
+    low: those score -87, near the end of FP32's exponents below 0."""
+    import torch
+
+    g = generator(25)
+    q, k, v, out = (normal(g, n, h, d, dtype=dtype) for h in (2, 1, 1, 2))
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    if low:
+        q[:, :, 2:].mul_(4)  # scores a few nats apart
+        q[:, :, 1], k[:, :, 1] = 16, -87 * d**0.5 / 16
+    i = torch.arange(n, device="cuda")
+    seen = i[:, None] >= i
+    seen[:, blocked] = False
+    y, tol = attention_of_seen_keys(q, k, v, seen, dtype == "bf16")
+    k[blocked, :, 0] = float("-inf")
+    run_attention(q, k, v, None, out, torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    off = (out.double() - y).abs() / (tol + U[dtype] * y.abs() + 1e-30)
+    assert off.max() <= 1, (off.max().item(), off.isnan().sum().item(), (off.amax((1, 2)) > 1).nonzero()[:, 0].tolist())
+
+
 @pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
 def test_attention_packed_a_prompt_gone_nan(dtype, d):
     """All of the middle sequence is NaN; its neighbours keep their values."""
