@@ -19,11 +19,11 @@
 // parts then exchange their maxima while P.V runs instead of before it (bf16
 // has FP32's exponents, so a P above 1 loses nothing).  The first tile's maximum
 // is exchanged before its P, and so are the next ones' while some row has met no
-// score above -inf.  The maximum moves, and O
-// is rescaled, only when it grows by more than 2^8.  A row whose scores jump by
-// more than 2^127 from one tile to the next comes out infinite, and is computed
-// again like one that came out NaN.  32 keys that every row of a warp masks
-// leave P = 0 and nothing else.
+// score above -inf.  The maximum moves, and O is rescaled, only when it grows
+// by more than 2^8.  Where scores jump from one tile to the next by so much that
+// P, a sum or an O leaves FP32's range (2^128), the row comes out infinite or NaN
+// and is computed again like any that came out NaN.  32 keys that every row of a
+// warp masks leave P = 0 and nothing else.
 //
 // D = 256: 128-key tiles, one CTA an SM (Q, K and V stages fill shared memory,
 // two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs
@@ -482,21 +482,23 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       }
       // O and l against a new maximum; false: a wait failed
       auto rescale = [&](float mn) -> bool {
-        const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+        // 2^(m - mn) in two steps: P_{t-1} may hold up to 2^128, whose inverse is no normal
+        // number.  A P or a sum that overflowed stays infinite or becomes NaN.
+        const float root = mn == -INFINITY ? 1.f : ex2_approx(0.5f * (m - mn));
         m = mn;  // also where the wait fails: the parts of a row go on deciding alike
         // O must hold P_{t-1} V_{t-1} before it is rescaled.
         const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
         __syncwarp();
         if (!__all_sync(0xffffffffu, done)) return false;
         tc_fence_after();
-        l = corr == 0.f ? 0.f : l * corr;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
+        l = root == 0.f ? 0.f : l * root * root;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
 #pragma unroll 1
         for (int c = part * DP; c < (part + 1) * DP; c += 16) {
           uint32_t o[16];
           tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * root * root);
           tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
         }
         tmem_wait_st();

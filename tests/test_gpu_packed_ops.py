@@ -451,6 +451,23 @@ def test_attention_packed_own_keys_of_minus_infinity(dtype, d, n, blocked, low):
     assert off.max() <= 1, (off.max().item(), off.isnan().sum().item(), (off.amax((1, 2)) > 1).nonzero()[:, 0].tolist())
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 128), ("fp32", 256)])
+def test_attention_packed_scores_that_jump_by_the_range_of_the_exponent(dtype, d):
+    """One key's score is 84 to 92 above those of the keys between it and the row, 2^121 to 2^133 in weight,
+    and keys before it score a little more than those: a finite weight whose inverse FP32 does not hold."""
+
+    def spoil(bounds, q, k, v):
+        import torch
+
+        q.mul_(0.3), k.mul_(0.3)
+        q[:, :, 0], k[:, :, 0] = 16, 0
+        k[:64, :, 0] = 6 * d**0.5 / 16
+        k[200, :, 0] = (84 + 0.5 * torch.arange(16, device="cuda")) * d**0.5 / 16
+        return ()
+
+    check_attention([512], 16, 16, d, dtype, layout="split", gate=False, spoil=spoil)
+
+
 @pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
 def test_attention_packed_a_prompt_gone_nan(dtype, d):
     """All of the middle sequence is NaN; its neighbours keep their values."""
