@@ -225,6 +225,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   return true;
 }
 
+// A CTA that gives up may have copies in flight that no barrier of its own will
+// report: they get a millisecond to land in shared memory before it exits.
+__device__ __forceinline__ void let_copies_land() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 2000000LL) {
+  }
+}
+
 // ---------------------------------------------------------------------------
 // TMA (no multicast anywhere in this library)
 // ---------------------------------------------------------------------------

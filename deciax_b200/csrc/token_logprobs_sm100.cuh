@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(192, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncthreads();
+  if (PAIR && *abort_flag) let_copies_land();  // their barriers lie with the leader, and wait for both CTAs
   if constexpr (PAIR) cluster_sync_all();  // no CTA frees TMEM while its pair may still use it
   tc_fence_after();
   if (warp == 1) {
@@ -584,6 +585,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) let_copies_land();  // their barriers wait for the splitting warps too
   tc_fence_after();
   if (warp == 16) tmem_dealloc(tmem_base, S::TMEM_COLS);
 }
