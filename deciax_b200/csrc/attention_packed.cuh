@@ -137,6 +137,15 @@ __device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h,
   __syncthreads();
 }
 
+// Rows of a tile whose kernel gave up on a wait: NaN, whatever the kernel has
+// stored there.  Every thread of the block must call it.
+template <typename T, int NT>
+__device__ __noinline__ void attn_packed_give_up(const AttnPackedArgs<T>& a, int h, int q_first, int q_end) {
+  const long long n = static_cast<long long>(q_end - q_first) * a.d;
+  for (long long i = threadIdx.x; i < n; i += NT)
+    a.out[(q_first + i / a.d) * a.ldo + h * a.hso + i % a.d] = from_f32<T>(__int_as_float(0x7fffffff));
+}
+
 template <int DP>
 struct AttnPackedSimtShape {
   static constexpr int BQ = 64, BK = 64, LD = DP + 4, LDP = BK + 4;

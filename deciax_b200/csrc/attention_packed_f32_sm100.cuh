@@ -376,7 +376,9 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
     float* lbuf = xbuf + 512;
     lbuf[part * 128 + r] = l;
     const bool fin = ok && mbar_wait(ofinal, 0, a.status, kTimeoutAttention);
-    if (!bar_red_or(1, NT, !fin)) {  // every softmax warp agrees
+    const bool out_ok = !bar_red_or(1, NT, !fin);  // every softmax warp agrees
+    if (!out_ok) *abort_flag = 1;
+    if (out_ok) {
       l = lbuf[r] + lbuf[128 + r];
       tc_fence_after();
       // The row goes through the Q parts (free: every MMA has completed), 16-byte
@@ -434,7 +436,10 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, Sh::TMEM_COLS);
-  if (*abort_flag) return;
+  if (*abort_flag) {
+    attn_packed_give_up<float, Sh::THREADS>(a, h, q_first, q_end);
+    return;
+  }
   for (int w = 0; w < 4; ++w)
     for (uint32_t rows = s_nan[w]; rows; rows &= rows - 1) {
       const int row = q0 + w * 32 + __ffs(static_cast<int>(rows)) - 1;

@@ -599,6 +599,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // end, and rows outside the sequences stay as they were.
     const bool whole = q_first == q0 && q_end == q0 + BQ;
     const bool out_ok = !bar_red_or(1, NT, !(fin && (have_gate || !a.gate)));  // every softmax warp agrees
+    if (!out_ok) *abort_flag = 1;
     if (out_ok) {
       tc_fence_after();
       auto store_atom = [&](int at) {
@@ -681,7 +682,12 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, Sh::TMEM_COLS);
-  if (*abort_flag) return;
+  if (*abort_flag) {
+    tma_store_wait_all();  // of the threads that stored
+    __syncthreads();
+    attn_packed_give_up<__nv_bfloat16, Sh::THREADS>(a, h, q_first, q_end);
+    return;
+  }
   for (int w = 0; w < 4; ++w)
     for (uint32_t rows = s_nan[w]; rows; rows &= rows - 1) {
       const int row = q0 + w * 32 + __ffs(static_cast<int>(rows)) - 1;

@@ -240,6 +240,15 @@ __device__ __forceinline__ void store_state(const LogprobArgs& a, const RowState
   list.store(a.top, a.list_x + at * a.top, a.list_id + at * a.top);
 }
 
+// In place of a state that a failed wait left out: the row's sums become NaN
+// (scratch may hold an earlier call's).
+__device__ __forceinline__ void store_no_state(const LogprobArgs& a, int split, int row) {
+  const size_t at = static_cast<size_t>(row) * a.splits + split;
+  const float nan = __int_as_float(0x7fffffff);
+  a.part[at] = make_float4(nan, nan, nan, 0.f);
+  for (int j = 0; j < a.top; ++j) a.list_id[at * a.top + j] = -1;
+}
+
 // ---------------------------------------------------------------------------
 // CUDA cores: 128 x 128 tiles, 8 x 8 a thread, FP32 products and sums
 // ---------------------------------------------------------------------------

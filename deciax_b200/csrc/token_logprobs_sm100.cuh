@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(192, 1)
     const int copies = PAIR ? 1 : args.copies, rows_seen = 128 / copies;
     const int share = r / rows_seen;
     const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
-    int local = 0;
+    int local = 0, done = worker;  // done: the first unit without a state
     bool ok = true;
     for (int unit = worker; ok && unit < units; unit += workers) {
       const int m = unit % args.num_m, split = unit / args.num_m;
@@ -289,7 +289,12 @@ __global__ void __launch_bounds__(192, 1)
         }
       }
       if (ok && share == 0 && row < args.rows) store_state(args, st, list, split, row);
+      if (ok) done += workers;
       if (!PAIR && copies > 1) asm volatile("bar.sync 1, 128;" ::: "memory");  // the lists may be cleared
+    }
+    for (; done < units; done += workers) {  // a wait failed
+      const int row = done % args.num_m * BM + static_cast<int>(rank) * 128 + r;
+      if (share == 0 && row < args.rows) store_no_state(args, done / args.num_m, row);
     }
   }
 
@@ -538,7 +543,7 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
     if (!ok) *abort_flag = 1;
   } else {
     const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter; row of the tile
-    int local = 0;
+    int local = 0, done = blockIdx.x;  // done: the first unit without a state
     bool ok = true;
     for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
       const int split = unit / args.num_m, row = unit % args.num_m * BM + r;
@@ -579,6 +584,11 @@ __global__ void __launch_bounds__(LogprobF32Shape::THREADS, 1)
         if (lane == 0) mbar_arrive(&tempty[acc]);
       }
       if (ok && row < args.rows) store_state(args, st, list, split, row);
+      if (ok) done += gridDim.x;
+    }
+    for (; done < units; done += gridDim.x) {  // a wait failed
+      const int row = done % args.num_m * BM + r;
+      if (row < args.rows) store_no_state(args, done / args.num_m, row);
     }
   }
 

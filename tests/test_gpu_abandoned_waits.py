@@ -2,7 +2,8 @@
 
 tests/abandoned_waits.cu launches them with tensor maps that deliver fewer bytes
 than a wait counts on.  Each wait then ends after its own limit (about two
-seconds), and the kernel returns: the context stays usable."""
+seconds), and the kernel returns: the context stays usable, and the rows that it
+could not compute are NaN."""
 
 from __future__ import annotations
 
@@ -73,3 +74,19 @@ def test_abandoned_kernels_return_and_the_context_stays_usable(abandoned):
     check_logprobs(ROWS, VOCAB, DIM, "fp32", top=TOP)
     check_attention([TOKENS], 1, 1, 64, "bf16")
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fp32", [0, 1])
+def test_abandoned_scores_are_nan(abandoned, fp32):
+    """Not what the scratch held, in either of the two runs of columns."""
+    logp, entropy, ids, best = abandoned["logprobs", fp32]
+    assert logp.isnan().all() and entropy.isnan().all()
+    assert (ids == -1).all()
+
+
+@pytest.mark.parametrize("which", [1, 2])
+@pytest.mark.parametrize("fp32", [0, 1])
+def test_abandoned_attention_rows_are_nan(abandoned, fp32, which):
+    """Whether the keys or the values are missing; rows of no sequence are left as they were."""
+    out = abandoned["attention", fp32, which]
+    assert out[:TOKENS].isnan().all() and (out[TOKENS:] == 3).all()
