@@ -54,6 +54,12 @@ static void require_on_device(std::initializer_list<const void*> pointers) {
   }
 }
 
+// So does one that reads a value across its type's alignment.
+static void require_aligned(std::initializer_list<const void*> pointers, int bytes) {
+  for (const void* p : pointers)
+    REQUIRE(reinterpret_cast<uintptr_t>(p) % bytes == 0, "an operand is not aligned to its values' size");
+}
+
 // Dynamic shared memory beyond the default is a per-device attribute of a kernel.
 template <typename K>
 static void allow_smem(K kern, size_t bytes) {
@@ -426,7 +432,7 @@ int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const voi
                            int top, int32_t* top_ids, float* top_logprobs, void* stream) {
   using namespace clef;
   return op_guarded([&] {
-    size_of(dtype);
+    const int size = size_of(dtype);
     REQUIRE(rows >= 0 && vocab > 0 && dim > 0, "rows must not be negative, vocab and dim must be positive");
     REQUIRE(vocab <= 1 << 30 && dim <= 1 << 20 && rows <= 1 << 24, "at most 2^24 rows, 2^30 tokens and 2^20 dimensions");
     REQUIRE(ldh >= dim && ldw >= dim, "row strides must be at least dim");
@@ -438,6 +444,10 @@ int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const voi
     REQUIRE(n_targets == 0 || (targets && logprobs), "targets need logprobs");
     REQUIRE(top == 0 || (top_ids && top_logprobs), "top alternatives need their outputs");
     REQUIRE(n_targets > 0 || top > 0 || entropy, "no output was asked for");
+    require_aligned({hidden, lm_head}, size);
+    require_aligned({n_targets ? targets : nullptr, n_targets ? logprobs : nullptr, entropy, top ? top_ids : nullptr,
+                     top ? top_logprobs : nullptr},
+                    4);
     require_on_device({hidden, lm_head, n_targets ? targets : nullptr, n_targets ? logprobs : nullptr, entropy,
                        top ? top_ids : nullptr, top ? top_logprobs : nullptr});
     FinishArgs f{};
@@ -477,7 +487,7 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
                              int d, float softcap, int window, void* stream) {
   using namespace clef;
   return op_guarded([&] {
-    size_of(dtype);
+    const int size = size_of(dtype);
     REQUIRE(n_seqs >= 0 && tokens >= 0, "sequences and tokens must not be negative");
     REQUIRE(tokens <= 65535 * 128, "at most 8388480 tokens");
     REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be a multiple of key/value heads");
@@ -493,6 +503,8 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
     REQUIRE(rows(hq, ldq, hsq) && rows(hkv, ldk, hsk) && rows(hkv, ldv, hsv) && (!gate || rows(hq, ldg, hsg)) &&
                 rows(hq, ldo, hso),
             "token and head strides must be at least head_dim");
+    require_aligned({q, k, v, gate, out}, size);
+    require_aligned({cu_seqlens}, 4);
     require_on_device({q, k, v, gate, out, cu_seqlens});
     auto call = [&](auto* type) {
       using T = std::remove_pointer_t<decltype(type)>;
@@ -528,7 +540,7 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
                               const void* k_norm, float eps, void* stream) {
   using namespace clef;
   return op_guarded([&] {
-    size_of(dtype);
+    const int size = size_of(dtype);
     REQUIRE(tokens >= 0 && hq >= 0 && hkv >= 0 && hq + hkv > 0, "tokens and heads must not be negative");
     REQUIRE(hq <= 65536 && hkv <= 65536, "at most 65536 heads");
     REQUIRE(d > 0 && d <= 2 * kRopeMaxHalf, "head_dim must be in [1, 256]");
@@ -555,6 +567,10 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
             "token and head strides must be at least head_dim");
     REQUIRE(axes == 1 || ldp >= tokens, "the positions' axis stride is below the token count");
     REQUIRE(static_cast<long long>(tokens) * (hq + hkv) < (1LL << 33), "tokens * heads must be below 2^33");
+    require_aligned({hq ? q : nullptr, hq ? q_out : nullptr, hkv ? k : nullptr, hkv ? k_out : nullptr, hq ? q_norm : nullptr,
+                     hkv ? k_norm : nullptr},
+                    size);
+    require_aligned({positions}, 4);
     require_on_device({hq ? q : nullptr, hq ? q_out : nullptr, hkv ? k : nullptr, hkv ? k_out : nullptr, positions,
                        hq ? q_norm : nullptr, hkv ? k_norm : nullptr});
     RopeAxesArgs a{};

@@ -281,9 +281,9 @@ int clef_op_gdn_core(int dtype, const void* proj, int ldp, const void* conv, int
  * Sequences laid end to end instead of padded to a rectangle: positions that
  * are given, attention that stays inside each sequence, and the language
  * head's own answer.  Operands are device memory of the current device
- * (anything else is CLEF_EINVAL); strides count elements; arithmetic is FP32
- * with one rounding to the operand type at each store.  No call synchronises
- * the host.  A wait inside a kernel that runs out (some 2 s: a broken pipeline)
+ * (anything else, or a pointer inside a value, is CLEF_EINVAL); strides count
+ * elements; arithmetic is FP32 with one rounding to the operand type at each
+ * store.  No call synchronises the host.  A wait inside a kernel that runs out (some 2 s: a broken pipeline)
  * does not fail the call, which has returned: the rows that it leaves without a
  * result are NaN (and alternatives may be missing, id -1). */
 

@@ -100,3 +100,25 @@ def test_token_logprobs_refusals(lib, kw):
 
 def test_token_logprobs_without_rows_is_a_no_op(lib):
     assert logprobs(lib, rows=0, hidden=None, head=None) == _lib.CLEF_OK
+
+
+# A kernel that reads a value across its type's alignment faults: such an operand is refused without a look at the device.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("name", ["q", "k", "qo", "ko", "pos", "qw", "kw"])
+def test_rope_axes_refuses_pointers_inside_a_value(lib, name, dtype):
+    off = 2 if name == "pos" or dtype == F32 else 1
+    assert rope(lib, dtype=dtype, **{name: P + off}) == _lib.CLEF_EINVAL
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("name", ["q", "k", "v", "gate", "out", "cu"])
+def test_attention_packed_refuses_pointers_inside_a_value(lib, name, dtype):
+    off = 2 if name == "cu" or dtype == F32 else 1
+    assert attention(lib, dtype=dtype, **{name: P + off}) == _lib.CLEF_EINVAL
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("name", ["hidden", "head", "targets", "logprobs", "entropy", "ids", "top_logprobs"])
+def test_token_logprobs_refuses_pointers_inside_a_value(lib, name, dtype):
+    off = 1 if name in ("hidden", "head") and dtype == BF16 else 2
+    assert logprobs(lib, dtype=dtype, **{name: P + off}) == _lib.CLEF_EINVAL
