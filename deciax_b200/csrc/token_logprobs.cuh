@@ -58,9 +58,16 @@ struct RowState {
   float m = -INFINITY, s = 0.f, t = 0.f;
 };
 
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if one is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The `top` largest scores of a row, entered by a chunk of 32 columns at a time.
 // Ids rise from chunk to chunk, so a score that equals the smallest entry stays
-// out.  Both forms use `area` (shared memory, list_bytes(top) a CTA); r is the
+// out.  A free place holds NaN, which no comparison "at most" admits: any score goes
+// before it, -inf too (a score of NaN goes nowhere).  Both forms use `area` (shared memory, list_bytes(top) a CTA); r is the
 // thread's place in it (0..127).
 //
 // The list lies in registers, largest first, K = 8 or 32 places.  An insertion is
@@ -77,16 +84,16 @@ struct TopList {
   __device__ __forceinline__ void clear(int top) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      v[j] = -INFINITY;
+      v[j] = __int_as_float(0x7fffffff);
       id[j] = -1;
     }
-    thr = top > 0 ? -INFINITY : INFINITY;
+    thr = top > 0 ? v[0] : INFINITY;
   }
   template <bool ANY_ORDER = false>
   __device__ __forceinline__ void insert(float x, int32_t i, int top) {
     bool before[K];  // x goes before entry j
 #pragma unroll
-    for (int j = 0; j < K; ++j) before[j] = x > v[j] || (ANY_ORDER && x == v[j] && i < id[j]);
+    for (int j = 0; j < K; ++j) before[j] = !(x <= v[j]) || (ANY_ORDER && x == v[j] && i < id[j]);
 #pragma unroll
     for (int j = K - 1; j > 0; --j) {
       v[j] = before[j - 1] ? v[j - 1] : before[j] ? x : v[j];
@@ -96,21 +103,22 @@ struct TopList {
     id[0] = before[0] ? i : id[0];
     thr = v[0];
 #pragma unroll
-    for (int j = 1; j < K; ++j) thr = j < top ? fminf(thr, v[j]) : thr;  // entry top - 1
+    for (int j = 1; j < K; ++j) thr = j < top ? min_nan(thr, v[j]) : thr;  // entry top - 1
   }
-  // best = the largest of x; entries that do not count are -inf
-  __device__ __forceinline__ void take(float (&x)[32], float best, int col, int top, float* area, int r) {
-    if (!(best > thr)) return;
+  // best = the largest of x, of which the first `valid` count
+  __device__ __forceinline__ void take(float (&x)[32], float best, int col, int valid, int top, float* area, int r) {
+    if (best <= thr) return;
     uint32_t mask[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int c = 0; c < 32; ++c) {
-      if (x[c] > thr) mask[c & 3] |= 1u << c;
+      if (!(x[c] <= thr)) mask[c & 3] |= 1u << c;
       area[c * 128 + r] = x[c];
     }
-    for (uint32_t left = (mask[0] | mask[1]) | (mask[2] | mask[3]); left; left &= left - 1) {
+    const uint32_t exist = valid < 32 ? (1u << valid) - 1 : ~0u;
+    for (uint32_t left = ((mask[0] | mask[1]) | (mask[2] | mask[3])) & exist; left; left &= left - 1) {
       const int c = __ffs(static_cast<int>(left)) - 1;
       const float y = area[c * 128 + r];
-      if (y > thr) insert(y, col + c, top);
+      if (!(y <= thr) && y == y) insert(y, col + c, top);
     }
   }
   __device__ __forceinline__ void publish(float* area, int r) const {
@@ -168,7 +176,8 @@ __device__ __forceinline__ void scan32(RowState& st, TopList<K>& list, float (&x
     st.s *= f;
     st.m = zmax;
   }
-  const float neg_m = -st.m;
+  const float neg_m = st.m == -INFINITY ? 0.f : -st.m;  // no score above -inf yet: exp2(-inf) = 0
+  bool done = false;
   if (valid >= 32) {  // two columns at a time
     const uint64_t log2e2 = pair2(LOG2E, LOG2E), neg_m2 = pair2(neg_m, neg_m);
     uint64_t ps[2] = {0ull, 0ull}, pt[2] = {0ull, 0ull};
@@ -204,9 +213,14 @@ __device__ __forceinline__ void scan32(RowState& st, TopList<K>& list, float (&x
       for (int e = 0; e < 16; ++e) add(e, pair2(x[2 * e], x[2 * e + 1]));
     }
     const float2 s2 = unpair2(add2(ps[0], ps[1])), t2 = unpair2(add2(pt[0], pt[1]));
-    st.s += s2.x + s2.y;
-    st.t += t2.x + t2.y;
-  } else {
+    const float t = t2.x + t2.y;
+    if (t == t) {
+      st.s += s2.x + s2.y;
+      st.t += t;
+      done = true;
+    }
+  }
+  if (!done) {  // few columns, or one of them scores -inf (whose product of 0 and -inf is NaN), +inf or NaN
     float ps = 0.f, pt = 0.f;
 #pragma unroll
     for (int c = 0; c < 32; ++c)
@@ -214,17 +228,23 @@ __device__ __forceinline__ void scan32(RowState& st, TopList<K>& list, float (&x
         const float d = fmaf(capped<CAP>(x[c], softcap), LOG2E, neg_m);
         const float e = ex2_approx(d);
         ps += e;
-        pt = fmaf(d, e, pt);
+        pt = e == 0.f ? pt : fmaf(d, e, pt);
       }
     st.s += ps;
     st.t += pt;
   }
-  list.take(x, best, col, top, area, r);
+  list.take(x, best, col, valid, top, area, r);
 }
 
-// Joins another state into this one.  A side without columns has m = -inf, s = t = 0: it weighs nothing.
+// Joins another state into this one.  A side without columns, or whose columns all score -inf, has m = -inf,
+// s = t = 0: it weighs nothing.
 __device__ __forceinline__ void join_state(RowState& st, float m, float s, float t) {
   const float mx = fmaxf(st.m, m);
+  if (mx == -INFINITY) {  // NaN sums stay
+    st.s += s;
+    st.t += t;
+    return;
+  }
   const float d0 = st.m - mx, d1 = m - mx, w0 = exp2f(d0), w1 = exp2f(d1);
   st.t = (w0 == 0.f ? 0.f : w0 * fmaf(d0, st.s, st.t)) + (w1 == 0.f ? 0.f : w1 * fmaf(d1, s, t));
   st.s = w0 * st.s + w1 * s;

@@ -346,11 +346,14 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
  * vocab or more gives NaN.  top_ids / top_logprobs [rows, top]: the `top` largest
  * x, largest first, equal ones by the lowest id (top <= 32).  Products and sums
  * are FP32 and x is not rounded.  n_targets = 0, entropy = NULL and top = 0 leave
- * an output out; rows = 0 does nothing.  A row with a NaN logit has NaN logprobs
- * and entropy; one with an infinite logit has NaN entropy, and its logprobs may be
- * NaN.  16-byte aligned rows (pointers, ldh and ldw, whole 16 bytes of
- * dim) run on the tensor cores, FP32 values as three bf16 parts each (what is left
- * out of a product is below 2^-24 of it).  Scratch comes from the library's stream-ordered
+ * an output out; rows = 0 does nothing.  A z of -inf weighs nothing, and its token is an
+ * alternative like any other.  A row with a NaN logit has NaN logprobs and entropy
+ * (and so has one whose largest z is infinite); a token whose logit is NaN is no
+ * alternative: ids behind the last one are -1, their top_logprobs -inf.  16-byte
+ * aligned rows (pointers, ldh and ldw, whole 16 bytes of dim) run on the tensor
+ * cores, FP32 values as three bf16 parts each (what is left out of a product is
+ * below 2^-24 of it, and an infinite value makes its logits NaN); their sums cut
+ * off what lies below the accumulator's last place.  Scratch comes from the library's stream-ordered
  * pool: make one call on each device before capturing one into a graph. */
 int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const void* lm_head, int64_t ldw, int rows, int vocab,
                            int dim, float softcap, const int32_t* targets, int n_targets, float* logprobs, float* entropy,

@@ -729,6 +729,70 @@ def test_token_logprobs_nan_rows_stay_alone(n, dtype):
         assert torch.equal(got[keep], want[keep])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 60, 200])
+@pytest.mark.parametrize("top", [4, 20, 32])
+@pytest.mark.parametrize("finite", [(), (5,), (33, 34, 700, 899), tuple(range(0, 900, 37))])
+def test_token_logprobs_tokens_of_minus_infinity_are_alternatives_too(finite, top, n, dtype):
+    """All tokens but a few score -inf: products of 3e38 and -3e38 that FP32 does not hold.  They follow the finite
+    ones as alternatives, the lowest ids first, with log probabilities of -inf; a row without any finite score has no sum."""
+    import torch
+
+    hidden, head = grid_operands(generator(13), n, 900, 64, dtype)
+    hidden[:, 0] = 2.0**127
+    low = torch.ones(900, dtype=torch.bool, device="cuda")
+    low[list(finite)] = False
+    head[:, 0] = torch.where(low, -(2.0**127), 0.0)
+    targets = torch.tensor([[5, 6]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    logp, ent, ids, best = run_logprobs(hidden, head, targets, top)
+    assert (ent.isfinite() if finite else ent.isnan()).all()
+    h, w = hidden.double(), head.double()
+    h[:, 0] = 0
+    raw = (h @ w.T).masked_fill(low, float("-inf"))
+    order = torch.sort(raw, dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(ids.long(), order)
+    if finite:
+        want = raw - torch.logsumexp(raw, 1, keepdim=True)
+        # the finite scores are exact: the relative error of the sum, and a few roundings of the results
+        tol = (900 / 32 + 64) * U32 + 2.0**-20 + 8 * U32 * (raw[:, ~low].abs().amax() + 10)
+        for got, at in ((logp, targets.long()), (best, order)):
+            expected = want.gather(1, at)
+            assert torch.equal(got == float("-inf"), expected == float("-inf"))
+            assert ((got.double() - expected).abs().nan_to_num(0) <= tol).all()
+        p = want.exp()
+        z = (raw - raw.amax(1, keepdim=True)).masked_fill(low, 0.0)
+        assert ((ent.double() + (p * want.masked_fill(low, 0.0)).sum(1)).abs() <= 4 * tol * ((p * z.abs()).sum(1) + 1)).all()
+    else:
+        assert logp.isnan().all() and best.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("n", [3, 200])
+def test_token_logprobs_a_token_of_infinity_comes_first(n, softcap, dtype):
+    """Without a cap it leaves no sum; under one it scores the cap, and one of -inf its negative."""
+    import torch
+
+    hidden, head = grid_operands(generator(14), n, 900, 64, dtype)
+    hidden[:, 0], head[:, 0] = 2.0**127, 0
+    head[700, 0], head[3, 0] = 2.0**127, -(2.0**127)
+    targets = torch.tensor([[700, 3]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    logp, ent, ids, best = run_logprobs(hidden, head, targets, 3, softcap)
+    assert (ids[:, 0] == 700).all() and (ids != 3).all()
+    if not softcap:
+        assert logp.isnan().all() and ent.isnan().all() and best.isnan().all()
+        return
+    h = hidden.double()
+    h[:, 0] = 0
+    z = softcap * torch.tanh(h @ head.double().T / softcap)
+    z[:, 700], z[:, 3] = softcap, -softcap
+    want = torch.log_softmax(z, 1)
+    tol = (900 / 32 + 64) * U32 + 2.0**-20 + 8 * U32 * (softcap + 10)
+    assert ((logp.double() - want[:, [700, 3]]).abs() <= tol).all() and ((best.double() - torch.topk(want, 3, 1).values).abs() <= tol).all()
+    away = (want.exp() * (z - z.amax(1, keepdim=True)).abs()).sum(1)
+    assert ((ent.double() + (want.exp() * want).sum(1)).abs() <= 4 * tol * (away + 1)).all()
+
+
 def test_token_logprobs_captured_and_replayed():
     import torch
 
