@@ -17,8 +17,13 @@
 // a tile's exponentials use the maximum of the tiles before, or an infinity) is
 // therefore computed once more from its own keys alone (attn_packed_redo), so
 // that what a sequence holds never reaches another.  A row whose own scores
-// hold a NaN is NaN whatever else it sees and is left as it came out: a prompt
-// gone NaN costs no second pass.
+// hold a NaN is NaN whatever else it sees: in BF16, and on the CUDA cores, it is
+// left as it came out, and FP32 on the tensor cores, where infinite operands come
+// out NaN too, ends the second pass at the first NaN score (4096 rows of NaN, 16
+// heads of 128: 624 us against 390 of numbers).  Costly is an infinite value among
+// the row's own: one at the start of 4096 rows makes all of them run twice, 11 ms
+// at 16 heads of 256 in BF16 against 0.13, 11 ms at 128 in FP32 against 0.39 (18 ms
+// at 128 in BF16).
 //
 // attn_packed_simt_kernel (here): FP32 products on the CUDA cores, any head
 // size to 256, any strides and alignment: bf16 rows that TMA cannot read, FP32
@@ -80,61 +85,90 @@ __device__ __forceinline__ float packed_score(float x, float scale, float softca
   return inv_cap > 0.f ? softcap * tanh_flat(x * inv_cap) : x;
 }
 
-// One row again from its own keys [lo, row] alone, by the whole block (NT
-// threads, d <= NT): chunks of NT keys, a key a thread for the scores, an
-// element a thread for P.V.  smem: 256 + 2 * NT floats.  For rows that came
-// out infinite or NaN; every thread of the block must call it.
-template <typename T, int NT>
-__device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int row, int lo, float* smem) {
-  float* sq = smem;            // [d]
-  float* sp = smem + 256;      // [NT]
-  float* red = smem + 256 + NT;  // [NT]
-  const int tid = threadIdx.x, hk = h / (a.H / a.Hk);
-  const T* q = a.q + row * a.ldq + h * a.hsq;
-  const T* k = a.k + hk * a.hsk;
-  const T* v = a.v + hk * a.hsv;
+// One row again from its own keys [lo, row] alone, by a warp: a lane holds eight
+// elements of every row it reads.  Four keys' partial products are summed over the
+// lanes at once, by halves: after the first two exchanges a lane holds the sum
+// of four lanes for one of the keys, `mine` below; after five of 32.  Eight such
+// groups give every lane the score of one of 32 keys.  VEC: rows by 16-byte loads.
+template <typename T, bool VEC>
+__device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, int h, int row, int lo) {
+  const int lane = threadIdx.x & 31, c = lane * 8, hk = h / (a.H / a.Hk);
+  const int mine = (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
+  const T* k = a.k + hk * a.hsk + lo * a.ldk;
+  const T* v = a.v + hk * a.hsv + lo * a.ldv;
+  T* out = a.out + row * a.ldo + h * a.hso;
   const float scale = rsqrtf(static_cast<float>(a.d)), inv_cap = inverse_cap(a.softcap);
-  for (int c = tid; c < a.d; c += NT) sq[c] = to_f32(q[c]);
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int k0 = lo; k0 <= row; k0 += NT) {
-    const int n = min(NT, row + 1 - k0);
-    __syncthreads();  // sq is staged; the last chunk's sp has been read
-    float x = -INFINITY;
-    if (tid < n) {
-      const T* kr = k + (k0 + tid) * a.ldk;
-      float s = 0.f;
-      for (int c = 0; c < a.d; ++c) s = fmaf(sq[c], to_f32(kr[c]), s);
-      x = packed_score(s, scale, a.softcap, inv_cap);
+  float q[8], o[8] = {};
+  load8<T, VEC>(a.q + row * a.ldq + h * a.hsq, c, a.d, true, q);
+  float m = -INFINITY, l = 0.f;
+  for (int left = row + 1 - lo; left > 0; left -= 32) {
+    const int groups = min(8, (left + 3) / 4);
+    float x = 0.f;
+#pragma unroll 1
+    for (int g = 0; g < groups; ++g) {
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j, k += a.ldk) {
+        float e[8];
+        load8<T, VEC>(k, c, a.d, 4 * g + j < left, e);
+        s[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[j] = fmaf(q[i], e[i], s[j]);
+      }
+#pragma unroll
+      for (int half = 2; half > 0; half /= 2) {
+        const bool upper = lane & 8 * half;
+#pragma unroll
+        for (int j = 0; j < half; ++j) {
+          const float other = __shfl_xor_sync(0xffffffffu, upper ? s[j] : s[j + half], 8 * half);
+          s[j] = (upper ? s[j + half] : s[j]) + other;
+        }
+      }
+#pragma unroll
+      for (int w = 4; w > 0; w /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], w);
+      if ((lane & 7) == g) x = s[0];
     }
-    red[tid] = x;
-    if (__syncthreads_or(x != x)) {  // a NaN score: the row is NaN
-      if (tid < a.d) a.out[row * a.ldo + h * a.hso + tid] = from_f32<T>(__int_as_float(0x7fffffff));
+    x = 4 * (lane & 7) + mine < left ? packed_score(x, scale, a.softcap, inv_cap) : -INFINITY;
+    if (__any_sync(0xffffffffu, x != x)) {  // a NaN score: the row is NaN
+      for (int i = lane; i < a.d; i += 32) out[i] = from_f32<T>(__int_as_float(0x7fffffff));
       return;
     }
-    for (int w = NT; w > 1;) {  // NT need not be a power of two
-      const int half = (w + 1) / 2;
-      if (tid + half < w) red[tid] = fmaxf(red[tid], red[tid + half]);
-      w = half;
-      __syncthreads();
-    }
-    const float mn = fmaxf(m, red[0]);
+    const float mn = fmaxf(m, warp_max(x));
     const float corr = m == mn ? 1.f : expf(m - mn);
     m = mn;
-    sp[tid] = x == -INFINITY ? 0.f : expf(x - mn);  // also where no score so far is above -inf
-    __syncthreads();
-    l *= corr;
-    o *= corr;
-    for (int j = 0; j < n; ++j) {
-      l += sp[j];
-      if (tid < a.d) o = fmaf(sp[j], to_f32(v[(k0 + j) * a.ldv + tid]), o);
+    const float p = x == -INFINITY ? 0.f : expf(x - mn);  // also where no score so far is above -inf
+    l = l * corr + warp_sum(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= corr;
+#pragma unroll 1
+    for (int g = 0; g < groups; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j, v += a.ldv) {
+        float e[8];
+        load8<T, VEC>(v, c, a.d, 4 * g + j < left, e);
+        const float pj = __shfl_sync(0xffffffffu, p, 8 * j + g);  // the lane of key 4 g + j
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(pj, e[i], o[i]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < a.d) {
+      float y = o[i] / l;
+      if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + c + i]));
+      out[c + i] = from_f32<T>(y);
     }
-  }
-  if (tid < a.d) {
-    float y = o / l;
-    if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + tid]));
-    a.out[row * a.ldo + h * a.hso + tid] = from_f32<T>(y);
-  }
-  __syncthreads();
+}
+
+// The rows q0 + (bits of `rows`) again, `warps` of the block sharing them.
+template <typename T, bool VEC>
+__device__ __forceinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int q0, unsigned long long rows, int warp,
+                                                 int warps) {
+  for (int turn = 0; rows; rows &= rows - 1, ++turn)
+    if (turn % warps == warp) {
+      const int row = q0 + __ffsll(static_cast<long long>(rows)) - 1;
+      attn_packed_redo_row<T, VEC>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1));
+    }
 }
 
 // Rows of a tile whose kernel gave up on a wait: NaN, whatever the kernel has
@@ -342,10 +376,7 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     if (bad && l[i] == l[i]) atomicOr(&s_nan, 1ULL << (ty * 4 + i));
   }
   __syncthreads();
-  for (unsigned long long rows = s_nan; rows; rows &= rows - 1) {
-    const int r = __ffsll(static_cast<long long>(rows)) - 1;
-    attn_packed_redo<T, 256>(a, h, q0 + r, s_lo[r], simt_smem);
-  }
+  attn_packed_redo<T, false>(a, h, q0, s_nan, tid / 32, 8);
 }
 
 }  // namespace clef

@@ -90,7 +90,7 @@ struct AttnPackedF32Maps {
 template <int D, bool CAP>
 __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
     attn_packed_f32_tc_kernel(const __grid_constant__ AttnPackedF32Maps maps,
-                              const __grid_constant__ AttnPackedArgs<float> a, bool vec) {
+                              const __grid_constant__ AttnPackedArgs<float> a, bool vec, bool vec_in) {
   using Sh = AttnPackedF32Shape<D>;
   constexpr int BQ = Sh::BQ, BK = Sh::BK, ATOMS = Sh::ATOMS;
   constexpr uint32_t IDESC_QK = idesc_bf16_f32(BQ, BK);
@@ -440,11 +440,13 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
     attn_packed_give_up<float, Sh::THREADS>(a, h, q_first, q_end);
     return;
   }
-  for (int w = 0; w < 4; ++w)
-    for (uint32_t rows = s_nan[w]; rows; rows &= rows - 1) {
-      const int row = q0 + w * 32 + __ffs(static_cast<int>(rows)) - 1;
-      attn_packed_redo<float, Sh::THREADS>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1), reinterpret_cast<float*>(sQ));
-    }
+  for (int half = 0; half < 2; ++half) {
+    const unsigned long long rows = s_nan[2 * half] | static_cast<unsigned long long>(s_nan[2 * half + 1]) << 32;
+    if (vec_in)
+      attn_packed_redo<float, true>(a, h, q0 + 64 * half, rows, warp, Sh::THREADS / 32);
+    else
+      attn_packed_redo<float, false>(a, h, q0 + 64 * half, rows, warp, Sh::THREADS / 32);
+  }
 }
 
 }  // namespace clef

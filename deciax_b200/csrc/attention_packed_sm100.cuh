@@ -688,12 +688,10 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     attn_packed_give_up<__nv_bfloat16, Sh::THREADS>(a, h, q_first, q_end);
     return;
   }
-  for (int w = 0; w < 4; ++w)
-    for (uint32_t rows = s_nan[w]; rows; rows &= rows - 1) {
-      const int row = q0 + w * 32 + __ffs(static_cast<int>(rows)) - 1;
-      attn_packed_redo<__nv_bfloat16, Sh::THREADS>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1),
-                                                   reinterpret_cast<float*>(sQ));
-    }
+  for (int half = 0; half < 2; ++half)
+    attn_packed_redo<__nv_bfloat16, true>(a, h, q0 + 64 * half,
+                                          s_nan[2 * half] | static_cast<unsigned long long>(s_nan[2 * half + 1]) << 32, warp,
+                                          Sh::THREADS / 32);
 }
 
 }  // namespace clef

@@ -237,7 +237,7 @@ static void launch_packed_f32_tc(const AttnPackedArgs<float>& a, cudaStream_t st
   cfg.stream = st;
   cfg.attrs = early;
   cfg.numAttrs = 1;
-  CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_packed_f32_tc_kernel<D, CAP>, maps, a, vec));
+  CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_packed_f32_tc_kernel<D, CAP>, maps, a, vec, sp.vec));
 }
 
 template <typename T>

@@ -281,28 +281,6 @@ constexpr size_t logprob_simt_smem(int top) {
   return (2 * 16 * 132 + 128 * kLogprobSimtLdc) * sizeof(float) + list_bytes(top);
 }
 
-// Elements k .. k + 7 of a row (zeros past its end); VEC: by 16-byte loads.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int k, int dim, bool live, float (&v)[8]) {
-  if constexpr (VEC && sizeof(T) == 4) {
-    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 a = live && k < dim ? *reinterpret_cast<const float4*>(p + k) : z;
-    const float4 b = live && k + 4 < dim ? *reinterpret_cast<const float4*>(p + k + 4) : z;
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else if constexpr (VEC) {
-    const uint4 u = live && k < dim ? *reinterpret_cast<const uint4*>(p + k) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = live && k + j < dim ? to_f32(p[k + j]) : 0.f;
-  }
-}
-
 template <typename T, bool CAP, int K>
 __global__ void __launch_bounds__(256) token_logprobs_simt_kernel(const __grid_constant__ LogprobArgs a) {
   extern __shared__ __align__(16) float lp_smem[];

@@ -322,8 +322,9 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
  * window > 0 keeps the last `window` keys.  tokens = rows of the buffers: rows
  * outside [cu_seqlens[0], cu_seqlens[n_seqs]) belong to no sequence, are not
  * read as keys, may hold anything, and their out is left as it was.  Infinities
- * and NaN of one sequence never reach another.  out must not overlap the
- * inputs.  d <= 256, tokens <= 8388480; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
+ * and NaN of one sequence never reach another; the rows that see an infinite one
+ * of their own are computed twice, the second time slowly.  out must not overlap
+ * the inputs, nor its rows one another.  d <= 256, tokens <= 8388480; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
  * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; FP32 with d <= 128
  * and more than a few tokens also, every value as three bf16 parts (what is left out of a
  * product is below 2^-24 of it; values below 2^-110 keep fewer bits); anything

@@ -97,7 +97,7 @@ int abandoned_attention(int fp32, int which, const void* q, const void* k, const
       using Sh = AttnPackedF32Shape<64>;
       auto kern = attn_packed_f32_tc_kernel<64, false>;
       CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sh::SMEM)));
-      kern<<<dim3(1, (tokens + 127) / 128), Sh::THREADS, Sh::SMEM, st>>>(maps, a, true);
+      kern<<<dim3(1, (tokens + 127) / 128), Sh::THREADS, Sh::SMEM, st>>>(maps, a, true, true);
     } else {
       AttnPackedArgs<__nv_bfloat16> a{};
       fill(a);
