@@ -239,6 +239,26 @@ def test_rope_axes_captured_and_replayed_on_another_stream():
         assert_rope(out, *rope_64(q, w, pos, None, False, 64, 1e4), "bf16")
 
 
+def test_rope_axes_replayed_on_a_stream_of_its_own():
+    """The graph runs behind what its stream holds, not on the stream that captured it."""
+    import torch
+
+    g = generator(28)
+    q, other = normal(g, 4000, 4, 128), normal(g, 4000, 4, 128)
+    out, pos = torch.empty_like(q), torch.arange(4000, device="cuda", dtype=torch.int32)[None].contiguous()
+    w = normal(g, 128, std=0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run_rope(q, None, out, None, pos, None, False, 64, 1e4, w, None)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        q.copy_(other)
+        graph.replay()
+    side.synchronize()
+    assert_rope(out, *rope_64(other, w, pos, None, False, 64, 1e4), "bf16")
+
+
 # --------------------------------------------------------------------------- packed attention
 
 
@@ -602,6 +622,31 @@ def test_attention_packed_rows_do_not_depend_on_their_neighbours():
     torch.cuda.synchronize()
     run_attention(q, k, v, None, outs[2], cu)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("check", [test_attention_packed_infinities_stay_in_their_sequence, test_attention_packed_scores_of_minus_infinity,
+                                   test_attention_packed_a_prompt_gone_nan], ids=lambda f: f.__name__.removeprefix("test_attention_packed_"))
+def test_attention_packed_fp32_heads_of_128_that_are_not_finite(check):
+    check("fp32", 128)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_packed_neighbours_of_any_size(d, dtype):
+    """A sequence keeps its values whatever the rows before and behind it in the same tiles hold."""
+    import torch
+
+    g = generator(27)
+    bounds = [0, 70, 300, 600]
+    q, k, v, gt = (normal(g, 600, h, d, dtype=dtype) for h in (4, 2, 2, 4))
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    y, tol = attention_64(q[70:300], k[70:300], v[70:300], gt[70:300], [0, 230], 0.0, 0, dtype == "bf16")[0, 230]
+    for fill in (0.0, 50.0, -3e38, float("inf"), float("nan")):
+        for x in (q, k, v, gt):
+            x[:70] = x[300:] = fill
+        out = torch.empty_like(q)
+        run_attention(q, k, v, gt, out, cu)
+        assert ((out[70:300].double() - y).abs() <= tol + U[dtype] * y.abs()).all(), fill
 
 
 # --------------------------------------------------------------------------- token log probabilities
