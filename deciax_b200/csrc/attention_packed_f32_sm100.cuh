@@ -136,7 +136,11 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
   int first, total, seq_start = 0;
   packed_extent(a, first, total);
   const int q_end = min(q0 + BQ, total), q_first = max(q0, first);
-  if (q_first >= q_end) return;  // no row of this tile belongs to a sequence
+  if (q_first >= q_end) {  // no row of this tile belongs to a sequence
+    // what follows this kernel counts on the parts being written, even where no tile reads them
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 15; ++i) mbar_init(&bars[i], i == 7 || i == 8 ? 256 : 1);  // pfull: every softmax thread
     *abort_flag = 0;

@@ -624,6 +624,24 @@ def test_attention_packed_rows_do_not_depend_on_their_neighbours():
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_packed_fp32_of_empty_sequences_then_full_ones(d):
+    """A call without a row leaves its scratch whole for the next one, which takes the same memory."""
+    import torch
+
+    g = generator(29)
+    q, k, v = (normal(g, 4000, h, d, dtype="fp32") for h in (4, 2, 2))
+    lengths = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 0, 0], [0, 1500, 4000])]
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    run_attention(q, k, v, None, want, lengths[1])
+    untouched = torch.full_like(q, 7.0)
+    for _ in range(5):
+        run_attention(q.neg(), v, k, None, untouched, lengths[0])
+        run_attention(q, k, v, None, out, lengths[1])
+        assert torch.equal(out, want)
+    assert (untouched == 7).all()
+
+
 @pytest.mark.parametrize("check", [test_attention_packed_infinities_stay_in_their_sequence, test_attention_packed_scores_of_minus_infinity,
                                    test_attention_packed_a_prompt_gone_nan], ids=lambda f: f.__name__.removeprefix("test_attention_packed_"))
 def test_attention_packed_fp32_heads_of_128_that_are_not_finite(check):
