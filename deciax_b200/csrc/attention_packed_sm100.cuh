@@ -17,13 +17,13 @@
 // the diagonal and tiles that reach below some row's first key need a mask.
 // P is taken against the maximum of the tiles before the last one: the row's
 // parts then exchange their maxima while P.V runs instead of before it (bf16
-// has FP32's exponents, so a P above 1 loses nothing).  The first tile's maximum
-// is exchanged before its P, and so are the next ones' while some row has met no
-// score above -inf.  The maximum moves, and O is rescaled, only when it grows
-// by more than 2^8.  Where scores jump from one tile to the next by so much that
-// P, a sum or an O leaves FP32's range (2^128), the row comes out infinite or NaN
-// and is computed again like any that came out NaN.  32 keys that every row of a
-// warp masks leave P = 0 and nothing else.
+// has FP32's exponents, so a P above 1 loses nothing); only the first tile's is
+// exchanged before its P.  The maximum moves, and O is rescaled, only when it
+// grows by more than 2^8.  Where scores jump from one tile to the next by so much
+// that P, a sum or an O leaves FP32's range (2^128), the row comes out infinite or
+// NaN and is computed again like any that came out NaN, and so is a row whose first
+// tile holds no score above -inf.  32 keys that every row of a warp masks leave P = 0
+// and nothing else.
 //
 // D = 256: 128-key tiles, one CTA an SM (Q, K and V stages fill shared memory,
 // two S buffers and O the tensor memory).  D <= 128: 64-key tiles, two CTAs
@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_begin = abort_flag + 1;  // first key of the tile's first row
   uint32_t* s_nan = tmem_slot + 3;         // [4] rows that came out infinite or NaN
+  uint32_t* s_lost = s_nan + 4;            // [4] rows whose first key tile holds no score above -inf
   float* xbuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);  // softmax parts' exchange
 
   // from a shuffle, so that the compiler knows the warp's index, and what follows from it, to be uniform
@@ -247,6 +248,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     }
     *abort_flag = 0;
     s_nan[0] = s_nan[1] = s_nan[2] = s_nan[3] = 0u;
+    s_lost[0] = s_lost[1] = s_lost[2] = s_lost[3] = 0u;
     fence_barrier_init();
     fence_async_smem();
     // the queries and the first keys wait for nothing
@@ -434,7 +436,6 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     // tiles before the last; l: this part's sum; last: this part's maximum of the last tile
     float m = -INFINITY, l = 0.f, last = -INFINITY;
     const int t_own = (k_end - 1 - w_last) / BK;  // the tile with the warp's own rows' keys: the first it sees
-    int t_exact = n;  // the last tile whose maximum was exchanged before its P (none yet)
     bool ok = true;
     // A failed wait sets `fail`; the two warps of a row leave together, by their
     // next exchange barrier, and the others by their own waits.
@@ -480,52 +481,50 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
           }
         }
       }
-      // O and l against a new maximum; false: a wait failed
-      auto rescale = [&](float mn) -> bool {
-        // 2^(m - mn) in two steps: P_{t-1} may hold up to 2^128, whose inverse is no normal
-        // number.  A P or a sum that overflowed stays infinite or becomes NaN.
-        const float root = mn == -INFINITY ? 1.f : ex2_approx(0.5f * (m - mn));
-        m = mn;  // also where the wait fails: the parts of a row go on deciding alike
-        // O must hold P_{t-1} V_{t-1} before it is rescaled.
-        const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
-        __syncwarp();
-        if (!__all_sync(0xffffffffu, done)) return false;
-        tc_fence_after();
-        l = root == 0.f ? 0.f : l * root * root;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
-#pragma unroll 1
-        for (int c = part * DP; c < (part + 1) * DP; c += 16) {
-          uint32_t o[16];
-          tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * root * root);
-          tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
-        }
-        tmem_wait_st();
-        return true;
-      };
-      // t_exact + 1 follows tiles whose maxima m holds.  A row that has met no score
-      // above -inf has no m to take this tile's P against: its warp exchanges again.
-      const bool exact = t == t_own || (t == t_exact + 1 && __any_sync(0xffffffffu, live && m == -INFINITY));
-      if (exact || t > t_exact + 1) {
-        if (exact) {
-          row_max();
-          xbuf[((t & 1) * NP + part) * 128 + r] = mt;
-        }
+      if (t == t_own) {
+        // the rows' first keys: the parts agree on their maximum at once
+        row_max();
+        xbuf[((t & 1) * NP + part) * 128 + r] = mt;
         if (bar_red_or(4 + q4, 32 * NP, fail)) {
           ok = false;
           break;
         }
-        // otherwise the maximum of the tile before: this one's P may be large
-        const float mn = exact ? fmaxf(fmaxf(m, mt), xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r])
-                               : fmaxf(fmaxf(m, last), xbuf[(((t - 1) & 1) * NP + (part ^ 1)) * 128 + r]);
-        if (exact) t_exact = t;
+        m = fmaxf(mt, xbuf[((t & 1) * NP + (part ^ 1)) * 128 + r]);
+        // nothing to take the next tile's P against: such a row is computed again
+        const unsigned lost = __ballot_sync(0xffffffffu, live && m == -INFINITY);
+        if (lost && lane == 0) s_lost[q4] = lost;
+      } else if (t > t_own + 1) {
+        // later the maximum of the tile before: this one's P may be large
+        if (bar_red_or(4 + q4, 32 * NP, fail)) {
+          ok = false;
+          break;
+        }
+        const float mn = fmaxf(fmaxf(m, last), xbuf[(((t - 1) & 1) * NP + (part ^ 1)) * 128 + r]);
         // the parts of a row see the same m and mn, so they decide alike
-        if (t == t_own) {
-          m = mn;  // the rows' first keys: O holds nothing yet
-        } else if (__any_sync(0xffffffffu, mn > m + 8.f) && !rescale(mn)) {
-          fail = true;
-          continue;
+        if (__any_sync(0xffffffffu, mn > m + 8.f)) {
+          // O must hold P_{t-1} V_{t-1} before it is rescaled.
+          const bool done = mbar_wait(ofull, (t - 1) & 1, a.status, kTimeoutAttention);
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, done)) {
+            fail = true;
+            continue;
+          }
+          tc_fence_after();
+          // 2^(m - mn) in two steps: P_{t-1} may hold up to 2^128, whose inverse is no normal
+          // number.  A P or a sum that overflowed stays infinite or becomes NaN.
+          const float root = mn == -INFINITY ? 1.f : ex2_approx(0.5f * (m - mn));
+          m = mn;
+          l = root == 0.f ? 0.f : l * root * root;  // 0 times a sum that overflowed: only a NaN score makes a NaN sum
+#pragma unroll 1
+          for (int c = part * DP; c < (part + 1) * DP; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(tmem + t_lane + Sh::O_COL + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * root * root);
+            tmem_st16(tmem + t_lane + Sh::O_COL + c, o);
+          }
+          tmem_wait_st();
         }
       }
       // P = exp2(x * scale_log2 - m) as bf16, the operand type of P.V; the row sum keeps the FP32 values
@@ -556,7 +555,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       mbar_arrive(&pfull[s]);
       const float2 sum = unpair2(add2(ps[0], ps[1]));
       l += sum.x + sum.y;
-      if (t > t_exact) {  // for the next tile, while P.V runs
+      if (t > t_own) {  // for the next tile, while P.V runs
         row_max();
         last = mt;
         xbuf[((t & 1) * NP + part) * 128 + r] = mt;
@@ -652,7 +651,7 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
       const float2 odd = unpair2(odd2);
       // a NaN sum has a NaN (or infinite) score of the row's own: the row is NaN, and stays so.
       // One that overflowed and was rescaled to 0 left NaN in O.
-      const bool bad = l == l && (l == INFINITY || odd.x != 0.f || odd.y != 0.f);
+      const bool bad = l == l && (l == INFINITY || odd.x != 0.f || odd.y != 0.f || (s_lost[q4] >> lane & 1u));
       const unsigned bad_rows = __ballot_sync(0xffffffffu, bad && live);
       if (lane == 0 && bad_rows) atomicOr(&s_nan[q4], bad_rows);
       if (D == 64 && whole) fence_async_smem();
