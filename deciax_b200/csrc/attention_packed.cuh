@@ -20,10 +20,10 @@
 // hold a NaN is NaN whatever else it sees: in BF16, and on the CUDA cores, it is
 // left as it came out, and FP32 on the tensor cores, where infinite operands come
 // out NaN too, ends the second pass at the first NaN score (4096 rows of NaN, 16
-// heads of 128: 624 us against 390 of numbers).  Costly is an infinite value among
-// the row's own: one at the start of 4096 rows makes all of them run twice, 11 ms
-// at 16 heads of 256 in BF16 against 0.13, 11 ms at 128 in FP32 against 0.39 (18 ms
-// at 128 in BF16).
+// heads of 128: 650 us against 390 of numbers).  Costly is an infinite value among
+// the row's own: one at the start of 4096 rows makes all of them run twice, 12 ms
+// at 16 heads of 256 in BF16 against 0.13 (15 ms at 128), 13 ms at 128 in FP32
+// against 0.39.
 //
 // attn_packed_simt_kernel (here): FP32 products on the CUDA cores, any head
 // size to 256, any strides and alignment: bf16 rows that TMA cannot read, FP32
@@ -90,18 +90,25 @@ __device__ __forceinline__ float packed_score(float x, float scale, float softca
 // lanes at once, by halves: after the first two exchanges a lane holds the sum
 // of four lanes for one of the keys, `mine` below; after five of 32.  Eight such
 // groups give every lane the score of one of 32 keys.  VEC: rows by 16-byte loads.
+// With `state` the warp takes every `warps`-th 32 keys from its own on and leaves
+// o [256], m and l there, to be joined with the other warps'.
+constexpr int kRedoState = 258;
 template <typename T, bool VEC>
-__device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, int h, int row, int lo) {
+__device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, int h, int row, int lo, int warp, int warps,
+                                                  float* state) {
   const int lane = threadIdx.x & 31, c = lane * 8, hk = h / (a.H / a.Hk);
   const int mine = (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
-  const T* k = a.k + hk * a.hsk + lo * a.ldk;
-  const T* v = a.v + hk * a.hsv + lo * a.ldv;
+  const int step = state ? 32 * warps : 32;  // keys from one turn of this warp to its next
+  if (state) lo += 32 * warp;
   T* out = a.out + row * a.ldo + h * a.hso;
   const float scale = rsqrtf(static_cast<float>(a.d)), inv_cap = inverse_cap(a.softcap);
   float q[8], o[8] = {};
   load8<T, VEC>(a.q + row * a.ldq + h * a.hsq, c, a.d, true, q);
   float m = -INFINITY, l = 0.f;
-  for (int left = row + 1 - lo; left > 0; left -= 32) {
+  for (; lo <= row; lo += step) {
+    const int left = row + 1 - lo;
+    const T* k = a.k + hk * a.hsk + lo * a.ldk;
+    const T* v = a.v + hk * a.hsv + lo * a.ldv;
     const int groups = min(8, (left + 3) / 4);
     float x = 0.f;
 #pragma unroll 1
@@ -130,6 +137,10 @@ __device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, in
     }
     x = 4 * (lane & 7) + mine < left ? packed_score(x, scale, a.softcap, inv_cap) : -INFINITY;
     if (__any_sync(0xffffffffu, x != x)) {  // a NaN score: the row is NaN
+      if (state) {
+        l = __int_as_float(0x7fffffff);
+        break;
+      }
       for (int i = lane; i < a.d; i += 32) out[i] = from_f32<T>(__int_as_float(0x7fffffff));
       return;
     }
@@ -151,6 +162,12 @@ __device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, in
         for (int i = 0; i < 8; ++i) o[i] = fmaf(pj, e[i], o[i]);
       }
   }
+  if (state) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) state[c + i] = o[i];
+    if (lane == 0) state[256] = m, state[257] = l;
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (c + i < a.d) {
@@ -160,15 +177,40 @@ __device__ __noinline__ void attn_packed_redo_row(const AttnPackedArgs<T>& a, in
     }
 }
 
-// The rows q0 + (bits of `rows`) again, `warps` of the block sharing them.
+// The rows of the tile at q0 whose bit in `bad` (32 rows a word) is set, again: a warp
+// a row where there are as many rows as warps, else the warps share each row's
+// keys.  smem: warps * kRedoState floats.  Every thread of the block must call it.
 template <typename T, bool VEC>
-__device__ __forceinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int q0, unsigned long long rows, int warp,
-                                                 int warps) {
-  for (int turn = 0; rows; rows &= rows - 1, ++turn)
-    if (turn % warps == warp) {
-      const int row = q0 + __ffsll(static_cast<long long>(rows)) - 1;
-      attn_packed_redo_row<T, VEC>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1));
+__device__ __noinline__ void attn_packed_redo(const AttnPackedArgs<T>& a, int h, int q0, const uint32_t* bad, int words, float* smem) {
+  const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  int count = 0;
+  for (int w = 0; w < words; ++w) count += __popc(bad[w]);
+  const bool shared = count < warps;
+  uint32_t rows = bad[0];
+  for (int turn = 0, w = 0; turn < count; ++turn, rows &= rows - 1) {
+    while (!rows) rows = bad[++w];
+    if (!shared && turn % warps != warp) continue;
+    const int row = q0 + 32 * w + __ffs(static_cast<int>(rows)) - 1;
+    attn_packed_redo_row<T, VEC>(a, h, row, packed_first_key(a, row, 0, a.n_seqs - 1), warp, warps,
+                                 shared ? smem + warp * kRedoState : nullptr);
+    if (!shared) continue;
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < a.d) {
+      float m = -INFINITY, l = 0.f, o = 0.f;
+      for (int w = 0; w < warps; ++w) m = fmaxf(m, smem[w * kRedoState + 256]);
+      for (int w = 0; w < warps; ++w) {
+        const float* st = smem + w * kRedoState;
+        const float weight = st[256] == -INFINITY ? 0.f : expf(st[256] - m);
+        l = fmaf(weight, st[257], l);
+        o = fmaf(weight, st[c], o);
+      }
+      float y = o / l;
+      if (a.gate) y *= sigmoidf_exact(to_f32(a.gate[row * a.ldg + h * a.hsg + c]));
+      a.out[row * a.ldo + h * a.hso + c] = from_f32<T>(y);
     }
+    __syncthreads();
+  }
 }
 
 // Rows of a tile whose kernel gave up on a wait: NaN, whatever the kernel has
@@ -230,7 +272,7 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
   float* sKV = sQ + BQ * LD;  // the key tile, then the value tile
   float* sP = sKV + BK * LD;
   __shared__ int s_lo[BQ];
-  __shared__ unsigned long long s_nan;
+  __shared__ uint32_t s_nan[2];
 
   int first, total;
   packed_extent(a, first, total);
@@ -243,7 +285,7 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
     const int row = q0 + tid;
     s_lo[tid] = row >= q_first && row < q_end ? packed_first_key(a, row, 0, a.n_seqs - 1) : row + 1;
   }
-  if (tid == 0) s_nan = 0;
+  if (tid < 2) s_nan[tid] = 0u;
   TileOnTheWay<T, DP> way;
   way.load(a.q + h * a.hsq, a.ldq, q0, q_end, a.d, vec);
   way.store(sQ, LD);
@@ -373,10 +415,10 @@ __global__ void __launch_bounds__(256, AttnPackedSimtShape<DP>::CTAS)
       a.out[row * a.ldo + h * a.hso + col] = from_f32<T>(y);
     }
     // a NaN sum has a NaN (or infinite) score of the row's own: the row is NaN, and stays so
-    if (bad && l[i] == l[i]) atomicOr(&s_nan, 1ULL << (ty * 4 + i));
+    if (bad && l[i] == l[i]) atomicOr(&s_nan[ty / 8], 1u << (ty * 4 + i) % 32);
   }
   __syncthreads();
-  attn_packed_redo<T, false>(a, h, q0, s_nan, tid / 32, 8);
+  if (s_nan[0] | s_nan[1]) attn_packed_redo<T, false>(a, h, q0, s_nan, 2, simt_smem);
 }
 
 }  // namespace clef

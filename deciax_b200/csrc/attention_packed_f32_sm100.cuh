@@ -444,12 +444,11 @@ __global__ void __launch_bounds__(AttnPackedF32Shape<D>::THREADS, 1)
     attn_packed_give_up<float, Sh::THREADS>(a, h, q_first, q_end);
     return;
   }
-  for (int half = 0; half < 2; ++half) {
-    const unsigned long long rows = s_nan[2 * half] | static_cast<unsigned long long>(s_nan[2 * half + 1]) << 32;
+  if (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3]) {
     if (vec_in)
-      attn_packed_redo<float, true>(a, h, q0 + 64 * half, rows, warp, Sh::THREADS / 32);
+      attn_packed_redo<float, true>(a, h, q0, s_nan, 4, reinterpret_cast<float*>(sQ));
     else
-      attn_packed_redo<float, false>(a, h, q0 + 64 * half, rows, warp, Sh::THREADS / 32);
+      attn_packed_redo<float, false>(a, h, q0, s_nan, 4, reinterpret_cast<float*>(sQ));
   }
 }
 

@@ -190,6 +190,7 @@ struct AttnPackedTcShape {
   static constexpr size_t SMEM = 1024 + Q_BYTES + 2 * KST * KV_BYTES + 256 + XCH_BYTES;
   static_assert(D + 2 * BK <= 512 && CTAS * TMEM_COLS <= 512, "tensor memory");
   static_assert(Q_BYTES <= KST * KV_BYTES, "the gate tile is loaded into the K stages");
+  static_assert(THREADS / 32 * kRedoState * 4 <= Q_BYTES, "rows computed again join in the Q tile");
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
@@ -687,10 +688,8 @@ __global__ void __launch_bounds__(AttnPackedTcShape<D>::THREADS, AttnPackedTcSha
     attn_packed_give_up<__nv_bfloat16, Sh::THREADS>(a, h, q_first, q_end);
     return;
   }
-  for (int half = 0; half < 2; ++half)
-    attn_packed_redo<__nv_bfloat16, true>(a, h, q0 + 64 * half,
-                                          s_nan[2 * half] | static_cast<unsigned long long>(s_nan[2 * half + 1]) << 32, warp,
-                                          Sh::THREADS / 32);
+  if (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3])
+    attn_packed_redo<__nv_bfloat16, true>(a, h, q0, s_nan, 4, reinterpret_cast<float*>(sQ));
 }
 
 }  // namespace clef

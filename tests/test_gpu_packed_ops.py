@@ -509,7 +509,7 @@ def test_attention_packed_a_prompt_gone_nan(dtype, d):
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("bf16", 256), ("fp32", 128)])
 def test_attention_packed_one_infinite_value_is_no_thousand_passes(dtype, d):
     """Every later row of the prompt is computed once more, as the rows' own keys ask: by warps side by side
-    (one row after the other they took 700 times the plain call at 128 and 1000 at 256; by warps, 40 to 200)."""
+    (one row after the other they took 700 times the plain call at 128 and 1000 at 256; by warps, 50 to 160)."""
     import torch
 
     g = generator(26)
@@ -665,6 +665,31 @@ def test_attention_packed_neighbours_of_any_size(d, dtype):
         out = torch.empty_like(q)
         run_attention(q, k, v, gt, out, cu)
         assert ((out[70:300].double() - y).abs() <= tol + U[dtype] * y.abs()).all(), fill
+
+
+@pytest.mark.parametrize("dtype,d,layout", [("bf16", 64, "split"), ("bf16", 128, "split"), ("bf16", 256, "split"), ("bf16", 72, "odd"),
+                                            ("fp32", 64, "split"), ("fp32", 128, "odd"), ("fp32", 256, "split")])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_attention_packed_some_rows_of_a_tile_are_computed_again(rows, dtype, d, layout):
+    """The first rows of a tile come before a value of their own tile that is infinite and masked for them, and
+    their scores jump by 100: the block's warps share a few such rows' keys, or take a row each."""
+    import torch
+
+    g = generator(30 + rows)
+    bounds, width = [0, 50, 1150, 1220], d + (layout == "odd")
+    q, k, v, gt, out = (normal(g, 1220, h, width, dtype=dtype)[..., width - d :] for h in (4, 2, 2, 4, 4))
+    bad = 7 * 128 + rows
+    v[bad] = float("inf")
+    q.mul_(0.3), k.mul_(0.3)
+    q[:, :, 0], k[:, :, 0] = 16, 0
+    k[70, :, 0] = 100 * d**0.5 / 16
+    run_attention(q, k, v, gt, out, torch.tensor(bounds, dtype=torch.int32, device="cuda"))
+    # weights of 2^-144 beside that key's: 0 times the infinite value is NaN
+    assert not out[bad : bounds[2]].isfinite().any()
+    v[bad] = 0  # nothing before it sees it
+    for a, b in ((0, 50), (50, bad), (1150, 1220)):
+        y, tol = attention_64(q[a:b], k[a:b], v[a:b], gt[a:b], [0, b - a], 0.0, 0, dtype == "bf16")[0, b - a]
+        assert ((out[a:b].double() - y).abs() <= tol + U[dtype] * y.abs()).all(), (a, b)
 
 
 # --------------------------------------------------------------------------- token log probabilities
