@@ -33,8 +33,10 @@
 // 16 heads, gated: one sequence of 16384, d = 256: 1.9 ms under the power cap
 // (1142 TFLOP/s), 1.6 ms alone; records of 600, 16384 rows: 350 us, half of a
 // tile's time outside its key loop; 32 heads of 128, records of 1 to 64, 16001
-// rows: 150 us.  Bound by the tensor pipe on long sequences (62% busy at 8192
+// rows: 150 us.  Bound by the tensor pipe on long sequences (61% busy at 8192
 // rows), at d = 128 by issue slots as much, by a tile's start and end on short ones.
+// A cap costs most beyond its bend: one sequence of 8192, d = 256, 450 us without
+// one, 540 with scores within the series of tanh, 820 beyond it.
 //
 // Differs from attention_sm100.cuh in what bounds a row's keys, and in the
 // rounding: the sigmoid gate multiplies in FP32 and the result is rounded once.

@@ -266,9 +266,12 @@ static void attention_packed(const AttnPackedArgs<T>& a, cudaStream_t st) {
     }
   }
   if constexpr (sizeof(T) == 4) {
-    // Splitting costs a launch: from a few rows on at heads above 64 (16 heads of 128,
-    // 16 rows: 25 us against 31 on the CUDA cores), from two tiles on below
-    // (4 heads of 64, 128 rows: 27 against 25, 192 rows: 27 against 31).
+    // Splitting costs a launch.  Heads above 64 gain from a few rows on: 16 rows, captured,
+    // take 14.4 us against 17.8 on the CUDA cores at 16 heads of 128, 14.7 against 18.2 at 64
+    // (27.8 against 25.1 at 256, where one CTA an SM makes two rounds of the heads).  Heads of
+    // 64, 2 to 64 of them, gain from a second tile of 64 rows on when captured (96 rows: 11
+    // against 14 us), but a program that launches each call pays 2 us for the launch
+    // (128 rows: 27 against 25, 192 rows: 27 against 31).
     if (a.d <= 128 && a.tokens > (a.d <= 64 ? 128 : 8)) {
       const bool cap = a.softcap > 0.f;
       if (a.d <= 64)

@@ -17,9 +17,10 @@
 // head's bytes, cuts it into equal tiles of any multiple of 8 columns, one box
 // each (a last tile in boxes of 16 rows made one row 30 us slower).
 //
-// Vocabulary 256000, dim 3584: 1 row 317 us and 32 rows 333 us, HBM bound (1.835 GB
-// at 5.8 and 5.5 TB/s; a stream of the head with nothing else takes 270 us); 2048
-// rows 2.86 ms, 1316 TFLOP/s, the tensor pipe under the power cap.
+// Vocabulary 256000, dim 3584: 1 row 313 us and 32 rows 324 us, HBM bound (1.835 GB
+// at 5.9 and 5.7 TB/s; a stream of the head with nothing else takes 270 us); 2048
+// rows 2.80 ms, 1341 TFLOP/s, the tensor pipe under the power cap.  Logits beyond
+// the series of tanh (scan32) make 2048 capped rows 3.3 ms, 2.5 within it.
 #pragma once
 
 #include "attention_sm100.cuh"
@@ -329,7 +330,9 @@ __global__ void __launch_bounds__(192, 1)
 //   warps 17..20 thread = row: scan
 //   warp 21      loads the hidden states' three tiles by TMA
 // Bound by shared memory at 128 columns: the products read 192 KB a step, the
-// tiles' writes are 96 KB (2300 cycles at 128 bytes a cycle).
+// tiles' writes are 96 KB (2300 cycles at 128 bytes a cycle).  22 warps leave 80
+// registers a thread: a list of 9 to 32 alternatives spills (500 to 700 bytes), and
+// 97 rows x 32003 x 1024 take 160 us with 20 alternatives in place of 63 with 5.
 // The accumulator cuts off below its last bit at every step, so the five small
 // products, 5 of 6 steps, have an accumulator of their own, 2^-8 as large.
 struct LogprobF32Shape {

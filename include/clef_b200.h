@@ -324,12 +324,17 @@ int clef_op_qk_norm_rope_axes(int dtype, const void* q, int64_t ldq, int64_t hsq
  * read as keys, may hold anything, and their out is left as it was.  Infinities
  * and NaN of one sequence never reach another; the rows that see an infinite one
  * of their own are computed twice, the second time slowly.  out must not overlap
- * the inputs, nor its rows one another.  d <= 256, tokens <= 8388480; bf16 with d % 8 == 0 and 16-byte aligned rows (pointers,
- * ld and hs) runs on the tensor cores, with P rounded to bf16 for P.V; FP32 with d <= 128
- * and more than a few tokens also, every value as three bf16 parts (what is left out of a
- * product is below 2^-24 of it; values below 2^-110 keep fewer bits); anything
- * else on the CUDA cores in FP32.  FP32 takes scratch, 6 bytes an element of q, k and v, from the
- * library's stream-ordered pool: make one such call on each device before capturing one into a graph. */
+ * the inputs, nor its rows one another.  d <= 256, tokens <= 8388480.  bf16 with
+ * d % 8 == 0 and 16-byte aligned rows (pointers, ld and hs) runs on the tensor
+ * cores, with P rounded to bf16 for P.V; FP32 with d <= 128 and more than a few
+ * tokens also, every value as three bf16 parts (what is left out of a product is
+ * below 2^-24 of it; values below 2^-110 keep fewer bits); anything else on the
+ * CUDA cores in FP32.  The tensor cores' sums cut off what lies below the
+ * accumulator's last place, and a capped score there is good to 2e-7 of the cap.
+ * Sums over p v precede the division by the sum of p: values beyond 2^127 divided
+ * by the number of keys may overflow.  FP32 takes scratch, 6 bytes an element of
+ * q, k and v, from the library's stream-ordered pool: make one such call on each
+ * device before capturing one into a graph. */
 int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk,
                              const void* v, int64_t ldv, int64_t hsv, const void* gate, int64_t ldg, int64_t hsg, void* out,
                              int64_t ldo, int64_t hso, const int32_t* cu_seqlens, int n_seqs, int tokens, int hq, int hkv,
@@ -353,9 +358,10 @@ int clef_op_attention_packed(int dtype, const void* q, int64_t ldq, int64_t hsq,
  * alternative: ids behind the last one are -1, their top_logprobs -inf.  16-byte
  * aligned rows (pointers, ldh and ldw, whole 16 bytes of dim) run on the tensor
  * cores, FP32 values as three bf16 parts each (what is left out of a product is
- * below 2^-24 of it, and an infinite value makes its logits NaN); their sums cut
- * off what lies below the accumulator's last place.  Scratch comes from the library's stream-ordered
- * pool: make one call on each device before capturing one into a graph. */
+ * below 2^-24 of it; values below 2^-110 keep fewer bits, and one that is infinite
+ * or beyond 3.39e38 makes its logits NaN); their sums cut off what lies below the
+ * accumulator's last place.  Scratch comes from the library's stream-ordered pool:
+ * make one call on each device before capturing one into a graph. */
 int clef_op_token_logprobs(int dtype, const void* hidden, int64_t ldh, const void* lm_head, int64_t ldw, int rows, int vocab,
                            int dim, float softcap, const int32_t* targets, int n_targets, float* logprobs, float* entropy,
                            int top, int32_t* top_ids, float* top_logprobs, void* stream);
